@@ -145,7 +145,7 @@ extern "C" int dlfx_copy(dlfx_stream_t stream, int dtype, int rank, const int64_
                          void* y, int64_t y_offset, const int64_t* y_strides) {
     if (!x || !y) return DLFX_ERR_INVALID_ARGUMENT;
     if (!view_ok(rank, dims, x_strides) || !view_ok(rank, dims, y_strides)) return DLFX_ERR_INVALID_ARGUMENT;
-    const size_t width = dtype_size(dtype);
+    const size_t width = dtype == DLFX_BF16 ? 2 : dtype_size(dtype);
     if (width == 0) return DLFX_ERR_UNSUPPORTED_DTYPE;
     DimMap2 dm;
     if (!make_dim_map2(rank, dims, x_strides, y_strides, &dm)) return DLFX_ERR_RANK;
@@ -188,7 +188,7 @@ extern "C" int dlfx_fill(dlfx_stream_t stream, int dtype, int rank, const int64_
                          void* x, int64_t x_offset, const void* value) {
     if (!x || !value) return DLFX_ERR_INVALID_ARGUMENT;
     if (!view_ok(rank, dims, strides)) return DLFX_ERR_INVALID_ARGUMENT;
-    const size_t width = dtype_size(dtype);
+    const size_t width = dtype == DLFX_BF16 ? 2 : dtype_size(dtype);
     if (width == 0) return DLFX_ERR_UNSUPPORTED_DTYPE;
     DimMap2 dm;
     if (!make_dim_map2(rank, dims, strides, strides, &dm)) return DLFX_ERR_RANK;

@@ -17,10 +17,13 @@ import numpy as np
 
 from .shape import Shape, ShapeError, norm_axes, norm_axis
 
+# numpy has no bfloat16: its arrays are held as the bits, under a type of their own
+BFLOAT16 = np.dtype([("bfloat16", np.uint16)])
+
 DTYPE_CODES = {np.dtype(np.float32): 0, np.dtype(np.float64): 1,
                np.dtype(np.int32): 2, np.dtype(np.int64): 3,
                np.dtype(np.float16): 4, np.dtype(np.int16): 5, np.dtype(np.bool_): 6,
-               np.dtype(np.complex64): 7, np.dtype(np.complex128): 8}
+               np.dtype(np.complex64): 7, np.dtype(np.complex128): 8, BFLOAT16: 9}
 
 REDUCE_NAMES = ("reduce_sum", "reduce_mean", "reduce_max", "reduce_min", "reduce_log_sum_exp",
                 "reduce_sum_exp", "reduce_log_sum", "reduce_prod", "reduce_asum",
@@ -33,6 +36,20 @@ def dtype_code(dtype) -> int:
         return DTYPE_CODES[np.dtype(dtype)]
     except KeyError:
         raise TypeError("unsupported element type %r" % (dtype,))
+
+
+def to_bfloat16(array) -> np.ndarray:
+    """A float array as BFLOAT16, rounded to nearest, ties to even (a NaN stays one)."""
+    bits = np.ascontiguousarray(array, dtype=np.float32).view(np.uint32)
+    rounded = ((bits + np.uint32(0x7fff) + ((bits >> np.uint32(16)) & np.uint32(1))) >> np.uint32(16)).astype(np.uint16)
+    quiet = ((bits >> np.uint32(16)) | np.uint32(0x40)).astype(np.uint16)
+    nan = (bits & np.uint32(0x7fffffff)) > np.uint32(0x7f800000)
+    return np.ascontiguousarray(np.where(nan, quiet, rounded)).view(BFLOAT16)
+
+
+def from_bfloat16(array: np.ndarray) -> np.ndarray:
+    """A BFLOAT16 array as float32 (exact)."""
+    return (np.ascontiguousarray(array).view(np.uint16).astype(np.uint32) << np.uint32(16)).view(np.float32)
 
 
 class Tensor:
@@ -348,3 +365,273 @@ def hardmax(X: Tensor, axis: int = 1) -> Tensor:
 def gather_elements(X: np.ndarray, I: np.ndarray, axis: int) -> np.ndarray:
     """Host helper of the reference's property tests (reorder_detail.h:190-207)."""
     return np.take_along_axis(X, I.astype(np.int64), axis=axis)
+
+
+# ---------------------------------------------------------------------------
+# sequence-model operators (no counterpart in the reference)
+
+GATE_KINDS = ("gated", "gated_exp", "gated_sigmoid", "gated_blend")
+SCORE_KINDS = ("softmax", "sigmoid")
+SEQUENCE_DTYPES = (np.dtype(np.float32), np.dtype(np.float16), BFLOAT16)
+
+
+def _sequence_dtype(where: str, X: Tensor) -> int:
+    if X.dtype not in SEQUENCE_DTYPES:
+        raise TypeError("%s: float32, float16 or bfloat16 elements, not %r" % (where, X.dtype))
+    return DTYPE_CODES[X.dtype]
+
+
+def _together(where: str, *tensors: Optional[Tensor]) -> None:
+    for T in tensors[1:]:
+        if T is not None and T.backend is not tensors[0].backend:
+            raise ValueError("%s: tensors of different backends" % where)
+
+
+def _like(where: str, what: str, T: Tensor, extents, dtype) -> Tensor:
+    if tuple(T.shape.extents) != tuple(extents):
+        raise ShapeError("%s: %s has extents %s, not %s" % (where, what, list(T.shape.extents), list(extents)))
+    if T.dtype != np.dtype(dtype):
+        raise TypeError("%s: %s has element type %r, not %r" % (where, what, T.dtype, np.dtype(dtype)))
+    return T
+
+
+def _along(shape: Shape, axis: int, reverse: bool) -> Shape:
+    view = shape.moveaxis(axis, -1)
+    return view.flip([-1]) if reverse else view
+
+
+def gated_scan(G: Tensor, X: Tensor, axis: int = -1, kind: str = "gated", reverse: bool = False,
+               initial: Optional[Tensor] = None, last: Optional[Tensor] = None, out: Optional[Tensor] = None):
+    """The gated linear recurrence along `axis` (reverse: from its last element): returns (Y, last).
+
+    kind "gated": h = g h + x; "gated_exp": h = exp(g) h + x; "gated_sigmoid": h = s(g) h + x;
+    "gated_blend": h = s(g) h + (1 - s(g)) x, s the logistic function.  The state is fp32: `initial`
+    (None: zeros) and `last` have X's extents without `axis`; `last` may be the tensor given as
+    `initial` (a decoding step updates its state in place).  G may share gates through strides of 0;
+    `out` may be X or G."""
+    where = "gated_scan(%s)" % kind
+    if kind not in GATE_KINDS:
+        raise ValueError("%s: kind is one of %s" % (where, ", ".join(GATE_KINDS)))
+    code = _sequence_dtype(where, X)
+    _together(where, X, G, initial, last, out)
+    axis = norm_axis(X.rank, axis)
+    extents = X.shape.extents
+    kept = extents[:axis] + extents[axis + 1:]
+    _like(where, "the gate", G, extents, X.dtype)
+    Y = _like(where, "out", out, extents, X.dtype) if out is not None else Tensor.empty(X.backend, extents, X.dtype)
+    if initial is not None:
+        _like(where, "initial", initial, kept, np.float32)
+    L = _like(where, "last", last, kept, np.float32) if last is not None else Tensor.empty(X.backend, kept, np.float32)
+    X.backend.gated_scan(kind, code, _along(G.shape, axis, reverse), G.storage, _along(X.shape, axis, reverse), X.storage,
+                         initial, _along(Y.shape, axis, reverse), Y.storage, L)
+    return Y, L
+
+
+def gated_scan_grad(G: Tensor, X: Optional[Tensor], Y: Tensor, dY: Tensor, axis: int = -1, kind: str = "gated", reverse: bool = False,
+                    initial: Optional[Tensor] = None, dlast: Optional[Tensor] = None):
+    """Gradients (dG, dX, dinitial) of gated_scan for dY and dlast (None: zeros), from the Y that it
+    returned.  Only "gated_blend" reads X (None otherwise will do).  dG has every element of X's
+    extents: where G shares a gate, sum it over the shared axes (reduce_sum)."""
+    where = "gated_scan_grad(%s)" % kind
+    if kind not in GATE_KINDS:
+        raise ValueError("%s: kind is one of %s" % (where, ", ".join(GATE_KINDS)))
+    code = _sequence_dtype(where, Y)
+    _together(where, Y, G, X, dY, initial, dlast)
+    axis = norm_axis(Y.rank, axis)
+    extents = Y.shape.extents
+    kept = extents[:axis] + extents[axis + 1:]
+    _like(where, "the gate", G, extents, Y.dtype)
+    _like(where, "dY", dY, extents, Y.dtype)
+    if X is not None:
+        _like(where, "X", X, extents, Y.dtype)
+    elif kind == "gated_blend":
+        raise ValueError("%s: X is needed" % where)
+    for what, T in (("initial", initial), ("dlast", dlast)):
+        if T is not None:
+            _like(where, what, T, kept, np.float32)
+    dG, dX = Tensor.empty(Y.backend, extents, Y.dtype), Tensor.empty(Y.backend, extents, Y.dtype)
+    dI = Tensor.empty(Y.backend, kept, np.float32)
+    views = [(_along(T.shape, axis, reverse), T.storage) if T is not None else None for T in (G, X, Y, dY, dG, dX)]
+    Y.backend.gated_scan_grad(kind, code, *views, initial, dlast, dI)
+    return dG, dX, dI
+
+
+def _rows(X: Tensor):
+    """(tensor, m, n, row stride) with the last axis contiguous and every other axis merged into
+    rows at one stride; a view that has no such form is copied first."""
+    sh = X.shape
+    if sh.rank == 0:
+        raise ShapeError("rows along the last axis: the tensor has none")
+    n = sh.extents[-1]
+    m = sh.size // n
+    if sh.strides[-1] == 1 or n == 1:
+        stride = size = None
+        for e, s in zip(reversed(sh.extents[:-1]), reversed(sh.strides[:-1])):
+            if e == 1:
+                continue
+            if stride is None:
+                stride, size = s, e
+            elif s == stride * size:
+                size *= e
+            else:
+                break
+        else:
+            if stride is None:
+                return X, m, n, n
+            if stride >= n:
+                return X, m, n, stride
+    return X.contiguous(), m, n, n
+
+
+def _rows_of_output(where: str, X: Tensor, out: Optional[Tensor]):
+    if out is None:
+        out = Tensor.empty(X.backend, X.shape.extents, X.dtype)
+    _like(where, "out", out, X.shape.extents, X.dtype)
+    direct, _, _, stride = _rows(out)
+    if direct is not out:
+        raise ShapeError("%s: out must have a contiguous last axis and rows at one stride" % where)
+    return out, stride
+
+
+def _dense(T: Optional[Tensor]) -> Optional[Tensor]:
+    return T if T is None or T.shape.is_contiguous() else T.contiguous()
+
+
+def _score_kind(where: str, score: str) -> None:
+    if score not in SCORE_KINDS:
+        raise ValueError("%s: score is one of %s" % (where, ", ".join(SCORE_KINDS)))
+
+
+def route(X: Tensor, k: int, score: str = "softmax", bias: Optional[Tensor] = None, groups: int = 1, kept_groups: Optional[int] = None,
+          group_best: int = 1, renormalise: bool = False, scale: float = 1.0, loads: Optional[Tensor] = None):
+    """The k experts of every row of router logits (experts on the last axis): (weights fp32, indices int32),
+    both with k in place of the experts, best first.
+
+    The score is the row's softmax or logistic function; experts are chosen by score + bias (fp32, one per
+    expert), weighed by scale * score, renormalised over the chosen ones on request.  With groups > 1 only the
+    kept_groups groups (neighbouring experts) with the largest sums of their group_best (1 or 2) best choices
+    take part.  loads (int32, one per expert): the number of rows that took each expert is added to it.
+    -inf or the type's lowest value masks an expert."""
+    where = "route(%s)" % score
+    _score_kind(where, score)
+    code = _sequence_dtype(where, X)
+    _together(where, X, bias, loads)
+    rows, m, n, stride = _rows(X)
+    if bias is not None:
+        _like(where, "bias", bias, (n,), np.float32)
+    if loads is not None:
+        _like(where, "loads", loads, (n,), np.int32)
+        if not loads.shape.is_contiguous():
+            raise ShapeError("%s: loads must be contiguous" % where)
+    k = int(k)
+    dims = X.shape.extents[:-1] + (k,)
+    W, I = Tensor.empty(X.backend, dims, np.float32), Tensor.empty(X.backend, dims, np.int32)
+    X.backend.route(score, code, m, n, rows, stride, _dense(bias), int(groups), int(groups if kept_groups is None else kept_groups),
+                    int(group_best), k, bool(renormalise), float(scale), W, I, loads)
+    return W, I
+
+
+def route_grad(X: Tensor, indices: Tensor, dweights: Tensor, score: str = "softmax", renormalise: bool = False, scale: float = 1.0,
+               out: Optional[Tensor] = None) -> Tensor:
+    """Gradient of the logits X for the gradient of route's weights, at the choice `indices` (both with k on the
+    last axis).  out may be X."""
+    where = "route_grad(%s)" % score
+    _score_kind(where, score)
+    code = _sequence_dtype(where, X)
+    _together(where, X, indices, dweights, out)
+    rows, m, n, stride = _rows(X)
+    if indices.rank < 1:
+        raise ShapeError("%s: indices have no axis of choices" % where)
+    dims = X.shape.extents[:-1] + (indices.shape.extents[-1],)
+    _like(where, "indices", indices, dims, np.int32)
+    _like(where, "dweights", dweights, dims, np.float32)
+    dX, dx_stride = _rows_of_output(where, X, out)
+    X.backend.route_grad(score, code, m, n, rows, stride, dims[-1], _dense(indices), _dense(dweights), bool(renormalise), float(scale),
+                         dX, dx_stride)
+    return dX
+
+
+def _targets_of(where: str, X: Tensor, targets: Tensor) -> Tensor:
+    if targets.dtype not in (np.dtype(np.int32), np.dtype(np.int64)):
+        raise TypeError("%s: targets are int32 or int64, not %r" % (where, targets.dtype))
+    return _dense(_like(where, "targets", targets, X.shape.extents[:-1], targets.dtype))
+
+
+def _weights_of(where: str, X: Tensor, weights: Optional[Tensor]) -> Optional[Tensor]:
+    return _dense(_like(where, "weights", weights, X.shape.extents[:-1], np.float32)) if weights is not None else None
+
+
+def cross_entropy(X: Tensor, targets: Tensor, z_loss: float = 0.0) -> Tensor:
+    """Softmax cross entropy (fp32) of every row of logits against its target column: lse - x[target] +
+    z_loss lse^2, lse the logarithm of the row's sum of exponentials.  The last axis is the vocabulary;
+    targets (int32, int64) have the other extents, a negative one takes its row out (loss 0)."""
+    where = "cross_entropy"
+    code = _sequence_dtype(where, X)
+    _together(where, X, targets)
+    rows, m, n, stride = _rows(X)
+    t = _targets_of(where, X, targets)
+    loss = Tensor.empty(X.backend, X.shape.extents[:-1], np.float32)
+    X.backend.cross_entropy(code, dtype_code(t.dtype), m, n, rows, stride, t, float(z_loss), loss)
+    return loss
+
+
+def cross_entropy_grad(X: Tensor, targets: Tensor, weights: Optional[Tensor] = None, z_loss: float = 0.0, out: Optional[Tensor] = None):
+    """(loss, gradient of the logits) of the sum of weights * loss over the rows (weights fp32, None: ones), from one
+    call.  out may be X."""
+    where = "cross_entropy_grad"
+    code = _sequence_dtype(where, X)
+    _together(where, X, targets, weights, out)
+    rows, m, n, stride = _rows(X)
+    t, w = _targets_of(where, X, targets), _weights_of(where, X, weights)
+    loss = Tensor.empty(X.backend, X.shape.extents[:-1], np.float32)
+    dX, dx_stride = _rows_of_output(where, X, out)
+    X.backend.cross_entropy_grad(code, dtype_code(t.dtype), m, n, rows, stride, t, w, float(z_loss), loss, dX, dx_stride)
+    return loss, dX
+
+
+def cross_entropy_piece(X: Tensor, targets: Tensor, first: int, state: Optional[Tensor] = None) -> Tensor:
+    """Folds the logits of columns first, first + 1, ... of a larger vocabulary into the rows' state (None: a new
+    one): [3, rows] fp32, the maxima, the sums of exp(x - maximum), the targets' logits.  Returns the state."""
+    where = "cross_entropy_piece"
+    code = _sequence_dtype(where, X)
+    _together(where, X, targets, state)
+    rows, m, n, stride = _rows(X)
+    t = _targets_of(where, X, targets)
+    resume = state is not None
+    state = _state_of(where, m, state) if resume else Tensor.empty(X.backend, [3, m], np.float32)
+    X.backend.cross_entropy_piece(code, dtype_code(t.dtype), m, n, rows, stride, t, int(first), resume, state)
+    return state
+
+
+def _state_of(where: str, m: int, state: Tensor) -> Tensor:
+    _like(where, "the state", state, (3, m), np.float32)
+    if not state.shape.is_contiguous():
+        raise ShapeError("%s: the state must be contiguous" % where)
+    return state
+
+
+def cross_entropy_join(state: Tensor, targets: Tensor, z_loss: float = 0.0) -> Tensor:
+    """The rows' losses from the state, once every piece of the vocabulary has gone by."""
+    where = "cross_entropy_join"
+    _together(where, state, targets)
+    if targets.dtype not in (np.dtype(np.int32), np.dtype(np.int64)):
+        raise TypeError("%s: targets are int32 or int64, not %r" % (where, targets.dtype))
+    t = _dense(targets)
+    _state_of(where, t.size, state)
+    loss = Tensor.empty(state.backend, targets.shape.extents, np.float32)
+    state.backend.cross_entropy_join(dtype_code(t.dtype), t.size, t, state, float(z_loss), loss)
+    return loss
+
+
+def cross_entropy_piece_grad(X: Tensor, targets: Tensor, first: int, state: Tensor, weights: Optional[Tensor] = None, z_loss: float = 0.0,
+                             out: Optional[Tensor] = None) -> Tensor:
+    """Gradient of a piece's logits from the finished state; see cross_entropy_grad.  out may be X."""
+    where = "cross_entropy_piece_grad"
+    code = _sequence_dtype(where, X)
+    _together(where, X, targets, state, weights, out)
+    rows, m, n, stride = _rows(X)
+    t, w = _targets_of(where, X, targets), _weights_of(where, X, weights)
+    _state_of(where, m, state)
+    dX, dx_stride = _rows_of_output(where, X, out)
+    X.backend.cross_entropy_piece_grad(code, dtype_code(t.dtype), m, n, rows, stride, t, int(first), state, w, float(z_loss), dX, dx_stride)
+    return dX

@@ -8,9 +8,12 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_int, c_int64, c_size_t, c_void_p, POINTER
+from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p, POINTER
 
 import numpy as np
+
+from .frontend import BFLOAT16, Tensor, to_bfloat16
+from .shape import Shape, ShapeError
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libdlfx.so")
@@ -107,6 +110,32 @@ def _declare(lib):
     lib.dlfx_copy.argtypes = [c_void_p, c_int, c_int, _I64P, c_void_p, c_int64, _I64P, c_void_p, c_int64, _I64P]
     lib.dlfx_fill.restype = c_int
     lib.dlfx_fill.argtypes = [c_void_p, c_int, c_int, _I64P, _I64P, c_void_p, c_int64, c_void_p]
+
+    part, scratch, rows = [c_void_p, c_int64, _I64P], [c_void_p, c_size_t], [c_void_p, c_int64, c_int64]
+    lib.dlfx_gated_scan_scratch_bytes.restype = c_size_t
+    lib.dlfx_gated_scan_scratch_bytes.argtypes = [c_int, c_int64, c_int64]
+    lib.dlfx_gated_scan.restype = c_int
+    lib.dlfx_gated_scan.argtypes = [c_void_p, c_char_p, c_int, c_int64, c_int64, c_int, _I64P] + part * 5 + scratch
+    lib.dlfx_gated_scan_grad.restype = c_int
+    lib.dlfx_gated_scan_grad.argtypes = [c_void_p, c_char_p, c_int, c_int64, c_int64, c_int, _I64P] + part * 9 + scratch
+    lib.dlfx_route.restype = c_int
+    lib.dlfx_route.argtypes = ([c_void_p, c_char_p, c_int, c_int64, c_int64] + rows + [c_void_p, c_int64, c_int64, c_int, c_int64, c_int, c_float]
+                               + [c_void_p] * 3)
+    lib.dlfx_route_grad.restype = c_int
+    lib.dlfx_route_grad.argtypes = ([c_void_p, c_char_p, c_int, c_int64, c_int64] + rows + [c_int64, c_void_p, c_void_p, c_int, c_float] + rows)
+    lib.dlfx_cross_entropy_scratch_bytes.restype = c_size_t
+    lib.dlfx_cross_entropy_scratch_bytes.argtypes = [c_int, c_int64, c_int64]
+    matrix = [c_void_p, c_int, c_int, c_int64, c_int64] + rows + [c_void_p]
+    lib.dlfx_cross_entropy.restype = c_int
+    lib.dlfx_cross_entropy.argtypes = matrix + [c_float, c_void_p] + scratch
+    lib.dlfx_cross_entropy_grad.restype = c_int
+    lib.dlfx_cross_entropy_grad.argtypes = matrix + [c_void_p, c_float, c_void_p] + rows + scratch
+    lib.dlfx_cross_entropy_piece.restype = c_int
+    lib.dlfx_cross_entropy_piece.argtypes = matrix + [c_int64, c_int, c_void_p] + scratch
+    lib.dlfx_cross_entropy_join.restype = c_int
+    lib.dlfx_cross_entropy_join.argtypes = [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_float, c_void_p]
+    lib.dlfx_cross_entropy_piece_grad.restype = c_int
+    lib.dlfx_cross_entropy_piece_grad.argtypes = matrix + [c_int64, c_void_p, c_void_p, c_float] + rows
     return lib
 
 
@@ -123,7 +152,10 @@ EXPORTS = ("dlfx_version", "dlfx_status_string", "dlfx_last_hip_error", "dlfx_se
            "dlfx_count_scratch_bytes", "dlfx_count",
            "dlfx_scan_nonzero_scratch_bytes", "dlfx_scan_nonzero", "dlfx_gather_indices",
            "dlfx_merge_scratch_bytes", "dlfx_merge", "dlfx_softmax_scratch_bytes", "dlfx_softmax",
-           "dlfx_copy", "dlfx_fill")
+           "dlfx_copy", "dlfx_fill",
+           "dlfx_gated_scan_scratch_bytes", "dlfx_gated_scan", "dlfx_gated_scan_grad", "dlfx_route", "dlfx_route_grad",
+           "dlfx_cross_entropy_scratch_bytes", "dlfx_cross_entropy", "dlfx_cross_entropy_grad", "dlfx_cross_entropy_piece",
+           "dlfx_cross_entropy_join", "dlfx_cross_entropy_piece_grad")
 
 
 def load_library():
@@ -162,13 +194,14 @@ def _torch_dtype(np_dtype):
                         np.dtype(np.int32): torch.int32, np.dtype(np.int64): torch.int64,
                         np.dtype(np.float16): torch.float16, np.dtype(np.int16): torch.int16,
                         np.dtype(np.bool_): torch.bool,
-                        np.dtype(np.complex64): torch.complex64, np.dtype(np.complex128): torch.complex128}
+                        np.dtype(np.complex64): torch.complex64, np.dtype(np.complex128): torch.complex128,
+                        BFLOAT16: torch.bfloat16}
     return _NP_TO_TORCH[np.dtype(np_dtype)]
 
 
 def _dtype_code_of(torch_dtype, torch):
     return {torch.float32: 0, torch.float64: 1, torch.int32: 2, torch.int64: 3, torch.float16: 4, torch.int16: 5,
-            torch.bool: 6, torch.complex64: 7, torch.complex128: 8}[torch_dtype]
+            torch.bool: 6, torch.complex64: 7, torch.complex128: 8, torch.bfloat16: 9}[torch_dtype]
 
 
 class HipBackend:
@@ -185,15 +218,20 @@ class HipBackend:
         self.lib = load_library()
         self._scratch = None
         self._retired = []
+        self._from_torch_dtype = None
 
     # -- storage ------------------------------------------------------------
     def alloc(self, dtype, count: int):
         return self.torch.empty(max(1, count), dtype=_torch_dtype(dtype), device=self.device)
 
     def upload(self, flat: np.ndarray):
+        if flat.dtype == BFLOAT16:
+            return self.torch.from_numpy(np.ascontiguousarray(flat).view(np.int16)).to(self.device).view(self.torch.bfloat16)
         return self.torch.from_numpy(np.ascontiguousarray(flat)).to(self.device)
 
     def download(self, storage) -> np.ndarray:
+        if storage.dtype == self.torch.bfloat16:
+            return storage.view(self.torch.int16).cpu().numpy().view(BFLOAT16)
         return storage.cpu().numpy()
 
     def copy_view(self, storage, shape):
@@ -216,7 +254,7 @@ class HipBackend:
     def fill(self, dtype, extents, strides, x, x_offset, value, defer=False):
         host_types = {0: np.float32, 1: np.float64, 2: np.int32, 3: np.int64, 4: np.float16, 5: np.int16,
                       6: np.bool_, 7: np.complex64, 8: np.complex128}
-        v = np.array([value], dtype=host_types[dtype])
+        v = to_bfloat16([value]) if dtype == 9 else np.array([value], dtype=host_types[dtype])
         call = self._issue(self.lib.dlfx_fill, "dlfx_fill", (dtype, len(extents), _arr(extents), _arr(strides)),
                            (x.data_ptr(), x_offset, v.ctypes.data_as(c_void_p)), defer, (x,))
         if call is None:
@@ -226,6 +264,37 @@ class HipBackend:
     def wrap(self, tensor):
         """Use an existing contiguous 1-D device tensor as storage."""
         return tensor
+
+    def from_torch(self, tensor) -> Tensor:
+        """A Tensor over the memory of a torch tensor of this backend's device (no copy; any strides)."""
+        if tensor.device != self.device:
+            raise ValueError("the tensor is on %s, this backend on %s" % (tensor.device, self.device))
+        tensor = tensor.detach()
+        shape = Shape(tensor.shape, tensor.stride())
+        if tensor.is_contiguous():
+            storage = tensor.view(-1)
+        else:
+            span = 1 + sum((e - 1) * s for e, s in zip(shape.extents, shape.strides))
+            storage = tensor.as_strided((span,), (1,))
+        return Tensor(self, shape, storage, self._np_dtype(tensor.dtype))
+
+    def to_torch(self, T: Tensor):
+        """The torch view of a Tensor's memory (no copy; torch has no negative strides)."""
+        sh = T.shape
+        if any(s < 0 for s in sh.strides):
+            raise ShapeError("to_torch: a flipped view has no torch form; take contiguous() first")
+        if sh.offset == 0 and sh.size == T.storage.numel() and sh.is_contiguous():
+            return T.storage.view(sh.extents)
+        return T.storage.as_strided(sh.extents, sh.strides, T.storage.storage_offset() + sh.offset)
+
+    def _np_dtype(self, torch_dtype):
+        if self._from_torch_dtype is None:
+            _torch_dtype(np.float32)
+            self._from_torch_dtype = {v: k for k, v in _NP_TO_TORCH.items()}
+        try:
+            return self._from_torch_dtype[torch_dtype]
+        except KeyError:
+            raise TypeError("unsupported element type %r" % (torch_dtype,))
 
     def scratch(self, nbytes: int):
         if nbytes == 0:
@@ -355,6 +424,89 @@ class HipBackend:
                             _arr(ys.extents), _arr(ys.strides), y.data_ptr(), ys.offset,
                             _arr(zs.extents), _arr(zs.strides), z.data_ptr(), zs.offset, sp, sb), defer, (x, y, z))
 
+    # -- sequence-model operators ---------------------------------------------
+    # Scratch is allocated call by call from torch's stream-ordered allocator, so calls on different
+    # streams and recorded graphs never share it.
+    def _call(self, fn, where, *args):
+        torch = self.torch
+        if torch.cuda.current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self._call(fn, where, *args)
+        _check(fn(torch.cuda.current_stream().cuda_stream, *args), where)
+
+    def _call_scratch(self, nbytes):
+        if nbytes == 0:
+            return None, 0, None
+        buffer = self.torch.empty(nbytes, dtype=self.torch.uint8, device=self.device)
+        return buffer.data_ptr(), nbytes, buffer
+
+    @staticmethod
+    def _state_args(T):
+        """Pointer, offset and strides of a tensor of one value per row, or nothing."""
+        return (None, 0, None) if T is None else (T.storage.data_ptr(), T.shape.offset, _arr(T.shape.strides))
+
+    @staticmethod
+    def _start(T):
+        return None if T is None else T.storage.data_ptr() + T.shape.offset * T.storage.element_size()
+
+    def gated_scan(self, kind, dtype, gs, g, xs, x, initial, ys, y, last):
+        where = "dlfx_gated_scan(%s)" % kind
+        n = xs.extents[-1]
+        m = xs.size // n
+        sp, sb, keep = self._call_scratch(self.lib.dlfx_gated_scan_scratch_bytes(dtype, m, n))
+        self._call(self.lib.dlfx_gated_scan, where, kind.encode(), dtype, m, n, xs.rank, _arr(xs.extents),
+                   g.data_ptr(), gs.offset, _arr(gs.strides), x.data_ptr(), xs.offset, _arr(xs.strides), *self._state_args(initial),
+                   y.data_ptr(), ys.offset, _arr(ys.strides), *self._state_args(last), sp, sb)
+
+    def gated_scan_grad(self, kind, dtype, g, x, y, dy, dg, dx, initial, dlast, dinitial):
+        """Every tensor of the call's extents as (axis-moved shape, storage); x may be None."""
+        where = "dlfx_gated_scan_grad(%s)" % kind
+
+        def part(p):
+            return (None, 0, None) if p is None else (p[1].data_ptr(), p[0].offset, _arr(p[0].strides))
+        shape = y[0]
+        n = shape.extents[-1]
+        m = shape.size // n
+        sp, sb, keep = self._call_scratch(self.lib.dlfx_gated_scan_scratch_bytes(dtype, m, n))
+        self._call(self.lib.dlfx_gated_scan_grad, where, kind.encode(), dtype, m, n, shape.rank, _arr(shape.extents),
+                   *part(g), *part(x), *self._state_args(initial), *part(y), *part(dy), *self._state_args(dlast), *part(dg), *part(dx),
+                   *self._state_args(dinitial), sp, sb)
+
+    def route(self, score, dtype, m, n, x, stride, bias, groups, kept_groups, group_best, k, renormalise, scale, weights, indices, loads):
+        where = "dlfx_route(%s)" % score
+        self._call(self.lib.dlfx_route, where, score.encode(), dtype, m, n, x.storage.data_ptr(), x.shape.offset, stride, self._start(bias),
+                   groups, kept_groups, group_best, k, int(renormalise), scale, self._start(weights), self._start(indices), self._start(loads))
+
+    def route_grad(self, score, dtype, m, n, x, stride, k, indices, dweights, renormalise, scale, dx, dx_stride):
+        where = "dlfx_route_grad(%s)" % score
+        self._call(self.lib.dlfx_route_grad, where, score.encode(), dtype, m, n, x.storage.data_ptr(), x.shape.offset, stride, k,
+                   self._start(indices), self._start(dweights), int(renormalise), scale, dx.storage.data_ptr(), dx.shape.offset, dx_stride)
+
+    def cross_entropy(self, dtype, index_dtype, m, n, x, stride, targets, z_loss, loss):
+        sp, sb, keep = self._call_scratch(self.lib.dlfx_cross_entropy_scratch_bytes(dtype, m, n))
+        self._call(self.lib.dlfx_cross_entropy, "dlfx_cross_entropy", dtype, index_dtype, m, n, x.storage.data_ptr(), x.shape.offset, stride,
+                   self._start(targets), z_loss, self._start(loss), sp, sb)
+
+    def cross_entropy_grad(self, dtype, index_dtype, m, n, x, stride, targets, weights, z_loss, loss, dx, dx_stride):
+        sp, sb, keep = self._call_scratch(self.lib.dlfx_cross_entropy_scratch_bytes(dtype, m, n))
+        self._call(self.lib.dlfx_cross_entropy_grad, "dlfx_cross_entropy_grad", dtype, index_dtype, m, n, x.storage.data_ptr(), x.shape.offset,
+                   stride, self._start(targets), self._start(weights), z_loss, self._start(loss), dx.storage.data_ptr(), dx.shape.offset,
+                   dx_stride, sp, sb)
+
+    def cross_entropy_piece(self, dtype, index_dtype, m, n, x, stride, targets, first, resume, state):
+        sp, sb, keep = self._call_scratch(self.lib.dlfx_cross_entropy_scratch_bytes(dtype, m, n))
+        self._call(self.lib.dlfx_cross_entropy_piece, "dlfx_cross_entropy_piece", dtype, index_dtype, m, n, x.storage.data_ptr(), x.shape.offset,
+                   stride, self._start(targets), first, int(resume), self._start(state), sp, sb)
+
+    def cross_entropy_join(self, index_dtype, m, targets, state, z_loss, loss):
+        self._call(self.lib.dlfx_cross_entropy_join, "dlfx_cross_entropy_join", index_dtype, m, self._start(targets), self._start(state), z_loss,
+                   self._start(loss))
+
+    def cross_entropy_piece_grad(self, dtype, index_dtype, m, n, x, stride, targets, first, state, weights, z_loss, dx, dx_stride):
+        self._call(self.lib.dlfx_cross_entropy_piece_grad, "dlfx_cross_entropy_piece_grad", dtype, index_dtype, m, n, x.storage.data_ptr(),
+                   x.shape.offset, stride, self._start(targets), first, self._start(state), self._start(weights), z_loss,
+                   dx.storage.data_ptr(), dx.shape.offset, dx_stride)
+
     def read_element(self, storage, index):
         """One element of a device buffer on the host (synchronises the stream)."""
         return storage[index].item()
@@ -364,3 +516,15 @@ class HipBackend:
 
     def synchronize(self):
         self.torch.cuda.synchronize(self.device)
+
+
+_default = {}
+
+
+def default_backend() -> HipBackend:
+    """The backend of torch's current device, one per device and process."""
+    import torch
+    device = torch.cuda.current_device()
+    if device not in _default:
+        _default[device] = HipBackend("cuda:%d" % device)
+    return _default[device]

@@ -52,7 +52,8 @@ typedef enum dlfx_dtype {
     DLFX_I16 = 5,   /* arg_reduce, sort, argsort, top_k (the reference's int16 instantiations) and merge */
     DLFX_BOOL = 6,  /* one byte per element; input of scan_nonzero only */
     DLFX_C64 = 7,   /* complex of two floats (the reference's float2): reduce, count, scan */
-    DLFX_C128 = 8   /* complex of two doubles (double2): reduce, count, scan */
+    DLFX_C128 = 8,  /* complex of two doubles (double2): reduce, count, scan */
+    DLFX_BF16 = 9   /* bfloat16: gated_scan, route, cross_entropy (fp32 inside, rounded once), copy, fill */
 } dlfx_dtype;
 
 typedef enum dlfx_status {
@@ -324,6 +325,143 @@ int dlfx_copy(dlfx_stream_t stream, int dtype, int rank, const int64_t* dims,
  */
 int dlfx_fill(dlfx_stream_t stream, int dtype, int rank, const int64_t* dims, const int64_t* strides,
               void* x, int64_t x_offset, const void* value);
+
+/* ---------------------------------------------------------------- gated_scan
+ * No counterpart in the reference: a linear recurrence with a gate of its own at every step, the
+ * scan that recurrent layers run over long sequences.  Along the last axis of dims (extent n, m
+ * rows), with the state h in fp32 and h[-1] = initial (NULL: 0):
+ *   name "gated"          h[t] = g[t] h[t-1] + x[t]
+ *        "gated_exp"      h[t] = exp(g[t]) h[t-1] + x[t]                      (g: log of the decay)
+ *        "gated_sigmoid"  h[t] = s(g[t]) h[t-1] + x[t]                        (s: logistic function)
+ *        "gated_blend"    h[t] = s(g[t]) h[t-1] + (1 - s(g[t])) x[t]
+ *   y[t] = h[t] rounded to dtype;  last = h[n-1] in fp32.
+ * gate, x and y share dims and dtype (DLFX_F32, DLFX_F16, DLFX_BF16) and have independent strides;
+ * a stride of 0 on the gate's side shares a gate between elements.  initial and last hold one fp32
+ * value per row: views over the kept dims, rank - 1 strides each, either may be NULL.  A gate that
+ * makes the factor 0 (g = 0, or -inf) starts a new sequence at that step; the arithmetic is the
+ * formula's, so a state that is already infinite or NaN is not forgotten by it.
+ * y may be x or gate (the same pointer, offset and strides), last may be initial: with n == 1 that
+ * is the step of a decoding loop, the state updated in place.  Outputs with a stride of 0 on an
+ * extent above 1 are refused.  The result depends on neither the stream nor the device's load: how
+ * an axis is cut follows from the shapes alone.
+ *
+ * dlfx_gated_scan_grad is its backward pass.  dy, and dlast (fp32 per row, NULL: 0), are the
+ * gradients of y and last; y holds what the forward call wrote, x is read by "gated_blend" alone
+ * (NULL otherwise).  With mu[n] = dlast:
+ *   lam[t] = dy[t] + mu[t+1],  mu[t] = a[t] lam[t],  dinitial = mu[0],
+ *   dx[t] = lam[t]                  ("gated_blend": (1 - a[t]) lam[t])
+ *   dgate[t] = lam[t] y[t-1] a'[t]  ("gated_blend": lam[t] (y[t-1] - x[t]) a'[t]),  y[-1] = initial,
+ * a[t] the factor and a'[t] its derivative by g.  dgate has an element of its own for every
+ * element of dims, also where the gate's stride is 0: its sum over the shared extents is then the
+ * gate's gradient (dlfx_reduce).  dx may be dy, dgate may be gate, dinitial may be dlast; the other
+ * tensors must not overlap the outputs.  dinitial may be NULL.
+ */
+size_t dlfx_gated_scan_scratch_bytes(int dtype, int64_t m, int64_t n);
+int dlfx_gated_scan(dlfx_stream_t stream, const char* name, int dtype, int64_t m, int64_t n,
+                    int rank, const int64_t* dims,
+                    const void* gate, int64_t gate_offset, const int64_t* gate_strides,
+                    const void* x, int64_t x_offset, const int64_t* x_strides,
+                    const float* initial, int64_t initial_offset, const int64_t* initial_strides,
+                    void* y, int64_t y_offset, const int64_t* y_strides,
+                    float* last, int64_t last_offset, const int64_t* last_strides,
+                    void* scratch, size_t scratch_bytes);
+int dlfx_gated_scan_grad(dlfx_stream_t stream, const char* name, int dtype, int64_t m, int64_t n,
+                         int rank, const int64_t* dims,
+                         const void* gate, int64_t gate_offset, const int64_t* gate_strides,
+                         const void* x, int64_t x_offset, const int64_t* x_strides,
+                         const float* initial, int64_t initial_offset, const int64_t* initial_strides,
+                         const void* y, int64_t y_offset, const int64_t* y_strides,
+                         const void* dy, int64_t dy_offset, const int64_t* dy_strides,
+                         const float* dlast, int64_t dlast_offset, const int64_t* dlast_strides,
+                         void* dgate, int64_t dgate_offset, const int64_t* dgate_strides,
+                         void* dx, int64_t dx_offset, const int64_t* dx_strides,
+                         float* dinitial, int64_t dinitial_offset, const int64_t* dinitial_strides,
+                         void* scratch, size_t scratch_bytes);
+
+/* ---------------------------------------------------------------- route
+ * No counterpart in the reference: the choice of k experts for every row (token) of an [m, n]
+ * matrix of router logits.  x: row r at x + x_offset + r * row_stride (row_stride >= n), dtype
+ * DLFX_F32, DLFX_F16 or DLFX_BF16.
+ *   score      name "softmax": s = softmax of the row;  "sigmoid": s = 1 / (1 + exp(-x)).
+ *   choice     by c = s + bias (bias: n fp32 values that balance the load, or NULL); it decides
+ *              which experts are taken and in which order, never what they weigh.
+ *   groups     n / groups neighbouring experts make a group; its value is the sum of its
+ *              group_best (1 or 2) largest c; only the kept_groups best groups take part
+ *              (groups == kept_groups: all do).  kept_groups * (n / groups) >= k.
+ *   indices    [m, k] int32: the k largest c, largest first; the lower index first among equals
+ *              (groups: the lower group).  Values are compared in 64 bits, and without a bias by
+ *              the logits themselves, so that rounding decides nothing.
+ *   weights    [m, k] fp32: scale * s[index], divided by the sum of the row's k chosen s when
+ *              renormalise is not 0 (0 where that sum is 0).
+ *   loads      n int32 counters or NULL: the number of rows that took each expert is ADDED.
+ * An expert whose logit is -inf or the type's lowest finite value is absent in that row: its score
+ * is 0, it comes after every present expert of the kept groups (lower index first), and it adds
+ * nothing to its group's value; a group of absent experts comes last.  A row without any present
+ * expert has weights of 0.  A row that holds a NaN (softmax: or +inf) gets k different valid
+ * indices, in no particular order, and weights that may be NaN.
+ *
+ * dlfx_route_grad writes the gradient of the logits [m, n] for the gradient dweights [m, k] of the
+ * weights, at the choice `indices` (what dlfx_route wrote; a repeated index counts as often as it
+ * stands there, one outside 0 .. n-1 is ignored); dx may be x.
+ * n <= DLFX_ROUTE_MAX_N, k <= DLFX_ROUTE_MAX_K, otherwise DLFX_ERR_TOO_LARGE.
+ */
+#define DLFX_ROUTE_MAX_N 1024
+#define DLFX_ROUTE_MAX_K 64
+int dlfx_route(dlfx_stream_t stream, const char* name, int dtype, int64_t m, int64_t n,
+               const void* x, int64_t x_offset, int64_t row_stride, const float* bias,
+               int64_t groups, int64_t kept_groups, int group_best,
+               int64_t k, int renormalise, float scale,
+               float* weights, int32_t* indices, int32_t* loads);
+int dlfx_route_grad(dlfx_stream_t stream, const char* name, int dtype, int64_t m, int64_t n,
+                    const void* x, int64_t x_offset, int64_t row_stride,
+                    int64_t k, const int32_t* indices, const float* dweights, int renormalise, float scale,
+                    void* dx, int64_t dx_offset, int64_t dx_row_stride);
+
+/* ---------------------------------------------------------------- cross_entropy
+ * No counterpart in the reference: the softmax cross entropy of every row of an [m, n] matrix of
+ * logits against the row's target column, and its gradient.
+ *   loss[r] = lse - x[r, target] + z_loss * lse^2,   lse = log(sum_j exp(x[r, j]))
+ *   dx[r, j] = weights[r] * ((1 + 2 z_loss lse) exp(x[r, j] - lse) - [j == target])
+ * x: row r at x + x_offset + r * row_stride (row_stride >= n), dtype DLFX_F32, DLFX_F16 or
+ * DLFX_BF16, sums in fp32.  targets: m values of index_dtype (DLFX_I32 or DLFX_I64).  A negative
+ * target takes its row out: loss 0, gradient 0, whatever the row holds.  A target beyond the last
+ * column is a mistake that shows: loss NaN, a gradient without the target's term.  weights: m fp32
+ * values or NULL (1 for every row).  -inf masks a column (gradient 0); a row whose every logit is
+ * -inf has loss +inf and gradient 0.  loss: m fp32 values (dlfx_cross_entropy_grad: or NULL).
+ * dx may be x (same offset and stride).
+ *
+ * A vocabulary too large to keep its logits goes by in pieces of columns, each with its own call
+ * as soon as it has been computed; first is the column of the whole that a piece's first column is:
+ *   dlfx_cross_entropy_piece       folds a piece into state, 3 m floats: the running maximum of
+ *                                  every row, then the sums of exp(x - maximum), then the targets'
+ *                                  logits (NaN until their column has gone by).  resume == 0
+ *                                  starts the state anew, whatever it holds.
+ *   dlfx_cross_entropy_join        loss from the state, once every piece has gone by.
+ *   dlfx_cross_entropy_piece_grad  the gradient of a piece, from the finished state: the piece is
+ *                                  computed a second time, or was kept; dx may be x.
+ * The order of the pieces is free, and a state of columns seen elsewhere can be folded in (larger
+ * maximum, sums scaled to it).  Scratch is optional (NULL): few long rows are cut into tiles for the
+ * whole device when scratch of dlfx_cross_entropy_scratch_bytes() bytes is given, and walked by one
+ * workgroup per row when it is not.
+ */
+size_t dlfx_cross_entropy_scratch_bytes(int dtype, int64_t m, int64_t n);
+int dlfx_cross_entropy(dlfx_stream_t stream, int dtype, int index_dtype, int64_t m, int64_t n,
+                       const void* x, int64_t x_offset, int64_t row_stride, const void* targets,
+                       float z_loss, float* loss, void* scratch, size_t scratch_bytes);
+int dlfx_cross_entropy_grad(dlfx_stream_t stream, int dtype, int index_dtype, int64_t m, int64_t n,
+                            const void* x, int64_t x_offset, int64_t row_stride, const void* targets,
+                            const float* weights, float z_loss, float* loss,
+                            void* dx, int64_t dx_offset, int64_t dx_row_stride,
+                            void* scratch, size_t scratch_bytes);
+int dlfx_cross_entropy_piece(dlfx_stream_t stream, int dtype, int index_dtype, int64_t m, int64_t n,
+                             const void* x, int64_t x_offset, int64_t row_stride, const void* targets,
+                             int64_t first, int resume, float* state, void* scratch, size_t scratch_bytes);
+int dlfx_cross_entropy_join(dlfx_stream_t stream, int index_dtype, int64_t m, const void* targets,
+                            const float* state, float z_loss, float* loss);
+int dlfx_cross_entropy_piece_grad(dlfx_stream_t stream, int dtype, int index_dtype, int64_t m, int64_t n,
+                                  const void* x, int64_t x_offset, int64_t row_stride, const void* targets,
+                                  int64_t first, const float* state, const float* weights, float z_loss,
+                                  void* dx, int64_t dx_offset, int64_t dx_row_stride);
 
 #ifdef __cplusplus
 } /* extern "C" */
