@@ -14,7 +14,7 @@ OBJ = os.path.join(CSRC, "obj")
 LIB = os.path.join(HERE, "lib", "libdlfx.so")
 
 # (the longest compilations first; topk_wide.hip and topk_narrow.hip include topk.hip)
-SOURCES = ["topk.hip", "topk_wide.hip", "topk_narrow.hip", "scan.hip", "softmax.hip", "sort.hip", "sort_split.hip", "reduce.hip", "gated_scan.hip",
+SOURCES = ["topk.hip", "topk_wide.hip", "topk_narrow.hip", "scan.hip", "softmax.hip", "sort.hip", "sort_split.hip", "reduce.hip", "gated_scan.hip", "gated_scan_grad.hip",
            "cross_entropy.hip", "route.hip", "lib.hip", "nonzero.hip", "merge.hip", "copy.hip"]
 INCLUDES = {"topk_wide.hip": ["topk.hip"], "topk_narrow.hip": ["topk.hip"]}
 

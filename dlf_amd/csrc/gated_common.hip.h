@@ -1,0 +1,163 @@
+// What the forward and backward gated_scan kernels share: gate functions, the walk over a call's
+// tensors, how a call's axis is cut.
+#pragma once
+
+#include <cstring>
+
+#include "sequence.hip.h"
+
+namespace dlfx {
+namespace {
+
+enum GateKind { kGated = 0, kGatedExp = 1, kGatedSigmoid = 2, kGatedBlend = 3 };
+
+// A tensor of the call: row r starts at base + row.at(r), step t is t * step elements further on.
+template <typename S>
+struct Track {
+    S* base;
+    int64_t step;
+    DimMap row;
+};
+
+// Factor a of the state, and 1 - a (blend: the factor of x; sigmoid and blend: a' = a (1 - a)).
+// The logistic function from e = exp(-|g|) <= 1: the larger of a and 1 - a is 1 / (1 + e), the
+// smaller e / (1 + e), so neither is a difference of nearby numbers and g = +-inf gives 1 and 0.
+template <typename S, int KIND>
+__device__ __forceinline__ void gate_of(float g, float& a, float& keep) {
+    if constexpr (KIND == kGated) {
+        a = g;
+    } else if constexpr (KIND == kGatedExp) {
+        a = fast_exp<S>(g);
+    } else {
+        const float e = fast_exp<S>(-fabsf(g));
+        const float r = fast_reciprocal<S>(1.0f + e);
+        const float small = e * r;
+        a = g < 0.0f ? small : r;
+        keep = g < 0.0f ? r : small;
+    }
+}
+
+// What a stretch of steps does to the state that enters it: h -> a h + b.  The product of many
+// gates can leave the range of fp32 where the states do not (growth from a tiny state, decay of a
+// large one), so it is held in 64 bits; an exact zero stays one under any growth.
+struct Stretch {
+    double a;
+    float b;
+};
+__device__ __forceinline__ float through(const Stretch& s, float h) {
+    return h == 0.0f ? s.b : static_cast<float>(s.a * static_cast<double>(h) + static_cast<double>(s.b));
+}
+__device__ __forceinline__ Stretch join(const Stretch& first, const Stretch& then) { return {first.a * then.a, through(then, first.b)}; }
+
+// V neighbouring elements at base + off bytes.
+template <typename S, int V, typename OFF>
+__device__ __forceinline__ Vec<S, V> load_at(const S* base, OFF off) {
+    if constexpr (sizeof(S) == 2 && V == 1) {
+        return {{bit_cast<S>(__builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(base) + off)))}};
+    } else {
+        constexpr int WORDS = sizeof(S) * V / 4;
+        return bit_cast<Vec<S, V>>(load_stream(reinterpret_cast<const Vec<uint32_t, WORDS>*>(reinterpret_cast<const char*>(base) + off)));
+    }
+}
+template <typename S, int V, typename OFF>
+__device__ __forceinline__ void store_at(S* base, OFF off, const Vec<S, V>& v) {
+    if constexpr (sizeof(S) == 2 && V == 1) {
+        __builtin_nontemporal_store(bit_cast<uint16_t>(v.v[0]), reinterpret_cast<uint16_t*>(reinterpret_cast<char*>(base) + off));
+    } else {
+        constexpr int WORDS = sizeof(S) * V / 4;
+        store_stream(reinterpret_cast<Vec<uint32_t, WORDS>*>(reinterpret_cast<char*>(base) + off), bit_cast<Vec<uint32_t, WORDS>>(v));
+    }
+}
+
+// A wavefront takes 64 groups of V neighbouring rows and S consecutive steps of a pass, W wavefronts
+// share a pass of W * S steps, and a segment of the axis is walked pass by pass.
+struct Cut {
+    int64_t m, n;
+    int64_t blocks;              // groups of 64 V rows
+    int64_t segments, length;    // of the axis; length steps each, the last one shorter
+};
+
+constexpr int kSegmentsMost = 64;
+constexpr int64_t kBlocksWanted = 512;
+
+// How many segments: one while the groups of rows alone give the device its workgroups, otherwise
+// about kBlocksWanted workgroups in all, none shorter than `shortest` steps.
+inline int64_t segments_of(int64_t groups, int64_t n, int64_t shortest, int64_t enough) {
+    if (groups >= enough) return 1;
+    int64_t s = ceil_div(kBlocksWanted, groups);
+    if (s > kSegmentsMost) s = kSegmentsMost;
+    const int64_t most = n / shortest;
+    return s < most ? s : (most < 1 ? 1 : most);
+}
+
+// Scratch of a cut call: what every segment but the last does to the state, and a copy of the
+// states that enter the axis (the tensor they come from may be the one that `last` is written to).
+inline size_t records_bytes(int64_t m, int64_t segments) {
+    return segments > 1 ? align_up(static_cast<size_t>(m * (segments - 1)) * sizeof(Stretch), 256) + static_cast<size_t>(m) * sizeof(float) : 0;
+}
+
+// Byte offsets of the rows fit 32 bits and none is negative: a row's offset rides in one register
+// beside a scalar base.
+template <typename S>
+bool short_offsets(const Track<S>& t) {
+    if (!t.base) return true;
+    unsigned __int128 span = 0;
+    for (int i = 0; i < t.row.rank; ++i) {
+        if (t.row.strides[i] < 0) return false;
+        span += static_cast<unsigned __int128>(t.row.dims[i] - 1) * static_cast<uint64_t>(t.row.strides[i]);
+    }
+    return span * sizeof(S) < (static_cast<unsigned __int128>(1) << 32) - 64;
+}
+// Rows 2 i and 2 i + 1 lie side by side on a boundary of their own size at every step.
+template <typename S>
+bool pairs_of_rows(const Track<S>& t) {
+    if (!t.base) return true;
+    const int r = t.row.rank;
+    if (r == 0 || t.row.strides[r - 1] != 1 || t.row.dims[r - 1] % 2 || t.step % 2) return false;
+    for (int i = 0; i + 1 < r; ++i)
+        if (t.row.strides[i] % 2) return false;
+    return reinterpret_cast<uintptr_t>(t.base) % (2 * sizeof(S)) == 0;
+}
+template <typename S>
+bool side_by_side(const Track<S>& t) {
+    return t.row.rank > 0 && t.row.strides[t.row.rank - 1] == 1;
+}
+
+template <typename S>
+bool make_track(int rank, const int64_t* dims, const void* base, int64_t offset, const int64_t* strides, bool per_row, Track<S>* out) {
+    using E = typename std::remove_const<S>::type;
+    out->base = nullptr;
+    out->step = 0;
+    out->row = DimMap{};
+    if (!base) return true;
+    out->base = const_cast<E*>(static_cast<const E*>(base)) + offset;
+    if (!per_row) out->step = strides[rank - 1];
+    return make_dim_map(dims, strides, 0, rank - 1, &out->row);
+}
+
+inline int kind_of(const char* name) {
+    if (!std::strcmp(name, "gated")) return kGated;
+    if (!std::strcmp(name, "gated_exp")) return kGatedExp;
+    if (!std::strcmp(name, "gated_sigmoid")) return kGatedSigmoid;
+    if (!std::strcmp(name, "gated_blend")) return kGatedBlend;
+    return -1;
+}
+
+template <typename F>
+int dispatch_kind(int kind, F&& f) {
+    switch (kind) {
+    case kGated: return f(std::integral_constant<int, kGated>());
+    case kGatedExp: return f(std::integral_constant<int, kGatedExp>());
+    case kGatedSigmoid: return f(std::integral_constant<int, kGatedSigmoid>());
+    default: return f(std::integral_constant<int, kGatedBlend>());
+    }
+}
+
+inline bool shape_ok(int64_t m, int64_t n, int rank, const int64_t* dims, const int64_t* some_strides) {
+    if (m <= 0 || n <= 0 || rank < 1) return false;
+    if (!view_ok(rank, dims, some_strides)) return false;
+    return dims[rank - 1] == n && view_size(rank - 1, dims) == m;
+}
+
+}  // namespace
+}  // namespace dlfx

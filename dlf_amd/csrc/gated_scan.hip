@@ -1,126 +1,203 @@
-// Gated linear recurrence h[t] = a[t] h[t-1] + b[t] along one axis of strided views, and its
-// backward pass.
-#include <cstring>
-
-#include "sequence.hip.h"
+// Gated linear recurrence h[t] = a[t] h[t-1] + b[t] along one axis of strided views.
+#include "gated_common.hip.h"
 
 namespace dlfx {
 namespace {
 
-enum GateKind { kGated = 0, kGatedExp = 1, kGatedSigmoid = 2, kGatedBlend = 3 };
-
-// Everything of a call that a kernel walks: row r of a tensor starts at base + row.at(r), step t is
-// t * step elements further on.
 template <typename S>
-struct Track {
-    S* base;
-    int64_t step;
-    DimMap row;
+struct ScanCall {
+    Cut cut;
+    Track<const S> g, x;
+    Track<S> y;
+    Track<const float> initial;
+    Track<float> last;
+    Stretch* records;       // cut.segments - 1 per row, segment-major
+    float* entering;        // m states (cut calls)
 };
 
-// Factor a of the state and 1 - a (blend: the factor of x; sigmoid and blend: a' = a (1 - a)).
-// The logistic function from e = exp(-|g|) <= 1: the larger of a and 1 - a is 1 / (1 + e), the
-// smaller e / (1 + e), so neither is a difference of nearby numbers and g = +-inf gives 1 and 0.
+// A short axis: one lane per row, step after step.
 template <typename S, int KIND>
-__device__ __forceinline__ void gate_of(float g, float& a, float& keep) {
-    if constexpr (KIND == kGated) {
-        a = g;
-    } else if constexpr (KIND == kGatedExp) {
-        a = fast_exp<S>(g);
-    } else {
-        const float e = fast_exp<S>(-fabsf(g));
-        const float r = fast_reciprocal<S>(1.0f + e);
-        const float small = e * r;
-        a = g < 0.0f ? small : r;
-        keep = g < 0.0f ? r : small;
-    }
-}
-
-// One lane per row, step after step.
-template <typename S, int KIND>
-__global__ __launch_bounds__(256) void gated_walk(int64_t m, int64_t n, Track<const S> g, Track<const S> x, Track<const float> initial,
-                                                  Track<S> y, Track<float> last) {
+__global__ __launch_bounds__(256) void gated_walk(ScanCall<S> p) {
     const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (r >= m) return;
-    const S* gp = g.base + g.row.at(r);
-    const S* xp = x.base + x.row.at(r);
-    S* yp = y.base + y.row.at(r);
-    float h = initial.base ? initial.base[initial.row.at(r)] : 0.0f;
-    for (int64_t t = 0; t < n; ++t) {
-        float a, keep = 1.0f, b = static_cast<float>(xp[t * x.step]);
-        gate_of<S, KIND>(static_cast<float>(gp[t * g.step]), a, keep);
+    if (r >= p.cut.m) return;
+    const S* gp = p.g.base + p.g.row.at(r);
+    const S* xp = p.x.base + p.x.row.at(r);
+    S* yp = p.y.base + p.y.row.at(r);
+    float h = p.initial.base ? p.initial.base[p.initial.row.at(r)] : 0.0f;
+    for (int64_t t = 0; t < p.cut.n; ++t) {
+        float a, keep = 1.0f, b = static_cast<float>(xp[t * p.x.step]);
+        gate_of<S, KIND>(static_cast<float>(gp[t * p.g.step]), a, keep);
         if constexpr (KIND == kGatedBlend) b *= keep;
         h = fmaf(a, h, b);
-        yp[t * y.step] = static_cast<S>(h);
+        yp[t * p.y.step] = static_cast<S>(h);
     }
-    if (last.base) last.base[last.row.at(r)] = h;
+    if (p.last.base) p.last.base[p.last.row.at(r)] = h;
+}
+
+constexpr int kSteps = 16;       // of a wavefront in a pass
+
+// Rows side by side: lanes run along the rows, wavefronts along the axis.  Every wavefront holds its
+// steps of a pass in registers, leaves what they do to the state in LDS, and walks them again from
+// the state that the wavefronts before it make of the pass's; the next pass is loaded meanwhile.
+// PARTIAL: only what the segment does to the state, for the segments behind it.
+template <typename S, int KIND, int V, int W, typename OFF, bool PARTIAL>
+__global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
+    __shared__ float lds[2][W][kWave][2 * V];
+    const int lane = threadIdx.x % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int64_t segment = PARTIAL ? blockIdx.x / p.cut.blocks : p.cut.segments - 1 - blockIdx.x / p.cut.blocks;
+    const int64_t block = blockIdx.x % p.cut.blocks;
+    const int64_t r = (block * kWave + lane) * V;
+    const bool live = r < p.cut.m;
+    const int64_t rr = live ? r : p.cut.m - V;
+    const OFF go = static_cast<OFF>(p.g.row.at(rr) * static_cast<int64_t>(sizeof(S)));
+    const OFF xo = static_cast<OFF>(p.x.row.at(rr) * static_cast<int64_t>(sizeof(S)));
+    const OFF yo = static_cast<OFF>(p.y.row.at(rr) * static_cast<int64_t>(sizeof(S)));
+    const int64_t begin = segment * p.cut.length;
+    const int64_t end = begin + p.cut.length < p.cut.n ? begin + p.cut.length : p.cut.n;
+
+    float carry[V];
+    double product[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        product[v] = 1.0;
+        carry[v] = 0.0f;
+        if (p.cut.segments == 1 || (PARTIAL && segment == 0)) {
+            const float h = p.initial.base ? p.initial.base[p.initial.row.at(rr + v)] : 0.0f;
+            if constexpr (PARTIAL) {
+                if (wave == 0 && live) p.entering[rr + v] = h;
+            } else {
+                carry[v] = h;
+            }
+        } else if (!PARTIAL) {
+            carry[v] = p.entering[rr + v];
+            for (int64_t s = 0; s < segment; ++s) carry[v] = through(p.records[s * p.cut.m + rr + v], carry[v]);
+        }
+    }
+
+    Vec<S, V> graw[kSteps], xraw[kSteps];
+    auto fetch = [&](int64_t t0) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const int64_t t = t0 + i < end ? t0 + i : end - 1;          // past the end: any step's values, dropped later
+            graw[i] = load_at<S, V>(p.g.base + t * p.g.step, go);
+            xraw[i] = load_at<S, V>(p.x.base + t * p.x.step, xo);
+        }
+    };
+    int64_t t0 = begin + wave * kSteps;
+    fetch(t0);
+    int parity = 0;
+    for (int64_t pass = begin; pass < end; pass += W * kSteps, t0 += W * kSteps, parity ^= 1) {
+        float a[kSteps][V], b[kSteps][V];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float keep = 1.0f;
+                b[i][v] = static_cast<float>(xraw[i].v[v]);
+                gate_of<S, KIND>(static_cast<float>(graw[i].v[v]), a[i][v], keep);
+                if constexpr (KIND == kGatedBlend) b[i][v] *= keep;
+            }
+        }
+        if (t0 + kSteps > end) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                if (t0 + i < end) continue;
+#pragma unroll
+                for (int v = 0; v < V; ++v) a[i][v] = 1.0f, b[i][v] = 0.0f;
+            }
+        }
+        if (pass + W * kSteps < end) fetch(t0 + W * kSteps);
+        float whole_a[V], whole_b[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float pa = a[0][v], h = b[0][v];
+#pragma unroll
+            for (int i = 1; i < kSteps; ++i) {
+                pa *= a[i][v];
+                h = fmaf(a[i][v], h, b[i][v]);
+            }
+            whole_a[v] = pa;
+            whole_b[v] = h;
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            lds[parity][wave][lane][2 * v] = whole_a[v];
+            lds[parity][wave][lane][2 * v + 1] = whole_b[v];
+        }
+        __syncthreads();
+        float h[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float c = carry[v], mine = carry[v];
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                if (w == wave) mine = c;
+                const float wa = lds[parity][w][lane][2 * v];
+                c = fmaf(wa, c, lds[parity][w][lane][2 * v + 1]);
+                if constexpr (PARTIAL) product[v] *= static_cast<double>(wa);
+            }
+            carry[v] = c;
+            h[v] = mine;
+        }
+        if constexpr (!PARTIAL) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                Vec<S, V> out;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    h[v] = fmaf(a[i][v], h[v], b[i][v]);
+                    out.v[v] = static_cast<S>(h[v]);
+                }
+                if (live && t0 + i < end) store_at<S, V>(p.y.base + (t0 + i) * p.y.step, yo, out);
+            }
+        }
+    }
+    if (wave == 0 && live) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if constexpr (PARTIAL) p.records[segment * p.cut.m + r + v] = {product[v], carry[v]};
+            else if (p.last.base && segment == p.cut.segments - 1) p.last.base[p.last.row.at(r + v)] = carry[v];
+        }
+    }
+}
+
+template <typename S, int KIND, int V, int W, typename OFF>
+int launch_cols(ScanCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
+    p.cut.blocks = ceil_div(p.cut.m, kWave * V);
+    int64_t segments = segments_of(p.cut.blocks, p.cut.n, 2 * W * kSteps, 192);
+    if (segments > 1 && (!scratch || scratch_bytes < records_bytes(p.cut.m, segments))) return DLFX_ERR_SCRATCH_TOO_SMALL;
+    p.cut.length = align_up(ceil_div(p.cut.n, segments), W * kSteps);
+    segments = p.cut.segments = ceil_div(p.cut.n, p.cut.length);
+    if (p.cut.blocks * segments > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
+    if (segments > 1) {
+        p.records = static_cast<Stretch*>(scratch);
+        p.entering = reinterpret_cast<float*>(static_cast<char*>(scratch) + align_up(static_cast<size_t>(p.cut.m * (segments - 1)) * sizeof(Stretch), 256));
+        gated_cols<S, KIND, V, W, OFF, true><<<dim3(static_cast<unsigned>(p.cut.blocks * (segments - 1))), dim3(W * kWave), 0, stream>>>(p);
+        DLFX_CHECK_LAUNCH();
+    }
+    gated_cols<S, KIND, V, W, OFF, false><<<dim3(static_cast<unsigned>(p.cut.blocks * segments)), dim3(W * kWave), 0, stream>>>(p);
+    DLFX_CHECK_LAUNCH();
+    return DLFX_OK;
 }
 
 template <typename S, int KIND>
-__global__ __launch_bounds__(256) void gated_grad_walk(int64_t m, int64_t n, Track<const S> g, Track<const S> x, Track<const float> initial,
-                                                       Track<const S> y, Track<const S> dy, Track<const float> dlast,
-                                                       Track<S> dg, Track<S> dx, Track<float> dinitial) {
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (r >= m) return;
-    const S* gp = g.base + g.row.at(r);
-    const S* xp = KIND == kGatedBlend ? x.base + x.row.at(r) : nullptr;
-    const S* yp = y.base + y.row.at(r);
-    const S* dyp = dy.base + dy.row.at(r);
-    S* dgp = dg.base + dg.row.at(r);
-    S* dxp = dx.base + dx.row.at(r);
-    float mu = dlast.base ? dlast.base[dlast.row.at(r)] : 0.0f;
-    const float h0 = initial.base ? initial.base[initial.row.at(r)] : 0.0f;
-    for (int64_t t = n - 1; t >= 0; --t) {
-        float a, keep = 1.0f;
-        gate_of<S, KIND>(static_cast<float>(gp[t * g.step]), a, keep);
-        const float lam = static_cast<float>(dyp[t * dy.step]) + mu;
-        float before = t > 0 ? static_cast<float>(yp[(t - 1) * y.step]) : h0;
-        if constexpr (KIND == kGatedBlend) before -= static_cast<float>(xp[t * x.step]);
-        float d = lam * before;
-        if constexpr (KIND == kGatedExp) d *= a;
-        if constexpr (KIND == kGatedSigmoid || KIND == kGatedBlend) d *= a * keep;
-        mu = a * lam;
-        dgp[t * dg.step] = static_cast<S>(d);
-        dxp[t * dx.step] = static_cast<S>(KIND == kGatedBlend ? lam * keep : lam);
+int launch_scan(const ScanCall<S>& p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
+    const int64_t m = p.cut.m, n = p.cut.n;
+    if (n <= kSteps) {
+        if (ceil_div(m, 256) > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
+        gated_walk<S, KIND><<<dim3(static_cast<unsigned>(ceil_div(m, 256))), dim3(256), 0, stream>>>(p);
+        DLFX_CHECK_LAUNCH();
+        return DLFX_OK;
     }
-    if (dinitial.base) dinitial.base[dinitial.row.at(r)] = mu;
-}
-
-template <typename S>
-bool make_track(int rank, const int64_t* dims, const void* base, int64_t offset, const int64_t* strides, bool per_row, Track<S>* out) {
-    using E = typename std::remove_const<S>::type;
-    out->base = base ? const_cast<S*>(static_cast<const E*>(base) + offset) : nullptr;
-    out->step = 0;
-    if (!base) {
-        out->row.rank = 0;
-        return true;
+    if (!(short_offsets(p.g) && short_offsets(p.x) && short_offsets(p.y)))
+        return launch_cols<S, KIND, 1, 16, int64_t>(p, scratch, scratch_bytes, stream);
+    if (n <= 64) return launch_cols<S, KIND, 1, 4, uint32_t>(p, scratch, scratch_bytes, stream);
+    if constexpr (sizeof(S) == 2) {
+        if (ceil_div(m, 2 * kWave) >= 512 && pairs_of_rows(p.g) && pairs_of_rows(p.x) && pairs_of_rows(p.y))
+            return launch_cols<S, KIND, 2, 8, uint32_t>(p, scratch, scratch_bytes, stream);
     }
-    if (!per_row) out->step = strides[rank - 1];
-    return make_dim_map(dims, strides, 0, rank - 1, &out->row);
-}
-
-int kind_of(const char* name) {
-    if (!std::strcmp(name, "gated")) return kGated;
-    if (!std::strcmp(name, "gated_exp")) return kGatedExp;
-    if (!std::strcmp(name, "gated_sigmoid")) return kGatedSigmoid;
-    if (!std::strcmp(name, "gated_blend")) return kGatedBlend;
-    return -1;
-}
-
-template <typename F>
-int dispatch_kind(int kind, F&& f) {
-    switch (kind) {
-    case kGated: return f(std::integral_constant<int, kGated>());
-    case kGatedExp: return f(std::integral_constant<int, kGatedExp>());
-    case kGatedSigmoid: return f(std::integral_constant<int, kGatedSigmoid>());
-    default: return f(std::integral_constant<int, kGatedBlend>());
-    }
-}
-
-bool shape_ok(int64_t m, int64_t n, int rank, const int64_t* dims, const int64_t* some_strides) {
-    if (m <= 0 || n <= 0 || rank < 1) return false;
-    if (!view_ok(rank, dims, some_strides)) return false;
-    return dims[rank - 1] == n && view_size(rank - 1, dims) == m;
+    return launch_cols<S, KIND, 1, 16, uint32_t>(p, scratch, scratch_bytes, stream);
 }
 
 }  // namespace
@@ -128,7 +205,11 @@ bool shape_ok(int64_t m, int64_t n, int rank, const int64_t* dims, const int64_t
 
 using namespace dlfx;
 
-extern "C" size_t dlfx_gated_scan_scratch_bytes(int, int64_t, int64_t) { return 0; }
+// (an upper bound over every layout of m rows of n steps, forward and backward: the query does not see the strides)
+extern "C" size_t dlfx_gated_scan_scratch_bytes(int dtype, int64_t m, int64_t n) {
+    if (m <= 0 || n <= 0 || (dtype != DLFX_F32 && dtype != DLFX_F16 && dtype != DLFX_BF16)) return 0;
+    return records_bytes(m, segments_of(ceil_div(m, kWave), n, 256, 192));
+}
 
 extern "C" int dlfx_gated_scan(dlfx_stream_t stream, const char* name, int dtype, int64_t m, int64_t n,
                                int rank, const int64_t* dims,
@@ -144,70 +225,18 @@ extern "C" int dlfx_gated_scan(dlfx_stream_t stream, const char* name, int dtype
     if (!shape_ok(m, n, rank, dims, y_strides) || !strides_distinct(rank, dims, y_strides)) return DLFX_ERR_INVALID_ARGUMENT;
     if (rank > 1 && ((initial && !initial_strides) || (last && !last_strides))) return DLFX_ERR_INVALID_ARGUMENT;
     if (last && !strides_distinct(rank - 1, dims, last_strides)) return DLFX_ERR_INVALID_ARGUMENT;
-    (void)scratch; (void)scratch_bytes;
     hipStream_t s = static_cast<hipStream_t>(stream);
     return dispatch_sequence_dtype(dtype, [&](auto tag) {
         using S = decltype(tag);
-        Track<const S> tg, tx;
-        Track<S> ty;
-        Track<const float> ti;
-        Track<float> tl;
-        if (!make_track(rank, dims, gate, gate_offset, gate_strides, false, &tg) || !make_track(rank, dims, x, x_offset, x_strides, false, &tx) ||
-            !make_track(rank, dims, y, y_offset, y_strides, false, &ty) || !make_track(rank, dims, initial, initial_offset, initial_strides, true, &ti) ||
-            !make_track(rank, dims, last, last_offset, last_strides, true, &tl))
+        ScanCall<S> p{};
+        p.cut.m = m;
+        p.cut.n = n;
+        if (!make_track(rank, dims, gate, gate_offset, gate_strides, false, &p.g) || !make_track(rank, dims, x, x_offset, x_strides, false, &p.x) ||
+            !make_track(rank, dims, y, y_offset, y_strides, false, &p.y) ||
+            !make_track(rank, dims, initial, initial_offset, initial_strides, true, &p.initial) ||
+            !make_track(rank, dims, last, last_offset, last_strides, true, &p.last))
             return static_cast<int>(DLFX_ERR_RANK);
-        if (ceil_div(m, 256) > 0x7fffffffLL) return static_cast<int>(DLFX_ERR_TOO_LARGE);
-        return dispatch_kind(kind, [&](auto k) {
-            gated_walk<S, decltype(k)::value><<<dim3(static_cast<unsigned>(ceil_div(m, 256))), dim3(256), 0, s>>>(m, n, tg, tx, ti, ty, tl);
-            DLFX_CHECK_LAUNCH();
-            return static_cast<int>(DLFX_OK);
-        });
+        return dispatch_kind(kind, [&](auto k) { return launch_scan<S, decltype(k)::value>(p, scratch, scratch_bytes, s); });
     });
 }
 
-extern "C" int dlfx_gated_scan_grad(dlfx_stream_t stream, const char* name, int dtype, int64_t m, int64_t n,
-                                    int rank, const int64_t* dims,
-                                    const void* gate, int64_t gate_offset, const int64_t* gate_strides,
-                                    const void* x, int64_t x_offset, const int64_t* x_strides,
-                                    const float* initial, int64_t initial_offset, const int64_t* initial_strides,
-                                    const void* y, int64_t y_offset, const int64_t* y_strides,
-                                    const void* dy, int64_t dy_offset, const int64_t* dy_strides,
-                                    const float* dlast, int64_t dlast_offset, const int64_t* dlast_strides,
-                                    void* dgate, int64_t dgate_offset, const int64_t* dgate_strides,
-                                    void* dx, int64_t dx_offset, const int64_t* dx_strides,
-                                    float* dinitial, int64_t dinitial_offset, const int64_t* dinitial_strides,
-                                    void* scratch, size_t scratch_bytes) {
-    if (!name || !gate || !y || !dy || !dgate || !dx || !gate_strides || !y_strides || !dy_strides || !dgate_strides || !dx_strides)
-        return DLFX_ERR_INVALID_ARGUMENT;
-    const int kind = kind_of(name);
-    if (kind < 0) return DLFX_ERR_UNKNOWN_OP;
-    if (kind == kGatedBlend && (!x || !x_strides)) return DLFX_ERR_INVALID_ARGUMENT;
-    if (!shape_ok(m, n, rank, dims, dx_strides) || !strides_distinct(rank, dims, dx_strides) || !strides_distinct(rank, dims, dgate_strides))
-        return DLFX_ERR_INVALID_ARGUMENT;
-    if (rank > 1 && ((initial && !initial_strides) || (dlast && !dlast_strides) || (dinitial && !dinitial_strides))) return DLFX_ERR_INVALID_ARGUMENT;
-    if (dinitial && !strides_distinct(rank - 1, dims, dinitial_strides)) return DLFX_ERR_INVALID_ARGUMENT;
-    if (kind != kGatedBlend) x = nullptr;
-    (void)scratch; (void)scratch_bytes;
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    return dispatch_sequence_dtype(dtype, [&](auto tag) {
-        using S = decltype(tag);
-        Track<const S> tg, tx, ty, tdy;
-        Track<S> tdg, tdx;
-        Track<const float> ti, tdl;
-        Track<float> tdi;
-        if (!make_track(rank, dims, gate, gate_offset, gate_strides, false, &tg) || !make_track(rank, dims, x, x_offset, x_strides, false, &tx) ||
-            !make_track(rank, dims, y, y_offset, y_strides, false, &ty) || !make_track(rank, dims, dy, dy_offset, dy_strides, false, &tdy) ||
-            !make_track(rank, dims, dgate, dgate_offset, dgate_strides, false, &tdg) || !make_track(rank, dims, dx, dx_offset, dx_strides, false, &tdx) ||
-            !make_track(rank, dims, initial, initial_offset, initial_strides, true, &ti) ||
-            !make_track(rank, dims, dlast, dlast_offset, dlast_strides, true, &tdl) ||
-            !make_track(rank, dims, dinitial, dinitial_offset, dinitial_strides, true, &tdi))
-            return static_cast<int>(DLFX_ERR_RANK);
-        if (ceil_div(m, 256) > 0x7fffffffLL) return static_cast<int>(DLFX_ERR_TOO_LARGE);
-        return dispatch_kind(kind, [&](auto k) {
-            gated_grad_walk<S, decltype(k)::value><<<dim3(static_cast<unsigned>(ceil_div(m, 256))), dim3(256), 0, s>>>(
-                m, n, tg, tx, ti, ty, tdy, tdl, tdg, tdx, tdi);
-            DLFX_CHECK_LAUNCH();
-            return static_cast<int>(DLFX_OK);
-        });
-    });
-}

@@ -1,0 +1,275 @@
+// Backward pass of the gated linear recurrence.
+#include "gated_common.hip.h"
+
+namespace dlfx {
+namespace {
+
+template <typename S>
+struct GradCall {
+    Cut cut;
+    Track<const S> g, x, y, dy;
+    Track<S> dg, dx;
+    Track<const float> initial, dlast;
+    Track<float> dinitial;
+    Stretch* records;
+    float* entering;
+};
+
+// Everything of one step that does not depend on what comes from the steps after it: the factor a,
+// the gradient dy, side = (state before the step) * a' and, for "gated_blend", 1 - a.
+template <typename S, int KIND>
+__device__ __forceinline__ void step_of(float g, float x, float before, float& a, float& keep, float& side) {
+    keep = 1.0f;
+    gate_of<S, KIND>(g, a, keep);
+    if constexpr (KIND == kGatedBlend) before -= x;
+    if constexpr (KIND == kGated) side = before;
+    else if constexpr (KIND == kGatedExp) side = before * a;
+    else side = before * (a * keep);
+}
+
+// A short axis: one lane per row, step after step.
+template <typename S, int KIND>
+__global__ __launch_bounds__(256) void gated_grad_walk(GradCall<S> p) {
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (r >= p.cut.m) return;
+    const S* gp = p.g.base + p.g.row.at(r);
+    const S* xp = KIND == kGatedBlend ? p.x.base + p.x.row.at(r) : nullptr;
+    const S* yp = p.y.base + p.y.row.at(r);
+    const S* dyp = p.dy.base + p.dy.row.at(r);
+    S* dgp = p.dg.base + p.dg.row.at(r);
+    S* dxp = p.dx.base + p.dx.row.at(r);
+    float mu = p.dlast.base ? p.dlast.base[p.dlast.row.at(r)] : 0.0f;
+    const float h0 = p.initial.base ? p.initial.base[p.initial.row.at(r)] : 0.0f;
+    for (int64_t t = p.cut.n - 1; t >= 0; --t) {
+        float a, keep, side;
+        step_of<S, KIND>(static_cast<float>(gp[t * p.g.step]), KIND == kGatedBlend ? static_cast<float>(xp[t * p.x.step]) : 0.0f,
+                         t > 0 ? static_cast<float>(yp[(t - 1) * p.y.step]) : h0, a, keep, side);
+        const float lam = static_cast<float>(dyp[t * p.dy.step]) + mu;
+        mu = a * lam;
+        dgp[t * p.dg.step] = static_cast<S>(lam * side);
+        dxp[t * p.dx.step] = static_cast<S>(KIND == kGatedBlend ? lam * keep : lam);
+    }
+    if (p.dinitial.base) p.dinitial.base[p.dinitial.row.at(r)] = mu;
+}
+
+constexpr int kGradSteps = 8;       // of a wavefront in a pass
+
+// Rows side by side, as in the forward kernel, from the last step to the first: position i of the
+// walk is step n - 1 - i.
+template <typename S, int KIND, int V, int W, typename OFF, bool PARTIAL>
+__global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
+    constexpr int N = kGradSteps;
+    __shared__ float lds[2][W][kWave][2 * V];
+    const int lane = threadIdx.x % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int64_t segment = PARTIAL ? blockIdx.x / p.cut.blocks : p.cut.segments - 1 - blockIdx.x / p.cut.blocks;
+    const int64_t block = blockIdx.x % p.cut.blocks;
+    const int64_t r = (block * kWave + lane) * V;
+    const bool live = r < p.cut.m;
+    const int64_t rr = live ? r : p.cut.m - V;
+    auto offset = [&](const auto& track) { return static_cast<OFF>(track.row.at(rr) * static_cast<int64_t>(sizeof(S))); };
+    const OFF go = offset(p.g), dyo = offset(p.dy);
+    const OFF xo = KIND == kGatedBlend ? offset(p.x) : OFF(0);
+    const OFF yo = offset(p.y), dgo = offset(p.dg), dxo = offset(p.dx);
+    const int64_t begin = segment * p.cut.length;
+    const int64_t end = begin + p.cut.length < p.cut.n ? begin + p.cut.length : p.cut.n;
+    const int64_t top = p.cut.n - 1;
+
+    float carry[V], h0[V];
+    double product[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        product[v] = 1.0;
+        carry[v] = h0[v] = 0.0f;
+        if constexpr (!PARTIAL) {
+            if (segment == p.cut.segments - 1 && p.initial.base) h0[v] = p.initial.base[p.initial.row.at(rr + v)];
+        }
+        if (p.cut.segments == 1 || (PARTIAL && segment == 0)) {
+            const float d = p.dlast.base ? p.dlast.base[p.dlast.row.at(rr + v)] : 0.0f;
+            if constexpr (PARTIAL) {
+                if (wave == 0 && live) p.entering[rr + v] = d;
+            } else {
+                carry[v] = d;
+            }
+        } else if (!PARTIAL) {
+            carry[v] = p.entering[rr + v];
+            for (int64_t s = 0; s < segment; ++s) carry[v] = through(p.records[s * p.cut.m + rr + v], carry[v]);
+        }
+    }
+
+    Vec<S, V> graw[N], dyraw[N], yraw[N], xraw[N];
+    auto fetch = [&](int64_t i0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int64_t t = top - (i0 + i < end ? i0 + i : end - 1);
+            graw[i] = load_at<S, V>(p.g.base + t * p.g.step, go);
+            dyraw[i] = load_at<S, V>(p.dy.base + t * p.dy.step, dyo);
+            if constexpr (!PARTIAL) {
+                yraw[i] = load_at<S, V>(p.y.base + (t > 0 ? t - 1 : 0) * p.y.step, yo);      // (step 0: initial, below)
+                if constexpr (KIND == kGatedBlend) xraw[i] = load_at<S, V>(p.x.base + t * p.x.step, xo);
+            }
+        }
+    };
+    int64_t i0 = begin + wave * N;
+    fetch(i0);
+    int parity = 0;
+    for (int64_t pass = begin; pass < end; pass += W * N, i0 += W * N, parity ^= 1) {
+        float a[N][V], d[N][V], keep[N][V], side[N][V];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                d[i][v] = static_cast<float>(dyraw[i].v[v]);
+                float before = 0.0f, x = 0.0f;
+                if constexpr (!PARTIAL) {
+                    before = i0 + i == top ? h0[v] : static_cast<float>(yraw[i].v[v]);
+                    if constexpr (KIND == kGatedBlend) x = static_cast<float>(xraw[i].v[v]);
+                }
+                step_of<S, KIND>(static_cast<float>(graw[i].v[v]), x, before, a[i][v], keep[i][v], side[i][v]);
+            }
+        }
+        if (i0 + N > end) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (i0 + i < end) continue;
+#pragma unroll
+                for (int v = 0; v < V; ++v) a[i][v] = 1.0f, d[i][v] = 0.0f;
+            }
+        }
+        if (pass + W * N < end) fetch(i0 + W * N);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float pa = a[0][v], mu = a[0][v] * d[0][v];
+#pragma unroll
+            for (int i = 1; i < N; ++i) {
+                pa *= a[i][v];
+                mu = a[i][v] * (d[i][v] + mu);
+            }
+            lds[parity][wave][lane][2 * v] = pa;
+            lds[parity][wave][lane][2 * v + 1] = mu;
+        }
+        __syncthreads();
+        float mu[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float c = carry[v], mine = carry[v];
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                if (w == wave) mine = c;
+                const float wa = lds[parity][w][lane][2 * v];
+                c = fmaf(wa, c, lds[parity][w][lane][2 * v + 1]);
+                if constexpr (PARTIAL) product[v] *= static_cast<double>(wa);
+            }
+            carry[v] = c;
+            mu[v] = mine;
+        }
+        if constexpr (!PARTIAL) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                Vec<S, V> dg, dx;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const float lam = d[i][v] + mu[v];
+                    mu[v] = a[i][v] * lam;
+                    dg.v[v] = static_cast<S>(lam * side[i][v]);
+                    dx.v[v] = static_cast<S>(KIND == kGatedBlend ? lam * keep[i][v] : lam);
+                }
+                if (live && i0 + i < end) {
+                    store_at<S, V>(p.dg.base + (top - i0 - i) * p.dg.step, dgo, dg);
+                    store_at<S, V>(p.dx.base + (top - i0 - i) * p.dx.step, dxo, dx);
+                }
+            }
+        }
+    }
+    if (wave == 0 && live) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if constexpr (PARTIAL) p.records[segment * p.cut.m + r + v] = {product[v], carry[v]};
+            else if (p.dinitial.base && segment == p.cut.segments - 1) p.dinitial.base[p.dinitial.row.at(r + v)] = carry[v];
+        }
+    }
+}
+
+template <typename S, int KIND, int V, int W, typename OFF>
+int launch_cols(GradCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
+    p.cut.blocks = ceil_div(p.cut.m, kWave * V);
+    int64_t segments = segments_of(p.cut.blocks, p.cut.n, 2 * W * kGradSteps, 192);
+    if (segments > 1 && (!scratch || scratch_bytes < records_bytes(p.cut.m, segments))) return DLFX_ERR_SCRATCH_TOO_SMALL;
+    p.cut.length = align_up(ceil_div(p.cut.n, segments), W * kGradSteps);
+    segments = p.cut.segments = ceil_div(p.cut.n, p.cut.length);
+    if (p.cut.blocks * segments > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
+    if (segments > 1) {
+        p.records = static_cast<Stretch*>(scratch);
+        p.entering = reinterpret_cast<float*>(static_cast<char*>(scratch) + align_up(static_cast<size_t>(p.cut.m * (segments - 1)) * sizeof(Stretch), 256));
+        gated_grad_cols<S, KIND, V, W, OFF, true><<<dim3(static_cast<unsigned>(p.cut.blocks * (segments - 1))), dim3(W * kWave), 0, stream>>>(p);
+        DLFX_CHECK_LAUNCH();
+    }
+    gated_grad_cols<S, KIND, V, W, OFF, false><<<dim3(static_cast<unsigned>(p.cut.blocks * segments)), dim3(W * kWave), 0, stream>>>(p);
+    DLFX_CHECK_LAUNCH();
+    return DLFX_OK;
+}
+
+template <typename S, int KIND>
+int launch_grad(const GradCall<S>& p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
+    const int64_t m = p.cut.m, n = p.cut.n;
+    if (n <= 2 * kGradSteps) {
+        if (ceil_div(m, 256) > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
+        gated_grad_walk<S, KIND><<<dim3(static_cast<unsigned>(ceil_div(m, 256))), dim3(256), 0, stream>>>(p);
+        DLFX_CHECK_LAUNCH();
+        return DLFX_OK;
+    }
+    if (!(short_offsets(p.g) && short_offsets(p.x) && short_offsets(p.y) && short_offsets(p.dy) && short_offsets(p.dg) && short_offsets(p.dx)))
+        return launch_cols<S, KIND, 1, 16, int64_t>(p, scratch, scratch_bytes, stream);
+    if (n <= 64) return launch_cols<S, KIND, 1, 4, uint32_t>(p, scratch, scratch_bytes, stream);
+    if constexpr (sizeof(S) == 2) {
+        if (ceil_div(m, 2 * kWave) >= 512 && pairs_of_rows(p.g) && pairs_of_rows(p.x) && pairs_of_rows(p.y) && pairs_of_rows(p.dy) &&
+            pairs_of_rows(p.dg) && pairs_of_rows(p.dx))
+            return launch_cols<S, KIND, 2, 8, uint32_t>(p, scratch, scratch_bytes, stream);
+    }
+    return launch_cols<S, KIND, 1, 16, uint32_t>(p, scratch, scratch_bytes, stream);
+}
+
+}  // namespace
+}  // namespace dlfx
+
+using namespace dlfx;
+
+extern "C" int dlfx_gated_scan_grad(dlfx_stream_t stream, const char* name, int dtype, int64_t m, int64_t n,
+                                    int rank, const int64_t* dims,
+                                    const void* gate, int64_t gate_offset, const int64_t* gate_strides,
+                                    const void* x, int64_t x_offset, const int64_t* x_strides,
+                                    const float* initial, int64_t initial_offset, const int64_t* initial_strides,
+                                    const void* y, int64_t y_offset, const int64_t* y_strides,
+                                    const void* dy, int64_t dy_offset, const int64_t* dy_strides,
+                                    const float* dlast, int64_t dlast_offset, const int64_t* dlast_strides,
+                                    void* dgate, int64_t dgate_offset, const int64_t* dgate_strides,
+                                    void* dx, int64_t dx_offset, const int64_t* dx_strides,
+                                    float* dinitial, int64_t dinitial_offset, const int64_t* dinitial_strides,
+                                    void* scratch, size_t scratch_bytes) {
+    if (!name || !gate || !y || !dy || !dgate || !dx || !gate_strides || !y_strides || !dy_strides || !dgate_strides || !dx_strides)
+        return DLFX_ERR_INVALID_ARGUMENT;
+    const int kind = kind_of(name);
+    if (kind < 0) return DLFX_ERR_UNKNOWN_OP;
+    if (kind == kGatedBlend && (!x || !x_strides)) return DLFX_ERR_INVALID_ARGUMENT;
+    if (!shape_ok(m, n, rank, dims, dx_strides) || !strides_distinct(rank, dims, dx_strides) || !strides_distinct(rank, dims, dgate_strides))
+        return DLFX_ERR_INVALID_ARGUMENT;
+    if (rank > 1 && ((initial && !initial_strides) || (dlast && !dlast_strides) || (dinitial && !dinitial_strides))) return DLFX_ERR_INVALID_ARGUMENT;
+    if (dinitial && !strides_distinct(rank - 1, dims, dinitial_strides)) return DLFX_ERR_INVALID_ARGUMENT;
+    if (kind != kGatedBlend) x = nullptr;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return dispatch_sequence_dtype(dtype, [&](auto tag) {
+        using S = decltype(tag);
+        GradCall<S> p{};
+        p.cut.m = m;
+        p.cut.n = n;
+        if (!make_track(rank, dims, gate, gate_offset, gate_strides, false, &p.g) || !make_track(rank, dims, x, x_offset, x_strides, false, &p.x) ||
+            !make_track(rank, dims, y, y_offset, y_strides, false, &p.y) || !make_track(rank, dims, dy, dy_offset, dy_strides, false, &p.dy) ||
+            !make_track(rank, dims, dgate, dgate_offset, dgate_strides, false, &p.dg) ||
+            !make_track(rank, dims, dx, dx_offset, dx_strides, false, &p.dx) ||
+            !make_track(rank, dims, initial, initial_offset, initial_strides, true, &p.initial) ||
+            !make_track(rank, dims, dlast, dlast_offset, dlast_strides, true, &p.dlast) ||
+            !make_track(rank, dims, dinitial, dinitial_offset, dinitial_strides, true, &p.dinitial))
+            return static_cast<int>(DLFX_ERR_RANK);
+        return dispatch_kind(kind, [&](auto k) { return launch_grad<S, decltype(k)::value>(p, scratch, scratch_bytes, s); });
+    });
+}
