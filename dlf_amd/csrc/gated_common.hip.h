@@ -80,6 +80,78 @@ struct Cut {
 constexpr int kSegmentsMost = 64;
 constexpr int64_t kBlocksWanted = 512;
 
+// ---- rows along memory: a lane takes kRun consecutive positions of its row in two 128-bit accesses
+template <typename S>
+constexpr int run_length() { return 32 / static_cast<int>(sizeof(S)); }
+
+// Positions i0 .. i0 + N - 1 of a row that goes up (DIR 1) or down (DIR -1) in memory from `row`; what
+// lies at or past `end` is left as it is.
+template <int DIR, typename S, int N>
+__device__ __forceinline__ void load_run(const S* row, int64_t i0, int64_t end, S (&out)[N]) {
+    constexpr int V = 16 / static_cast<int>(sizeof(S));
+    using VecT = typename AnyVec<S, V>::type;
+    if (i0 + N <= end) {
+        const S* at = DIR > 0 ? row + i0 : row - i0 - (N - 1);
+#pragma unroll
+        for (int k = 0; k < N; k += V) {
+            const VecT v = *reinterpret_cast<const VecT*>(at + k);
+#pragma unroll
+            for (int e = 0; e < V; ++e) out[DIR > 0 ? k + e : N - 1 - k - e] = v[e];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (i0 + k < end) out[k] = row[DIR * (i0 + k)];
+    }
+}
+template <int DIR, typename S, int N>
+__device__ __forceinline__ void store_run(S* row, int64_t i0, int64_t end, const S (&in)[N]) {
+    constexpr int V = 16 / static_cast<int>(sizeof(S));
+    using VecT = typename AnyVec<S, V>::type;
+    if (i0 + N <= end) {
+        S* at = DIR > 0 ? row + i0 : row - i0 - (N - 1);
+#pragma unroll
+        for (int k = 0; k < N; k += V) {
+            VecT v;
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = in[DIR > 0 ? k + e : N - 1 - k - e];
+            *reinterpret_cast<VecT*>(at + k) = v;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (i0 + k < end) row[DIR * (i0 + k)] = in[k];
+    }
+}
+
+// The stretches of a group of G lanes (16 or 64, in order) joined from the group's first lane up to
+// each; `before` is what lies before the lane, `all` the whole group's.
+template <int G>
+__device__ __forceinline__ void join_lanes(Stretch s, Stretch& before, Stretch& all) {
+    auto step = [&](double pa, float pb) {
+        s.b = through(s, pb);
+        s.a *= pa;
+    };
+    step(dpp_fetch<kRowShr1>(s.a, 1.0), dpp_fetch<kRowShr1>(s.b, 0.0f));
+    step(dpp_fetch<kRowShr2>(s.a, 1.0), dpp_fetch<kRowShr2>(s.b, 0.0f));
+    step(dpp_fetch<kRowShr4>(s.a, 1.0), dpp_fetch<kRowShr4>(s.b, 0.0f));
+    step(dpp_fetch<kRowShr8>(s.a, 1.0), dpp_fetch<kRowShr8>(s.b, 0.0f));
+    if constexpr (G == kWave) {
+        step(dpp_fetch<kRowBcast15, 0xa>(s.a, 1.0), dpp_fetch<kRowBcast15, 0xa>(s.b, 0.0f));
+        step(dpp_fetch<kRowBcast31, 0xc>(s.a, 1.0), dpp_fetch<kRowBcast31, 0xc>(s.b, 0.0f));
+    }
+    const int lane = lane_id();
+    before.a = lane_get(s.a, (lane + kWave - 1) % kWave);
+    before.b = lane_get(s.b, (lane + kWave - 1) % kWave);
+    if (lane % G == 0) before = {1.0, 0.0f};
+    if constexpr (G == kWave) all = {lane_read(s.a, kWave - 1), lane_read(s.b, kWave - 1)};
+    else all = {lane_get(s.a, lane | (G - 1)), lane_get(s.b, lane | (G - 1))};
+}
+
+// +1 or -1 when a track's steps lie one element apart in memory, 0 otherwise.
+template <typename S>
+int direction(const Track<S>& t) { return t.step == 1 ? 1 : t.step == -1 ? -1 : 0; }
+
 // How many segments: one while the groups of rows alone give the device its workgroups, otherwise
 // about kBlocksWanted workgroups in all, none shorter than `shortest` steps.
 inline int64_t segments_of(int64_t groups, int64_t n, int64_t shortest, int64_t enough) {

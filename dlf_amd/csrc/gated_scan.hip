@@ -1,4 +1,6 @@
 // Gated linear recurrence h[t] = a[t] h[t-1] + b[t] along one axis of strided views.
+#include <algorithm>
+
 #include "gated_common.hip.h"
 
 namespace dlfx {
@@ -181,6 +183,135 @@ int launch_cols(ScanCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t 
     return DLFX_OK;
 }
 
+// Rows along memory: G lanes (16 or 64) or W wavefronts per row, a run of consecutive steps to a
+// lane; the lanes' stretches are joined by DPP, the wavefronts' through LDS, pass after pass.
+template <typename S, int KIND, int G, int W, int DIR, bool PARTIAL>
+__global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_rows(ScanCall<S> p) {
+    static_assert(W == 1 || G == kWave, "whole wavefronts share a row");
+    constexpr int N = run_length<S>();
+    constexpr int BLOCK = W > 4 ? W * kWave : 256, TEAM = W * G, TEAMS = BLOCK / TEAM;
+    constexpr int PASS = TEAM * N;
+    __shared__ Stretch lds[W > 1 ? 2 : 1][W > 1 ? TEAMS : 1][W];
+    const int team = threadIdx.x / TEAM, place = threadIdx.x % TEAM, wave = place / kWave;
+    const int64_t segment = PARTIAL ? blockIdx.x / p.cut.blocks : p.cut.segments - 1 - blockIdx.x / p.cut.blocks;
+    const int64_t r = (blockIdx.x % p.cut.blocks) * TEAMS + team;
+    const bool live = r < p.cut.m;
+    const int64_t rr = live ? r : p.cut.m - 1;
+    const S* gp = p.g.base + p.g.row.at(rr);
+    const S* xp = p.x.base + p.x.row.at(rr);
+    S* yp = p.y.base + p.y.row.at(rr);
+    const int64_t begin = segment * p.cut.length;
+    const int64_t end = begin + p.cut.length < p.cut.n ? begin + p.cut.length : p.cut.n;
+
+    float carry = 0.0f;
+    double product = 1.0;
+    if (p.cut.segments == 1 || (PARTIAL && segment == 0)) {
+        const float h = p.initial.base ? p.initial.base[p.initial.row.at(rr)] : 0.0f;
+        if constexpr (PARTIAL) {
+            if (place == 0 && live) p.entering[rr] = h;
+        } else {
+            carry = h;
+        }
+    } else if (!PARTIAL) {
+        carry = p.entering[rr];
+        for (int64_t s = 0; s < segment; ++s) carry = through(p.records[s * p.cut.m + rr], carry);
+    }
+
+    S graw[N], xraw[N];
+    int64_t i0 = begin + place * N;
+    load_run<DIR>(gp, i0, end, graw);
+    load_run<DIR>(xp, i0, end, xraw);
+    int parity = 0;
+    for (int64_t pass = begin; pass < end; pass += PASS, i0 += PASS, parity ^= 1) {
+        float a[N], b[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float keep = 1.0f;
+            b[i] = static_cast<float>(xraw[i]);
+            gate_of<S, KIND>(static_cast<float>(graw[i]), a[i], keep);
+            if constexpr (KIND == kGatedBlend) b[i] *= keep;
+        }
+        if (i0 + N > end) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (i0 + i >= end) a[i] = 1.0f, b[i] = 0.0f;
+        }
+        if (pass + PASS < end) {
+            load_run<DIR>(gp, i0 + PASS, end, graw);
+            load_run<DIR>(xp, i0 + PASS, end, xraw);
+        }
+        float pa = a[0], h = b[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) {
+            pa *= a[i];
+            h = fmaf(a[i], h, b[i]);
+        }
+        Stretch before, all;
+        join_lanes<G>({pa, h}, before, all);
+        float enter = carry;
+        if constexpr (W > 1) {
+            if (lane_id() == 0) lds[parity][team][wave] = all;
+            __syncthreads();
+            float c = carry;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                if (w == wave) enter = c;
+                const Stretch s = lds[parity][team][w];
+                c = through(s, c);
+                if constexpr (PARTIAL) product *= s.a;
+            }
+            carry = c;
+        } else {
+            carry = through(all, carry);
+            if constexpr (PARTIAL) product *= all.a;
+        }
+        if constexpr (!PARTIAL) {
+            h = through(before, enter);
+            S out[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                h = fmaf(a[i], h, b[i]);
+                out[i] = static_cast<S>(h);
+            }
+            if (live) store_run<DIR>(yp, i0, end, out);
+        }
+    }
+    if (place == 0 && live) {
+        if constexpr (PARTIAL) p.records[segment * p.cut.m + r] = {product, carry};
+        else if (p.last.base && segment == p.cut.segments - 1) p.last.base[p.last.row.at(r)] = carry;
+    }
+}
+
+template <typename S, int KIND, int G, int W, int DIR>
+int launch_rows(ScanCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
+    constexpr int BLOCK = W > 4 ? W * kWave : 256, PASS = W * G * run_length<S>();
+    p.cut.blocks = ceil_div(p.cut.m, BLOCK / (W * G));
+    int64_t segments = W > 4 ? segments_of(p.cut.blocks, p.cut.n, PASS, 192) : 1;
+    if (segments > 1 && (!scratch || scratch_bytes < records_bytes(p.cut.m, segments))) return DLFX_ERR_SCRATCH_TOO_SMALL;
+    p.cut.length = align_up(ceil_div(p.cut.n, segments), PASS);
+    segments = p.cut.segments = ceil_div(p.cut.n, p.cut.length);
+    if (p.cut.blocks * segments > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
+    if constexpr (W > 4) {
+        if (segments > 1) {
+            p.records = static_cast<Stretch*>(scratch);
+            p.entering = reinterpret_cast<float*>(static_cast<char*>(scratch) + align_up(static_cast<size_t>(p.cut.m * (segments - 1)) * sizeof(Stretch), 256));
+            gated_rows<S, KIND, G, W, DIR, true><<<dim3(static_cast<unsigned>(p.cut.blocks * (segments - 1))), dim3(BLOCK), 0, stream>>>(p);
+            DLFX_CHECK_LAUNCH();
+        }
+    }
+    gated_rows<S, KIND, G, W, DIR, false><<<dim3(static_cast<unsigned>(p.cut.blocks * segments)), dim3(BLOCK), 0, stream>>>(p);
+    DLFX_CHECK_LAUNCH();
+    return DLFX_OK;
+}
+
+template <typename S, int KIND, int DIR>
+int launch_direction(const ScanCall<S>& p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
+    if (p.cut.n <= 16 * run_length<S>()) return launch_rows<S, KIND, 16, 1, DIR>(p, scratch, scratch_bytes, stream);
+    if (p.cut.m >= 2048) return launch_rows<S, KIND, kWave, 1, DIR>(p, scratch, scratch_bytes, stream);
+    if (p.cut.m >= 512 || p.cut.n <= 4 * kWave * run_length<S>()) return launch_rows<S, KIND, kWave, 4, DIR>(p, scratch, scratch_bytes, stream);
+    return launch_rows<S, KIND, kWave, 16, DIR>(p, scratch, scratch_bytes, stream);
+}
+
 template <typename S, int KIND>
 int launch_scan(const ScanCall<S>& p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     const int64_t m = p.cut.m, n = p.cut.n;
@@ -190,6 +321,9 @@ int launch_scan(const ScanCall<S>& p, void* scratch, size_t scratch_bytes, hipSt
         DLFX_CHECK_LAUNCH();
         return DLFX_OK;
     }
+    const int d = direction(p.y);
+    if (d != 0 && d == direction(p.g) && d == direction(p.x))
+        return d > 0 ? launch_direction<S, KIND, 1>(p, scratch, scratch_bytes, stream) : launch_direction<S, KIND, -1>(p, scratch, scratch_bytes, stream);
     if (!(short_offsets(p.g) && short_offsets(p.x) && short_offsets(p.y)))
         return launch_cols<S, KIND, 1, 16, int64_t>(p, scratch, scratch_bytes, stream);
     if (n <= 64) return launch_cols<S, KIND, 1, 4, uint32_t>(p, scratch, scratch_bytes, stream);
@@ -208,7 +342,7 @@ using namespace dlfx;
 // (an upper bound over every layout of m rows of n steps, forward and backward: the query does not see the strides)
 extern "C" size_t dlfx_gated_scan_scratch_bytes(int dtype, int64_t m, int64_t n) {
     if (m <= 0 || n <= 0 || (dtype != DLFX_F32 && dtype != DLFX_F16 && dtype != DLFX_BF16)) return 0;
-    return records_bytes(m, segments_of(ceil_div(m, kWave), n, 256, 192));
+    return records_bytes(m, std::max(segments_of(ceil_div(m, kWave), n, 256, 192), segments_of(m, n, 8192, 192)));
 }
 
 extern "C" int dlfx_gated_scan(dlfx_stream_t stream, const char* name, int dtype, int64_t m, int64_t n,

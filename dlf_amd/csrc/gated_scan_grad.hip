@@ -209,6 +209,156 @@ int launch_cols(GradCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t 
     return DLFX_OK;
 }
 
+// Rows along memory, as in the forward kernel, from the last step to the first; DIR is the direction
+// of the walk in memory.
+template <typename S, int KIND, int G, int W, int DIR, bool PARTIAL>
+__global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_grad_rows(GradCall<S> p) {
+    static_assert(W == 1 || G == kWave, "whole wavefronts share a row");
+    constexpr int N = run_length<S>();
+    constexpr int BLOCK = W > 4 ? W * kWave : 256, TEAM = W * G, TEAMS = BLOCK / TEAM;
+    constexpr int PASS = TEAM * N;
+    __shared__ Stretch lds[W > 1 ? 2 : 1][W > 1 ? TEAMS : 1][W];
+    const int team = threadIdx.x / TEAM, place = threadIdx.x % TEAM, wave = place / kWave;
+    const int64_t segment = PARTIAL ? blockIdx.x / p.cut.blocks : p.cut.segments - 1 - blockIdx.x / p.cut.blocks;
+    const int64_t r = (blockIdx.x % p.cut.blocks) * TEAMS + team;
+    const bool live = r < p.cut.m;
+    const int64_t rr = live ? r : p.cut.m - 1;
+    const int64_t n = p.cut.n, top = n - 1;
+    // position i of the walk is step n - 1 - i, DIR elements further on in memory each
+    auto start = [&](const auto& track) { return track.base + track.row.at(rr) - DIR * top; };
+    const S* gp = start(p.g);
+    const S* dyp = start(p.dy);
+    const S* xp = KIND == kGatedBlend ? start(p.x) : nullptr;
+    const S* before_p = start(p.y) + DIR;            // the state before position i is the one of position i + 1
+    S* dgp = start(p.dg);
+    S* dxp = start(p.dx);
+    const int64_t begin = segment * p.cut.length;
+    const int64_t end = begin + p.cut.length < n ? begin + p.cut.length : n;
+
+    float carry = 0.0f, h0 = 0.0f;
+    double product = 1.0;
+    if constexpr (!PARTIAL) {
+        if (segment == p.cut.segments - 1 && p.initial.base) h0 = p.initial.base[p.initial.row.at(rr)];
+    }
+    if (p.cut.segments == 1 || (PARTIAL && segment == 0)) {
+        const float d = p.dlast.base ? p.dlast.base[p.dlast.row.at(rr)] : 0.0f;
+        if constexpr (PARTIAL) {
+            if (place == 0 && live) p.entering[rr] = d;
+        } else {
+            carry = d;
+        }
+    } else if (!PARTIAL) {
+        carry = p.entering[rr];
+        for (int64_t s = 0; s < segment; ++s) carry = through(p.records[s * p.cut.m + rr], carry);
+    }
+
+    S graw[N], dyraw[N], yraw[N], xraw[N];
+    auto fetch = [&](int64_t i0) {
+        load_run<DIR>(gp, i0, end, graw);
+        load_run<DIR>(dyp, i0, end, dyraw);
+        if constexpr (!PARTIAL) {
+            load_run<DIR>(before_p, i0, end < top ? end : top, yraw);      // (the last position: initial, below)
+            if constexpr (KIND == kGatedBlend) load_run<DIR>(xp, i0, end, xraw);
+        }
+    };
+    int64_t i0 = begin + place * N;
+    fetch(i0);
+    int parity = 0;
+    for (int64_t pass = begin; pass < end; pass += PASS, i0 += PASS, parity ^= 1) {
+        float a[N], d[N], keep[N], side[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            d[i] = static_cast<float>(dyraw[i]);
+            float before = 0.0f, x = 0.0f;
+            if constexpr (!PARTIAL) {
+                before = i0 + i == top ? h0 : static_cast<float>(yraw[i]);
+                if constexpr (KIND == kGatedBlend) x = static_cast<float>(xraw[i]);
+            }
+            step_of<S, KIND>(static_cast<float>(graw[i]), x, before, a[i], keep[i], side[i]);
+        }
+        if (i0 + N > end) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (i0 + i >= end) a[i] = 1.0f, d[i] = 0.0f;
+        }
+        if (pass + PASS < end) fetch(i0 + PASS);
+        float pa = a[0], mu = a[0] * d[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) {
+            pa *= a[i];
+            mu = a[i] * (d[i] + mu);
+        }
+        Stretch before, all;
+        join_lanes<G>({pa, mu}, before, all);
+        float enter = carry;
+        if constexpr (W > 1) {
+            if (lane_id() == 0) lds[parity][team][wave] = all;
+            __syncthreads();
+            float c = carry;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                if (w == wave) enter = c;
+                const Stretch s = lds[parity][team][w];
+                c = through(s, c);
+                if constexpr (PARTIAL) product *= s.a;
+            }
+            carry = c;
+        } else {
+            carry = through(all, carry);
+            if constexpr (PARTIAL) product *= all.a;
+        }
+        if constexpr (!PARTIAL) {
+            mu = through(before, enter);
+            S dg[N], dx[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float lam = d[i] + mu;
+                mu = a[i] * lam;
+                dg[i] = static_cast<S>(lam * side[i]);
+                dx[i] = static_cast<S>(KIND == kGatedBlend ? lam * keep[i] : lam);
+            }
+            if (live) {
+                store_run<DIR>(dgp, i0, end, dg);
+                store_run<DIR>(dxp, i0, end, dx);
+            }
+        }
+    }
+    if (place == 0 && live) {
+        if constexpr (PARTIAL) p.records[segment * p.cut.m + r] = {product, carry};
+        else if (p.dinitial.base && segment == p.cut.segments - 1) p.dinitial.base[p.dinitial.row.at(r)] = carry;
+    }
+}
+
+template <typename S, int KIND, int G, int W, int DIR>
+int launch_rows(GradCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
+    constexpr int BLOCK = W > 4 ? W * kWave : 256, PASS = W * G * run_length<S>();
+    p.cut.blocks = ceil_div(p.cut.m, BLOCK / (W * G));
+    int64_t segments = W > 4 ? segments_of(p.cut.blocks, p.cut.n, PASS, 192) : 1;
+    if (segments > 1 && (!scratch || scratch_bytes < records_bytes(p.cut.m, segments))) return DLFX_ERR_SCRATCH_TOO_SMALL;
+    p.cut.length = align_up(ceil_div(p.cut.n, segments), PASS);
+    segments = p.cut.segments = ceil_div(p.cut.n, p.cut.length);
+    if (p.cut.blocks * segments > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
+    if constexpr (W > 4) {
+        if (segments > 1) {
+            p.records = static_cast<Stretch*>(scratch);
+            p.entering = reinterpret_cast<float*>(static_cast<char*>(scratch) + align_up(static_cast<size_t>(p.cut.m * (segments - 1)) * sizeof(Stretch), 256));
+            gated_grad_rows<S, KIND, G, W, DIR, true><<<dim3(static_cast<unsigned>(p.cut.blocks * (segments - 1))), dim3(BLOCK), 0, stream>>>(p);
+            DLFX_CHECK_LAUNCH();
+        }
+    }
+    gated_grad_rows<S, KIND, G, W, DIR, false><<<dim3(static_cast<unsigned>(p.cut.blocks * segments)), dim3(BLOCK), 0, stream>>>(p);
+    DLFX_CHECK_LAUNCH();
+    return DLFX_OK;
+}
+
+template <typename S, int KIND, int DIR>
+int launch_direction(const GradCall<S>& p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
+    if (p.cut.n <= 16 * run_length<S>()) return launch_rows<S, KIND, 16, 1, DIR>(p, scratch, scratch_bytes, stream);
+    if (p.cut.m >= 2048) return launch_rows<S, KIND, kWave, 1, DIR>(p, scratch, scratch_bytes, stream);
+    if (p.cut.m >= 512 || p.cut.n <= 4 * kWave * run_length<S>()) return launch_rows<S, KIND, kWave, 4, DIR>(p, scratch, scratch_bytes, stream);
+    return launch_rows<S, KIND, kWave, 16, DIR>(p, scratch, scratch_bytes, stream);
+}
+
 template <typename S, int KIND>
 int launch_grad(const GradCall<S>& p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     const int64_t m = p.cut.m, n = p.cut.n;
@@ -218,6 +368,9 @@ int launch_grad(const GradCall<S>& p, void* scratch, size_t scratch_bytes, hipSt
         DLFX_CHECK_LAUNCH();
         return DLFX_OK;
     }
+    const int d = direction(p.y);
+    if (d != 0 && d == direction(p.g) && d == direction(p.dy) && d == direction(p.dg) && d == direction(p.dx) && (KIND != kGatedBlend || d == direction(p.x)))
+        return d > 0 ? launch_direction<S, KIND, -1>(p, scratch, scratch_bytes, stream) : launch_direction<S, KIND, 1>(p, scratch, scratch_bytes, stream);
     if (!(short_offsets(p.g) && short_offsets(p.x) && short_offsets(p.y) && short_offsets(p.dy) && short_offsets(p.dg) && short_offsets(p.dx)))
         return launch_cols<S, KIND, 1, 16, int64_t>(p, scratch, scratch_bytes, stream);
     if (n <= 64) return launch_cols<S, KIND, 1, 4, uint32_t>(p, scratch, scratch_bytes, stream);

@@ -93,6 +93,7 @@ SHAPES = [
     ((1,), 0), ((5,), 0), ((1, 1, 1), 1), ((3, 1, 70), 1), ((2, 2, 65), 1), ((2, 15, 64), 1), ((1, 16, 3), 1), ((2, 17, 130), 1),
     ((1, 127, 66), 1), ((3, 128, 5), 1), ((1, 257, 192), 1), ((2, 511, 31), 1), ((1, 513, 258), 1), ((1, 2049, 70), 1), ((1, 4500, 8), 1),
     ((4, 7), 1), ((3, 64), 1), ((2, 3, 509), 2), ((5, 513), 1), ((2, 2048), 1), ((3, 2051), 1), ((1, 9001), 1), ((700, 33), 0), ((40, 3, 5, 2), 0),
+    ((2100, 300), 1), ((2, 300, 1100), 2), ((2, 40001), 1), ((1, 20000, 3), 1),
 ]
 
 
@@ -114,7 +115,8 @@ def test_forward_and_gradient(hip_backend, extents, axis, kind, dtype):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("extents,axis", [((2, 1400, 96), 1), ((1, 3000, 7), 1), ((6, 2500), 1), ((1, 700, 4099), 1), ((2, 40, 8200), 1), ((300, 600), 1)])
+@pytest.mark.parametrize("extents,axis", [((2, 1400, 96), 1), ((1, 3000, 7), 1), ((6, 2500), 1), ((1, 700, 4099), 1), ((2, 40, 8200), 1), ((300, 600), 1),
+                                          ((2100, 310), 1), ((3, 33000), 1), ((520, 1100), 1), ((1, 70, 66000), 1)])
 def test_every_kind_and_type(hip_backend, kind, dtype, extents, axis):
     seed = 50 + sum(extents)
     kept = extents[:axis] + extents[axis + 1:]
