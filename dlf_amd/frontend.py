@@ -387,17 +387,28 @@ def _together(where: str, *tensors: Optional[Tensor]) -> None:
             raise ValueError("%s: tensors of different backends" % where)
 
 
-def _like(where: str, what: str, T: Tensor, extents, dtype) -> Tensor:
-    if tuple(T.shape.extents) != tuple(extents):
+def _like(where: str, what: str, T: Tensor, extents: tuple, dtype) -> Tensor:
+    if T.shape.extents != extents:
         raise ShapeError("%s: %s has extents %s, not %s" % (where, what, list(T.shape.extents), list(extents)))
-    if T.dtype != np.dtype(dtype):
+    if T.dtype != dtype:
         raise TypeError("%s: %s has element type %r, not %r" % (where, what, T.dtype, np.dtype(dtype)))
     return T
 
 
-def _along(shape: Shape, axis: int, reverse: bool) -> Shape:
-    view = shape.moveaxis(axis, -1)
-    return view.flip([-1]) if reverse else view
+def _along(T: Tensor, axis: int, reverse: bool):
+    """(storage, offset, strides) of the view with `axis` last, from its other end when reverse."""
+    sh = T.shape
+    st, step = sh.strides, sh.strides[axis]
+    offset = sh.offset
+    if reverse:
+        offset += (sh.extents[axis] - 1) * step
+        step = -step
+    return T.storage, offset, st[:axis] + st[axis + 1:] + (step,)
+
+
+def _new(like: Tensor, extents: tuple, dtype) -> Tensor:
+    shape = Shape.dense(extents)
+    return Tensor(like.backend, shape, like.backend.alloc(dtype, shape.size), dtype)
 
 
 def gated_scan(G: Tensor, X: Tensor, axis: int = -1, kind: str = "gated", reverse: bool = False,
@@ -418,12 +429,12 @@ def gated_scan(G: Tensor, X: Tensor, axis: int = -1, kind: str = "gated", revers
     extents = X.shape.extents
     kept = extents[:axis] + extents[axis + 1:]
     _like(where, "the gate", G, extents, X.dtype)
-    Y = _like(where, "out", out, extents, X.dtype) if out is not None else Tensor.empty(X.backend, extents, X.dtype)
+    Y = _like(where, "out", out, extents, X.dtype) if out is not None else _new(X, extents, X.dtype)
     if initial is not None:
         _like(where, "initial", initial, kept, np.float32)
-    L = _like(where, "last", last, kept, np.float32) if last is not None else Tensor.empty(X.backend, kept, np.float32)
-    X.backend.gated_scan(kind, code, _along(G.shape, axis, reverse), G.storage, _along(X.shape, axis, reverse), X.storage,
-                         initial, _along(Y.shape, axis, reverse), Y.storage, L)
+    L = _like(where, "last", last, kept, np.float32) if last is not None else _new(X, kept, np.float32)
+    X.backend.gated_scan(kind, code, kept + (extents[axis],), _along(G, axis, reverse), _along(X, axis, reverse), initial,
+                         _along(Y, axis, reverse), L)
     return Y, L
 
 
@@ -449,10 +460,10 @@ def gated_scan_grad(G: Tensor, X: Optional[Tensor], Y: Tensor, dY: Tensor, axis:
     for what, T in (("initial", initial), ("dlast", dlast)):
         if T is not None:
             _like(where, what, T, kept, np.float32)
-    dG, dX = Tensor.empty(Y.backend, extents, Y.dtype), Tensor.empty(Y.backend, extents, Y.dtype)
-    dI = Tensor.empty(Y.backend, kept, np.float32)
-    views = [(_along(T.shape, axis, reverse), T.storage) if T is not None else None for T in (G, X, Y, dY, dG, dX)]
-    Y.backend.gated_scan_grad(kind, code, *views, initial, dlast, dI)
+    dG, dX = _new(Y, extents, Y.dtype), _new(Y, extents, Y.dtype)
+    dI = _new(Y, kept, np.float32)
+    views = [_along(T, axis, reverse) if T is not None else None for T in (G, X, Y, dY, dG, dX)]
+    Y.backend.gated_scan_grad(kind, code, kept + (extents[axis],), *views, initial, dlast, dI)
     return dG, dX, dI
 
 
@@ -485,7 +496,7 @@ def _rows(X: Tensor):
 
 def _rows_of_output(where: str, X: Tensor, out: Optional[Tensor]):
     if out is None:
-        out = Tensor.empty(X.backend, X.shape.extents, X.dtype)
+        out = _new(X, X.shape.extents, X.dtype)
     _like(where, "out", out, X.shape.extents, X.dtype)
     direct, _, _, stride = _rows(out)
     if direct is not out:
@@ -525,7 +536,7 @@ def route(X: Tensor, k: int, score: str = "softmax", bias: Optional[Tensor] = No
             raise ShapeError("%s: loads must be contiguous" % where)
     k = int(k)
     dims = X.shape.extents[:-1] + (k,)
-    W, I = Tensor.empty(X.backend, dims, np.float32), Tensor.empty(X.backend, dims, np.int32)
+    W, I = _new(X, dims, np.float32), _new(X, dims, np.int32)
     X.backend.route(score, code, m, n, rows, stride, _dense(bias), int(groups), int(groups if kept_groups is None else kept_groups),
                     int(group_best), k, bool(renormalise), float(scale), W, I, loads)
     return W, I
@@ -570,7 +581,7 @@ def cross_entropy(X: Tensor, targets: Tensor, z_loss: float = 0.0) -> Tensor:
     _together(where, X, targets)
     rows, m, n, stride = _rows(X)
     t = _targets_of(where, X, targets)
-    loss = Tensor.empty(X.backend, X.shape.extents[:-1], np.float32)
+    loss = _new(X, X.shape.extents[:-1], np.float32)
     X.backend.cross_entropy(code, dtype_code(t.dtype), m, n, rows, stride, t, float(z_loss), loss)
     return loss
 
@@ -583,7 +594,7 @@ def cross_entropy_grad(X: Tensor, targets: Tensor, weights: Optional[Tensor] = N
     _together(where, X, targets, weights, out)
     rows, m, n, stride = _rows(X)
     t, w = _targets_of(where, X, targets), _weights_of(where, X, weights)
-    loss = Tensor.empty(X.backend, X.shape.extents[:-1], np.float32)
+    loss = _new(X, X.shape.extents[:-1], np.float32)
     dX, dx_stride = _rows_of_output(where, X, out)
     X.backend.cross_entropy_grad(code, dtype_code(t.dtype), m, n, rows, stride, t, w, float(z_loss), loss, dX, dx_stride)
     return loss, dX
@@ -598,7 +609,7 @@ def cross_entropy_piece(X: Tensor, targets: Tensor, first: int, state: Optional[
     rows, m, n, stride = _rows(X)
     t = _targets_of(where, X, targets)
     resume = state is not None
-    state = _state_of(where, m, state) if resume else Tensor.empty(X.backend, [3, m], np.float32)
+    state = _state_of(where, m, state) if resume else _new(X, (3, m), np.float32)
     X.backend.cross_entropy_piece(code, dtype_code(t.dtype), m, n, rows, stride, t, int(first), resume, state)
     return state
 
@@ -618,7 +629,7 @@ def cross_entropy_join(state: Tensor, targets: Tensor, z_loss: float = 0.0) -> T
         raise TypeError("%s: targets are int32 or int64, not %r" % (where, targets.dtype))
     t = _dense(targets)
     _state_of(where, t.size, state)
-    loss = Tensor.empty(state.backend, targets.shape.extents, np.float32)
+    loss = _new(state, targets.shape.extents, np.float32)
     state.backend.cross_entropy_join(dtype_code(t.dtype), t.size, t, state, float(z_loss), loss)
     return loss
 

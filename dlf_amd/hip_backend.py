@@ -7,6 +7,8 @@ There is no fallback: if the library is missing or a call fails, this raises.
 from __future__ import annotations
 
 import ctypes
+import functools
+import math
 import os
 from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p, POINTER
 
@@ -174,6 +176,12 @@ def _arr(values):
     return (c_int64 * max(1, len(values)))(*values)
 
 
+@functools.lru_cache(maxsize=4096)
+def _const(values: tuple):
+    """A C array of extents or strides that a call only reads."""
+    return (c_int64 * max(1, len(values)))(*values)
+
+
 def _check(status: int, where: str):
     if status != 0:
         lib = load_library()
@@ -188,8 +196,8 @@ _NP_TO_TORCH = None
 
 def _torch_dtype(np_dtype):
     global _NP_TO_TORCH
-    import torch
     if _NP_TO_TORCH is None:
+        import torch
         _NP_TO_TORCH = {np.dtype(np.float32): torch.float32, np.dtype(np.float64): torch.float64,
                         np.dtype(np.int32): torch.int32, np.dtype(np.int64): torch.int64,
                         np.dtype(np.float16): torch.float16, np.dtype(np.int16): torch.int16,
@@ -222,7 +230,7 @@ class HipBackend:
 
     # -- storage ------------------------------------------------------------
     def alloc(self, dtype, count: int):
-        return self.torch.empty(max(1, count), dtype=_torch_dtype(dtype), device=self.device)
+        return self.torch.empty(count or 1, dtype=_torch_dtype(dtype), device=self.device)
 
     def upload(self, flat: np.ndarray):
         if flat.dtype == BFLOAT16:
@@ -269,22 +277,22 @@ class HipBackend:
         """A Tensor over the memory of a torch tensor of this backend's device (no copy; any strides)."""
         if tensor.device != self.device:
             raise ValueError("the tensor is on %s, this backend on %s" % (tensor.device, self.device))
-        tensor = tensor.detach()
-        shape = Shape(tensor.shape, tensor.stride())
+        if tensor.requires_grad:
+            tensor = tensor.detach()
+        extents, strides = tuple(tensor.shape), tensor.stride()
+        if 0 in extents:
+            raise ShapeError("extent must be positive")
         if tensor.is_contiguous():
             storage = tensor.view(-1)
         else:
-            span = 1 + sum((e - 1) * s for e, s in zip(shape.extents, shape.strides))
-            storage = tensor.as_strided((span,), (1,))
-        return Tensor(self, shape, storage, self._np_dtype(tensor.dtype))
+            storage = tensor.as_strided((1 + sum((e - 1) * s for e, s in zip(extents, strides)),), (1,))
+        return Tensor(self, Shape.of(extents, strides), storage, self._np_dtype(tensor.dtype))
 
     def to_torch(self, T: Tensor):
         """The torch view of a Tensor's memory (no copy; torch has no negative strides)."""
         sh = T.shape
-        if any(s < 0 for s in sh.strides):
+        if sh.strides and min(sh.strides) < 0:
             raise ShapeError("to_torch: a flipped view has no torch form; take contiguous() first")
-        if sh.offset == 0 and sh.size == T.storage.numel() and sh.is_contiguous():
-            return T.storage.view(sh.extents)
         return T.storage.as_strided(sh.extents, sh.strides, T.storage.storage_offset() + sh.offset)
 
     def _np_dtype(self, torch_dtype):
@@ -429,7 +437,7 @@ class HipBackend:
     # streams and recorded graphs never share it.
     def _call(self, fn, where, *args):
         torch = self.torch
-        if torch.cuda.current_device() != self.device.index:
+        if torch.cuda.current_device() != (self.device.index or 0):
             with torch.cuda.device(self.device):
                 return self._call(fn, where, *args)
         _check(fn(torch.cuda.current_stream().cuda_stream, *args), where)
@@ -441,45 +449,39 @@ class HipBackend:
         return buffer.data_ptr(), nbytes, buffer
 
     @staticmethod
-    def _state_args(T):
-        """Pointer, offset and strides of a tensor of one value per row, or nothing."""
-        return (None, 0, None) if T is None else (T.storage.data_ptr(), T.shape.offset, _arr(T.shape.strides))
+    def _part(part):
+        """Pointer, offset and strides of a (storage, offset, strides), or nothing."""
+        return (None, 0, None) if part is None else (part[0].data_ptr(), part[1], _const(part[2]))
+
+    @staticmethod
+    def _state(T):
+        """The same of a tensor of one value per row."""
+        return (None, 0, None) if T is None else (T.storage.data_ptr(), T.shape.offset, _const(T.shape.strides))
 
     @staticmethod
     def _start(T):
         return None if T is None else T.storage.data_ptr() + T.shape.offset * T.storage.element_size()
 
-    def gated_scan(self, kind, dtype, gs, g, xs, x, initial, ys, y, last):
-        where = "dlfx_gated_scan(%s)" % kind
-        n = xs.extents[-1]
-        m = xs.size // n
+    def gated_scan(self, kind, dtype, dims, g, x, initial, y, last):
+        """g, x, y: (storage, offset, strides) of views with the scanned axis last; initial (or None) and last: tensors."""
+        n, m = dims[-1], math.prod(dims[:-1])
         sp, sb, keep = self._call_scratch(self.lib.dlfx_gated_scan_scratch_bytes(dtype, m, n))
-        self._call(self.lib.dlfx_gated_scan, where, kind.encode(), dtype, m, n, xs.rank, _arr(xs.extents),
-                   g.data_ptr(), gs.offset, _arr(gs.strides), x.data_ptr(), xs.offset, _arr(xs.strides), *self._state_args(initial),
-                   y.data_ptr(), ys.offset, _arr(ys.strides), *self._state_args(last), sp, sb)
+        self._call(self.lib.dlfx_gated_scan, "dlfx_gated_scan", kind.encode(), dtype, m, n, len(dims), _const(dims),
+                   *self._part(g), *self._part(x), *self._state(initial), *self._part(y), *self._state(last), sp, sb)
 
-    def gated_scan_grad(self, kind, dtype, g, x, y, dy, dg, dx, initial, dlast, dinitial):
-        """Every tensor of the call's extents as (axis-moved shape, storage); x may be None."""
-        where = "dlfx_gated_scan_grad(%s)" % kind
-
-        def part(p):
-            return (None, 0, None) if p is None else (p[1].data_ptr(), p[0].offset, _arr(p[0].strides))
-        shape = y[0]
-        n = shape.extents[-1]
-        m = shape.size // n
+    def gated_scan_grad(self, kind, dtype, dims, g, x, y, dy, dg, dx, initial, dlast, dinitial):
+        n, m = dims[-1], math.prod(dims[:-1])
         sp, sb, keep = self._call_scratch(self.lib.dlfx_gated_scan_scratch_bytes(dtype, m, n))
-        self._call(self.lib.dlfx_gated_scan_grad, where, kind.encode(), dtype, m, n, shape.rank, _arr(shape.extents),
-                   *part(g), *part(x), *self._state_args(initial), *part(y), *part(dy), *self._state_args(dlast), *part(dg), *part(dx),
-                   *self._state_args(dinitial), sp, sb)
+        self._call(self.lib.dlfx_gated_scan_grad, "dlfx_gated_scan_grad", kind.encode(), dtype, m, n, len(dims), _const(dims),
+                   *self._part(g), *self._part(x), *self._state(initial), *self._part(y), *self._part(dy), *self._state(dlast),
+                   *self._part(dg), *self._part(dx), *self._state(dinitial), sp, sb)
 
     def route(self, score, dtype, m, n, x, stride, bias, groups, kept_groups, group_best, k, renormalise, scale, weights, indices, loads):
-        where = "dlfx_route(%s)" % score
-        self._call(self.lib.dlfx_route, where, score.encode(), dtype, m, n, x.storage.data_ptr(), x.shape.offset, stride, self._start(bias),
+        self._call(self.lib.dlfx_route, "dlfx_route", score.encode(), dtype, m, n, x.storage.data_ptr(), x.shape.offset, stride, self._start(bias),
                    groups, kept_groups, group_best, k, int(renormalise), scale, self._start(weights), self._start(indices), self._start(loads))
 
     def route_grad(self, score, dtype, m, n, x, stride, k, indices, dweights, renormalise, scale, dx, dx_stride):
-        where = "dlfx_route_grad(%s)" % score
-        self._call(self.lib.dlfx_route_grad, where, score.encode(), dtype, m, n, x.storage.data_ptr(), x.shape.offset, stride, k,
+        self._call(self.lib.dlfx_route_grad, "dlfx_route_grad", score.encode(), dtype, m, n, x.storage.data_ptr(), x.shape.offset, stride, k,
                    self._start(indices), self._start(dweights), int(renormalise), scale, dx.storage.data_ptr(), dx.shape.offset, dx_stride)
 
     def cross_entropy(self, dtype, index_dtype, m, n, x, stride, targets, z_loss, loss):

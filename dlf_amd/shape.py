@@ -52,6 +52,23 @@ class Shape:
             self.strides = tuple(int(s) for s in strides)
         self.offset = int(offset)
 
+    @classmethod
+    def of(cls, extents: tuple, strides: tuple, offset: int = 0) -> "Shape":
+        """A view of tuples of ints that are known to be in order (positive extents, as many strides)."""
+        shape = cls.__new__(cls)
+        shape.extents, shape.strides, shape.offset = extents, strides, offset
+        return shape
+
+    @classmethod
+    def dense(cls, extents: tuple) -> "Shape":
+        """The row-major view of a tuple of positive ints."""
+        strides, size = [], 1
+        for e in reversed(extents):
+            strides.append(size)
+            size *= e
+        strides.reverse()
+        return cls.of(extents, tuple(strides), 0)
+
     # -- basic queries ------------------------------------------------------
     @property
     def rank(self) -> int:
