@@ -1,5 +1,17 @@
 // Routing to experts: scores of a row of router logits, the k largest choices among the kept
 // groups, their weights; and the gradient of the logits.
+//
+// A row belongs to a team of L lanes (16 up to 256 experts, else a wavefront): expert i * L + lane is
+// the lane's item i, so that any run of neighbouring experts spreads over all lanes.  Nothing leaves
+// the wavefront: no barrier, no scratch.  The work per row is a few hundred vector instructions on a
+// kilobyte of logits, so arithmetic bounds it, and the choice is what the time goes to:
+//   * choices in fp32.  A bound from the lanes' largest items (the (k+1)-th largest of them) leaves
+//     little more than k candidates; those are gathered through LDS, one or two to a lane, and
+//     ordered by a bitonic network of (choice, index) words.
+//   * where fp32 cannot tell two neighbours of the result apart (a gap under twice the scores' error
+//     bound, about one row in a hundred with random scores), where candidates are too many, or
+//     k >= L, the wavefront does its rows over in 64 bits, picking one expert after the other.
+// Without a bias the logits order the experts exactly, and only sums of two scores can need 64 bits.
 #include <cstring>
 
 #include "sequence.hip.h"
@@ -14,211 +26,525 @@ template <> __device__ __forceinline__ float lowest_of<float>() { return -3.4028
 template <> __device__ __forceinline__ float lowest_of<half_t>() { return -65504.0f; }
 template <> __device__ __forceinline__ float lowest_of<bf16_t>() { return -3.38953138925153547590e38f; }
 
-// Choices are compared as unsigned images that keep the order of doubles: an expert outside the
-// kept groups 0, an absent one (or a NaN) 1, every number above that.
+constexpr float kMinusInfinity = -std::numeric_limits<float>::infinity();
+
+// Choices are compared as unsigned images that keep the order of the numbers: an expert outside the
+// kept groups is 0, an absent one (or a NaN) 1, every number above that.
+__device__ __forceinline__ uint32_t image_of(float v) {
+    if (v != v) return 1;
+    const uint32_t u = bit_cast<uint32_t>(v + 0.0f);          // -0.0 and +0.0 are one value
+    return (u >> 31) ? ~u : (u | 0x80000000u);
+}
 __device__ __forceinline__ uint64_t image_of(double v) {
     if (v != v) return 1;
-    v += 0.0;                              // -0.0 and +0.0 are one value
-    const uint64_t u = bit_cast<uint64_t>(v);
+    const uint64_t u = bit_cast<uint64_t>(v + 0.0);
     return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
+__device__ __forceinline__ float value_of(uint32_t image) { return bit_cast<float>((image >> 31) ? image & 0x7fffffffu : ~image); }
 
-// One wavefront per row: item i of a lane is expert i * 64 + lane.
-template <typename S, int KIND, int ITEMS>
-__global__ __launch_bounds__(256) void route_rows(const S* x, int64_t m, int n, int64_t stride, const float* bias, int groups, int kept_groups,
-                                                  int group_best, int k, int renormalise, float scale, float* weights, int32_t* indices,
-                                                  int32_t* loads) {
-    const int lane = threadIdx.x % kWave;
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
-    if (r >= m) return;
-    const S* xr = x + r * stride;
-    double score[ITEMS], choice[ITEMS];
-    bool present[ITEMS];
-    double mx = -std::numeric_limits<double>::infinity();
+template <typename C> struct ImageOf;
+template <> struct ImageOf<float> { using type = uint32_t; };
+template <> struct ImageOf<double> { using type = uint64_t; };
+
+template <int L, typename T, typename Join>
+__device__ __forceinline__ T team_reduce(T v, Join join) {
+    return group_reduce(v, L, join);
+}
+
+// Orders the LDS accesses of a wavefront: what its lanes have written is there for all of them.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+struct RouteCall {
+    int64_t m, stride;
+    int n, groups, kept_groups, group_best, size, size_magic, k, renormalise;      // e / size == (e * size_magic) >> 20
+    float scale;
+    const float* bias;
+    float* weights;
+    int32_t* indices;
+    int32_t* loads;
+};
+
+// Errors of fp32 scores: an exponential within (d + 3) u of itself at a distance d below the maximum
+// (exp(-d) d < 0.4), sums of 1024 terms in lanes of 16 and a tree within 24 u, a division: under 32 u
+// for scores up to 1, a rounding of the sum with the bias besides.  Two choices are told apart when
+// they differ by more than both errors.
+__device__ __forceinline__ float border(float a, float b) { return 0x1p-18f * (2.0f + fmaxf(fabsf(a), fabsf(b))); }
+
+// LDS of a team: the items' values and the groups' (fp32), or the groups' (64 bits), or the candidates;
+// then a byte per group.  (8 of 32 doubles left over: the teams of a wavefront start 16 banks apart.)
+template <int L, int ITEMS>
+constexpr int team_doubles() { return L * ITEMS + L * ITEMS / 8 + (40 - (L * ITEMS + L * ITEMS / 8) % 32) % 32; }
+
+// The two largest of a group's values and how many there are.
+template <typename C>
+struct Best {
+    C first, second;
+    int count;
+    __device__ __forceinline__ void add(C v) {
+        if (v != v) return;
+        ++count;
+        second = v > first ? first : (v > second ? v : second);
+        first = v > first ? v : first;
+    }
+    __device__ __forceinline__ void add(const Best& o) {
+        count += o.count;
+        const C low = o.first > first ? first : o.first;
+        second = o.second > second ? o.second : second;
+        second = low > second ? low : second;
+        first = o.first > first ? o.first : first;
+    }
+    __device__ __forceinline__ C value(int best) const {
+        if (count == 0) return std::numeric_limits<C>::quiet_NaN();
+        return best == 2 && count > 1 ? first + second : first;
+    }
+};
+
+// Values of the groups in sums[]; value[i]: what a present item adds to its group.
+template <int L, int ITEMS>
+__device__ __forceinline__ void group_values(const RouteCall& p, const float (&value)[ITEMS], uint32_t present, float* items, float* sums, int lane) {
+    const float none = -std::numeric_limits<float>::infinity();
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+        if (i * L + lane < p.n) items[i * L + lane] = (present >> i & 1) ? value[i] : std::numeric_limits<float>::quiet_NaN();
+    wave_sync();
+    // lanes_per lanes (a power of two) to a group; a lane walks its part of the group's experts from a
+    // place of its own, so that the lanes read different LDS banks
+    int lanes_per = L;
+    while (lanes_per > 1 && lanes_per * p.groups > L) lanes_per >>= 1;
+    const int part = lane & (lanes_per - 1), side_by_side = L / lanes_per;
+    for (int g0 = 0; g0 < p.groups; g0 += side_by_side) {
+        const int g = g0 + lane / lanes_per;
+        Best<float> best = {none, none, 0};
+        if (g < p.groups) {
+            const int from = g - p.size * ((g * p.size_magic) >> 20);
+            for (int i = part; i < p.size; i += lanes_per) {
+                int e = i + from;
+                e -= e >= p.size ? p.size : 0;
+                best.add(items[g * p.size + e]);
+            }
+        }
+        for (int j = 1; j < lanes_per; j <<= 1) best.add({lane_xor(best.first, j), lane_xor(best.second, j), lane_xor(best.count, j)});
+        if (g < p.groups && part == 0) sums[g] = best.value(p.group_best);
+    }
+    wave_sync();
+}
+// The same in 64 bits, a group at a time (rows that fp32 does not settle).
+template <int L, int ITEMS>
+__device__ __forceinline__ void group_values(const RouteCall& p, const double (&value)[ITEMS], uint32_t present, double* sums, int lane) {
+    const double none = -std::numeric_limits<double>::infinity();
+    for (int g = 0; g < p.groups; ++g) {
+        Best<double> best = {none, none, 0};
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if ((present >> i & 1) && ((i * L + lane) * p.size_magic) >> 20 == g) best.add(value[i]);
+        for (int j = 1; j < L; j <<= 1) best.add({lane_xor(best.first, j), lane_xor(best.second, j), lane_xor(best.count, j)});
+        if (lane == 0) sums[g] = best.value(p.group_best);
+    }
+    wave_sync();
+}
+
+// Which items lie in a kept group, a bit per item of the lane.  `unsure` when the values are not exact
+// and a kept group's lies too close to one that was left.
+template <typename C, int L, int ITEMS>
+__device__ __forceinline__ uint32_t kept_items(const RouteCall& p, const C* sums, uint8_t* kept, bool exact, int lane, bool& unsure) {
+    const C none = -std::numeric_limits<C>::infinity();
+    C worst_kept = -none, best_left = none;
+    for (int g = lane; g < p.groups; g += L) {
+        // a group's rank: how many come before it (larger value, or equal and lower)
+        const C v = sums[g];
+        const auto mine = image_of(v);
+        int rank = 0;
+        for (int o = 0; o < p.groups; ++o) {
+            const auto other = image_of(sums[o]);
+            rank += other > mine || (other == mine && o < g);
+        }
+        const bool keep = rank < p.kept_groups;
+        kept[g] = keep;
+        if (v == v) {
+            if (keep) worst_kept = v < worst_kept ? v : worst_kept;
+            else best_left = v > best_left ? v : best_left;
+        }
+    }
+    wave_sync();
+    uint32_t open = 0;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        const int e = i * kWave + lane;
-        const float v = e < n ? static_cast<float>(xr[e]) : -std::numeric_limits<float>::infinity();
-        present[i] = !(v <= lowest_of<S>());
-        score[i] = v;
-        if (present[i]) mx = v > mx ? v : mx;
+        const int e = i * L + lane;
+        if (e < p.n && kept[(e * p.size_magic) >> 20]) open |= 1u << i;
     }
-    mx = wave_reduce(mx, [](double a, double b) { return b > a ? b : a; });
+    if (!exact) {
+        worst_kept = team_reduce<L>(worst_kept, [](C a, C b) { return b < a ? b : a; });
+        best_left = team_reduce<L>(best_left, [](C a, C b) { return b > a ? b : a; });
+        // (a sum of two choices carries two errors)
+        const float a = static_cast<float>(worst_kept), b = static_cast<float>(best_left);
+        if (best_left != none && !(a - b > 2.0f * border(a, b))) unsure = true;
+    }
+    return open;
+}
+
+template <typename S, int KIND, int L, int ITEMS>
+struct RouteRow {
+    float x[ITEMS];
+    uint32_t present;
+    float mx, inverse;        // softmax: the largest present logit, 1 / sum of exp(x - mx)
+
+    __device__ __forceinline__ void load(const S* row, int n, int lane, bool live) {
+        present = 0;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) x[i] = live && i * L + lane < n ? static_cast<float>(row[i * L + lane]) : kMinusInfinity;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) present |= (x[i] <= lowest_of<S>() ? 0u : 1u) << i;
+        mx = kMinusInfinity;
+        inverse = 0.0f;
+        if constexpr (KIND == kSoftmaxScore) {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                if (present >> i & 1) mx = fmaxf(mx, x[i]);
+            mx = team_reduce<L>(mx, [](float a, float b) { return fmaxf(a, b); });
+        }
+    }
+    __device__ __forceinline__ void normalise() {
+        if constexpr (KIND == kSoftmaxScore) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                if (present >> i & 1) sum += power(x[i]);
+            sum = team_reduce<L>(sum, [](float a, float b) { return a + b; });
+            inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+        }
+    }
+    __device__ __forceinline__ float power(float v) const { return __builtin_amdgcn_exp2f((v - mx) * kLog2E); }
+    __device__ __forceinline__ float score(float v) const {
+        if constexpr (KIND == kSoftmaxScore) {
+            return power(v) * inverse;
+        } else {
+            const float e = __builtin_amdgcn_exp2f(-fabsf(v) * kLog2E), r = 1.0f / (1.0f + e);
+            return v < 0.0f ? e * r : r;
+        }
+    }
+};
+
+// The k choices in 64 bits, one after the other: place t ends in lane t.
+template <typename S, int KIND, int L, int ITEMS>
+__device__ __forceinline__ int choose_exactly(const RouteCall& p, const RouteRow<S, KIND, L, ITEMS>& row, double* lds, int lane) {
+    double value[ITEMS];
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        choice[i] = score[i];
-        if constexpr (KIND == kSoftmaxScore) score[i] = present[i] ? exp(score[i] - mx) : 0.0;
-        else score[i] = present[i] ? 1.0 / (1.0 + exp(-score[i])) : 0.0;
-        sum += score[i];
+        const double v = row.x[i];
+        if constexpr (KIND == kSoftmaxScore) value[i] = (row.present >> i & 1) ? exp(v - static_cast<double>(row.mx)) : 0.0;
+        else value[i] = 1.0 / (1.0 + exp(-v));
+        sum += value[i];
     }
     if constexpr (KIND == kSoftmaxScore) {
-        sum = wave_reduce(sum, [](double a, double b) { return a + b; });
-        const double scale_by = sum == 0.0 ? 0.0 : 1.0 / sum;
+        sum = team_reduce<L>(sum, [](double a, double b) { return a + b; });
+        const double by = sum == 0.0 ? 0.0 : 1.0 / sum;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) score[i] *= scale_by;
+        for (int i = 0; i < ITEMS; ++i) value[i] *= by;
     }
-    const bool by_score = bias || kept_groups < groups;
+    if (p.bias) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (i * L + lane < p.n) value[i] += static_cast<double>(p.bias[i * L + lane]);
+    }
+    uint32_t open = 0xffffffffu;
+    bool unsure = false;
+    if (p.kept_groups < p.groups) {
+        if (!p.bias && p.group_best == 1) {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) value[i] = row.x[i];
+        }
+        wave_sync();
+        group_values<L, ITEMS>(p, value, row.present, lds, lane);
+        open = kept_items<double, L, ITEMS>(p, lds, reinterpret_cast<uint8_t*>(lds + L * ITEMS), true, lane, unsure);
+    }
     uint64_t image[ITEMS];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        const int e = i * kWave + lane;
-        if (by_score) choice[i] = score[i] + (bias && e < n ? static_cast<double>(bias[e]) : 0.0);
-        image[i] = e >= n ? 0 : present[i] ? image_of(choice[i]) : 1;
+        const double c = p.bias ? value[i] : static_cast<double>(row.x[i]);
+        image[i] = i * L + lane >= p.n || !(open >> i & 1) ? 0 : (row.present >> i & 1) ? image_of(c) : 1;
     }
-    if (kept_groups < groups) {
-        const int size = n / groups;
-        // one group at a time: its value; then the groups are kept best first
-        uint64_t group_image[ITEMS];       // group i * 64 + lane
-        for (int i = 0; i < ITEMS; ++i) group_image[i] = 0;
-        for (int g = 0; g < groups; ++g) {
-            uint64_t best = 0;
-            int at = -1;
-            double value = 0.0;
-            bool any = false;
-            for (int round = 0; round < group_best; ++round) {
-                uint64_t mine = 0;
-                int where = 0x7fffffff;
-                for (int i = 0; i < ITEMS; ++i) {
-                    const int e = i * kWave + lane;
-                    if (e / size != g || e >= n || e == at || image[i] <= 1) continue;
-                    if (image[i] > mine) mine = image[i], where = e;
-                }
-                best = wave_reduce(mine, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-                if (best <= 1) break;
-                int first = mine == best ? where : 0x7fffffff;
-                first = wave_reduce(first, [](int a, int b) { return a < b ? a : b; });
-                at = first;
-                value += (best >> 63) ? bit_cast<double>(best & 0x7fffffffffffffffull) : bit_cast<double>(~best);
-                any = true;
-            }
-            const uint64_t gi = any ? image_of(value) : 1;
-            for (int i = 0; i < ITEMS; ++i)
-                if (i * kWave + lane == g) group_image[i] = gi;
+    int mine = 0;
+    for (int t = 0; t < p.k; ++t) {
+        uint64_t best = 0;
+        int at = 0x7fffffff;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (image[i] > best) best = image[i], at = i * L + lane;
+        const uint64_t top = team_reduce<L>(best, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+        at = team_reduce<L>(best == top ? at : 0x7fffffff, [](int a, int b) { return a < b ? a : b; });
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (i * L + lane == at) image[i] = 0;
+        if (lane == t) mine = at;
+    }
+    return mine;
+}
+
+// The k choices in fp32 (k < L): place t ends in lane t.  `unsure` when they may not be the exact ones.
+template <typename S, int KIND, int L, int ITEMS>
+__device__ __forceinline__ int choose(const RouteCall& p, const RouteRow<S, KIND, L, ITEMS>& row, const S* x, float* lds, int lane, bool& unsure) {
+    uint32_t image[ITEMS];
+    uint32_t open = 0xffffffffu;
+    {
+        float c[ITEMS];
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            c[i] = row.x[i];
+            if (p.bias) c[i] = row.score(c[i]) + (i * L + lane < p.n ? p.bias[i * L + lane] : 0.0f);
         }
-        uint64_t open[ITEMS];
-        for (int i = 0; i < ITEMS; ++i) open[i] = 0;
-        for (int t = 0; t < kept_groups; ++t) {
-            uint64_t mine = 0;
-            int where = 0x7fffffff;
-            for (int i = 0; i < ITEMS; ++i)
-                if (group_image[i] > mine) mine = group_image[i], where = i * kWave + lane;
-            const uint64_t best = wave_reduce(mine, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-            int first = mine == best ? where : 0x7fffffff;
-            first = wave_reduce(first, [](int a, int b) { return a < b ? a : b; });
-            for (int i = 0; i < ITEMS; ++i) {
-                if (i * kWave + lane == first) group_image[i] = 0;
-                if ((i * kWave + lane) / size == first) open[i] = 1;
+        if (p.kept_groups < p.groups) {
+            // (without a bias: by the scores where two are added, else by the logits themselves)
+            const bool exact = !p.bias && p.group_best == 1;
+            float v[ITEMS];
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) v[i] = p.bias || exact ? c[i] : row.score(row.x[i]);
+            wave_sync();
+            group_values<L, ITEMS>(p, v, row.present, lds, lds + L * ITEMS, lane);
+            open = kept_items<float, L, ITEMS>(p, lds + L * ITEMS, reinterpret_cast<uint8_t*>(lds + 2 * L * ITEMS), exact, lane, unsure);
+        }
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            image[i] = i * L + lane >= p.n || !(open >> i & 1) ? 0 : (row.present >> i & 1) ? image_of(c[i]) : 1;
+    }
+    // candidates: everything from the (k+1)-th largest of the lanes' largest items on
+    uint32_t most = image[0];
+#pragma unroll
+    for (int i = 1; i < ITEMS; ++i) most = image[i] > most ? image[i] : most;
+    wave_bitonic<L, true>([&](auto jc, bool keep_better) {
+        const uint32_t other = lane_xor_const<decltype(jc)::value>(most);
+        most = keep_better == (other > most) ? other : most;
+    });
+    const int base = lane_id() & ~(L - 1);
+    uint32_t bound = lane_get(most, base + p.k);
+    if (bound == 0) bound = 1;
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) count += image[i] >= bound;
+    int upto = count;
+    {
+        int o = dpp_fetch<kRowShr1>(upto, 0);
+        upto += o;
+        o = dpp_fetch<kRowShr2>(upto, 0);
+        upto += o;
+        o = dpp_fetch<kRowShr4>(upto, 0);
+        upto += o;
+        o = dpp_fetch<kRowShr8>(upto, 0);
+        upto += o;
+        if constexpr (L == kWave) {
+            o = dpp_fetch<kRowBcast15, 0xa>(upto, 0);
+            upto += o;
+            o = dpp_fetch<kRowBcast31, 0xc>(upto, 0);
+            upto += o;
+        }
+    }
+    const int total = lane_get(upto, base + L - 1);
+    uint64_t* slots = reinterpret_cast<uint64_t*>(lds);
+    constexpr int SLOTS = 2 * L;
+    wave_sync();
+    int place = upto - count;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        if (image[i] >= bound) {
+            if (place < SLOTS) slots[place] = static_cast<uint64_t>(image[i]) << 32 | (0xffffffffu - static_cast<uint32_t>(i * L + lane));
+            ++place;
+        }
+    }
+    wave_sync();
+    uint64_t mine = lane < total ? slots[lane] : 0;
+    auto sort = [&](uint64_t& v) {
+        wave_bitonic<L, true>([&](auto jc, bool keep_better) {
+            const uint64_t other = lane_xor_const<decltype(jc)::value>(v);
+            v = keep_better == (other > v) ? other : v;
+        });
+    };
+    sort(mine);
+    if (__any(total > L)) {
+        // a second word for some lanes: ordered by itself, its largest against the first words' smallest
+        uint64_t more = L + lane < total ? slots[L + lane] : 0;
+        sort(more);
+        const uint64_t other = lane_get(more, base + (L - 1) - (lane_id() & (L - 1)));
+        mine = other > mine ? other : mine;
+        sort(mine);
+    }
+    if (total > SLOTS) unsure = true;
+    if (p.bias) {
+        // neighbours too close for fp32; equal logits with equal biases are equal, whatever the precision
+        const uint64_t next = lane_get(mine, base + ((lane + 1) & (L - 1)));
+        const uint32_t a = static_cast<uint32_t>(mine >> 32), b = static_cast<uint32_t>(next >> 32);
+        if (lane < p.k && a > 1 && b > 1) {
+            const float va = value_of(a), vb = value_of(b);
+            if (!(va - vb > border(va, vb))) {
+                const int ea = static_cast<int>(0xffffffffu - static_cast<uint32_t>(mine)), eb = static_cast<int>(0xffffffffu - static_cast<uint32_t>(next));
+                const bool equal = static_cast<float>(x[ea]) == static_cast<float>(x[eb]) && p.bias[ea] == p.bias[eb];
+                // (the last place against the first one left out: others of that value may follow unseen)
+                if (!equal || lane == p.k - 1) unsure = true;
             }
         }
-        for (int i = 0; i < ITEMS; ++i)
-            if (!open[i]) image[i] = 0;
     }
-    double total = 0.0, my_score = 0.0;
-    int my_index = 0;
-    for (int t = 0; t < k; ++t) {
-        uint64_t mine = 0;
-        int where = 0x7fffffff;
-        double s = 0.0;
-        for (int i = 0; i < ITEMS; ++i)
-            if (image[i] > mine) mine = image[i], where = i * kWave + lane, s = score[i];
-        const uint64_t best = wave_reduce(mine, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-        int first = mine == best ? where : 0x7fffffff;
-        first = wave_reduce(first, [](int a, int b) { return a < b ? a : b; });
-        const double chosen = lane_get(s, first % kWave);
-        for (int i = 0; i < ITEMS; ++i)
-            if (i * kWave + lane == first) image[i] = 0;
-        total += chosen;
-        if (lane == t) my_index = first, my_score = chosen;
+    return static_cast<int>(0xffffffffu - static_cast<uint32_t>(mine));
+}
+
+template <typename S, int KIND, int L, int ITEMS>
+__global__ __launch_bounds__(256) void route_rows(const S* x, RouteCall p) {
+    constexpr int TEAMS = 256 / L;
+    __shared__ double lds[TEAMS][team_doubles<L, ITEMS>()];
+    __shared__ int32_t histogram[L * ITEMS];
+    const int lane = threadIdx.x % L, team = threadIdx.x / L;
+    if (p.loads) {
+        for (int e = threadIdx.x; e < p.n; e += 256) histogram[e] = 0;
+        __syncthreads();
     }
-    if (lane < k) {
-        double w = my_score;
-        if (renormalise) w = total == 0.0 ? 0.0 : w / total;
-        weights[r * k + lane] = static_cast<float>(w * static_cast<double>(scale));
-        indices[r * k + lane] = my_index;
-        if (loads) atomicAdd(&loads[my_index], 1);
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * TEAMS; r0 < p.m; r0 += static_cast<int64_t>(gridDim.x) * TEAMS) {
+        const int64_t r = r0 + team;
+        const bool live = r < p.m;
+        const S* xr = x + (live ? r : 0) * p.stride;
+        RouteRow<S, KIND, L, ITEMS> row;
+        row.load(xr, p.n, lane, true);
+        if (p.bias || p.kept_groups < p.groups || !p.renormalise) row.normalise();
+        bool unsure = p.k >= L;
+        int e = 0;
+        if (p.k < L) e = choose<S, KIND, L, ITEMS>(p, row, xr, reinterpret_cast<float*>(lds[team]), lane, unsure);
+        if (__any(unsure)) e = choose_exactly<S, KIND, L, ITEMS>(p, row, lds[team], lane);
+        float s = 0.0f, total = 1.0f;
+        const bool place = lane < p.k;
+        const float v = place ? static_cast<float>(xr[e]) : kMinusInfinity;
+        const bool there = place && !(v <= lowest_of<S>());
+        if (KIND == kSoftmaxScore && p.renormalise) {
+            // the chosen logits' own softmax: what all scores have in common cancels
+            const float top = team_reduce<L>(there ? v : kMinusInfinity, [](float a, float b) { return fmaxf(a, b); });
+            if (there) s = __builtin_amdgcn_exp2f((v - top) * kLog2E);
+        } else if (there) {
+            s = row.score(v);
+        }
+        if (p.renormalise) {
+            total = team_reduce<L>(s, [](float a, float b) { return a + b; });
+            if (total == 0.0f) total = 1.0f;
+        }
+        if (live && place) {
+            p.weights[r * p.k + lane] = p.renormalise ? s / total * p.scale : s * p.scale;
+            p.indices[r * p.k + lane] = e;
+            if (p.loads) atomicAdd(&histogram[e], 1);
+        }
+    }
+    if (p.loads) {
+        __syncthreads();
+        for (int e = threadIdx.x; e < p.n; e += 256)
+            if (histogram[e]) atomicAdd(&p.loads[e], histogram[e]);
     }
 }
 
-template <typename S, int KIND, int ITEMS>
-__global__ __launch_bounds__(256) void route_grad_rows(const S* x, int64_t m, int n, int64_t stride, int k, const int32_t* indices,
-                                                       const float* dweights, int renormalise, float scale, S* dx, int64_t dx_stride) {
-    const int lane = threadIdx.x % kWave;
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
-    if (r >= m) return;
-    const S* xr = x + r * stride;
-    float s[ITEMS], ds[ITEMS], rest[ITEMS];
-    float mx = -std::numeric_limits<float>::infinity();
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        const int e = i * kWave + lane;
-        s[i] = e < n ? static_cast<float>(xr[e]) : -std::numeric_limits<float>::infinity();
-        if (s[i] <= lowest_of<S>()) s[i] = -std::numeric_limits<float>::infinity();
-        mx = fmaxf(mx, s[i]);
-        ds[i] = 0.0f;
+struct RouteGradCall {
+    int64_t m, stride, dx_stride;
+    int n, k, renormalise;
+    float scale;
+    const int32_t* indices;
+    const float* dweights;
+};
+
+// With c the chosen experts, d the weights' gradients times scale:
+//   sigmoid:                 ds[c] = d;  renormalised: (d - sum d s / S) / S, S the chosen scores' sum;  dx = ds s (1 - s)
+//   softmax:                 dx = s (ds - sum ds s), over every expert
+//   softmax, renormalised:   the weights are the chosen logits' own softmax q: dx[c] = q (d - sum d q), 0 elsewhere -
+//                            only the k chosen logits are read.
+template <typename S, int KIND, int L, int ITEMS>
+__global__ __launch_bounds__(256) void route_grad_rows(const S* x, S* dx, RouteGradCall p) {
+    constexpr int TEAMS = 256 / L;
+    const int lane = threadIdx.x % L, team = threadIdx.x / L;
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * TEAMS + team;
+    const bool live = r < p.m;
+    const int64_t rr = live ? r : p.m - 1;
+    const S* xr = x + rr * p.stride;
+    const int32_t* index = p.indices + rr * p.k;
+    const float* dw = p.dweights + rr * p.k;
+    auto add = [](float a, float b) { return a + b; };
+
+    RouteRow<S, KIND, L, ITEMS> row;
+    if (!(KIND == kSoftmaxScore && p.renormalise)) {
+        row.load(xr, p.n, lane, true);
+        row.normalise();
     }
-    mx = wave_reduce(mx, [](float a, float b) { return fmaxf(a, b); });
-    float sum = 0.0f;
+    float grad[ITEMS];
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        const float v = s[i];
-        const bool present = v != -std::numeric_limits<float>::infinity();
-        if constexpr (KIND == kSoftmaxScore) {
-            s[i] = present ? expf(v - mx) : 0.0f;
-        } else {
-            const float e = expf(-fabsf(v)), big = 1.0f / (1.0f + e), small = e * big;
-            s[i] = !present ? 0.0f : v < 0.0f ? small : big;
-            rest[i] = v < 0.0f ? big : small;
+    for (int i = 0; i < ITEMS; ++i) grad[i] = 0.0f;
+    // the places of the row, L at a time: place t in lane t % L
+    float top = kMinusInfinity, total = 0.0f, dot = 0.0f;
+    auto place = [&](int t, int& e, float& v, float& d) {
+        e = t < p.k ? index[t] : -1;
+        const bool ok = e >= 0 && e < p.n;
+        v = ok ? static_cast<float>(xr[e]) : kMinusInfinity;
+        d = ok ? dw[t] * p.scale : 0.0f;
+        if (v <= lowest_of<S>()) e = -1;                 // absent: no weight, no gradient
+    };
+    if (KIND == kSoftmaxScore && p.renormalise) {
+        for (int t0 = 0; t0 < p.k; t0 += L) {
+            int e;
+            float v, d;
+            place(t0 + lane, e, v, d);
+            if (e >= 0) top = fmaxf(top, v);
         }
-        sum += s[i];
+        top = team_reduce<L>(top, [](float a, float b) { return fmaxf(a, b); });
     }
-    if constexpr (KIND == kSoftmaxScore) {
-        sum = wave_reduce(sum, [](float a, float b) { return a + b; });
-        const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) s[i] *= by;
+    auto score = [&](float v) {
+        if (KIND == kSoftmaxScore && p.renormalise) return __builtin_amdgcn_exp2f((v - top) * kLog2E);
+        return row.score(v);
+    };
+    for (int t0 = 0; t0 < p.k; t0 += L) {
+        int e;
+        float v, d;
+        place(t0 + lane, e, v, d);
+        const float s = e >= 0 ? score(v) : 0.0f;
+        total += s;
+        dot += d * s;
     }
-    // chosen[i]: how often the row's k places name the expert; ds its share of the weights' gradients
-    float chosen[ITEMS];
-    for (int i = 0; i < ITEMS; ++i) chosen[i] = 0.0f;
-    for (int t = 0; t < k; ++t) {
-        const int e = indices[r * k + t];
-        const float d = dweights[r * k + t] * scale;
-        for (int i = 0; i < ITEMS; ++i)
-            if (i * kWave + lane == e && e < n) ds[i] += d, chosen[i] += 1.0f;
-    }
-    if (renormalise) {
-        float total = 0.0f, dot = 0.0f;
-        for (int i = 0; i < ITEMS; ++i) total += chosen[i] * s[i], dot += ds[i] * s[i];
-        total = wave_reduce(total, [](float a, float b) { return a + b; });
-        dot = wave_reduce(dot, [](float a, float b) { return a + b; });
-        const float by = total == 0.0f ? 0.0f : 1.0f / total;
-        for (int i = 0; i < ITEMS; ++i) ds[i] = (ds[i] - chosen[i] * dot * by) * by;
-    }
-    if constexpr (KIND == kSoftmaxScore) {
-        float dot = 0.0f;
-        // renormalised weights do not change with the scores' common factor: the sum is 0
-        if (!renormalise) {
-            for (int i = 0; i < ITEMS; ++i) dot += ds[i] * s[i];
-            dot = wave_reduce(dot, [](float a, float b) { return a + b; });
+    total = team_reduce<L>(total, add);
+    dot = team_reduce<L>(dot, add);
+    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+    const int base = lane_id() & ~(L - 1);
+    for (int t0 = 0; t0 < p.k; t0 += L) {
+        int e;
+        float v, d;
+        place(t0 + lane, e, v, d);
+        float g = 0.0f;
+        if (e >= 0) {
+            const float s = score(v);
+            if (p.renormalise) d = (d - dot * by) * by;
+            if constexpr (KIND == kSoftmaxScore) g = s * d;
+            else g = s * d * row.score(-v);
         }
-        for (int i = 0; i < ITEMS; ++i) s[i] *= ds[i] - dot;
-    } else {
-        for (int i = 0; i < ITEMS; ++i) s[i] *= ds[i] * rest[i];
+        for (int t = 0; t < L && t0 + t < p.k; ++t) {
+            const int ee = lane_get(e, base + t);
+            const float gg = lane_get(g, base + t);
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) grad[i] += ee == i * L + lane ? gg : 0.0f;
+        }
     }
+    if (!live) return;
+#pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        const int e = i * kWave + lane;
-        if (e < n) dx[r * dx_stride + e] = static_cast<S>(s[i]);
+        const int e = i * L + lane;
+        if (e >= p.n) continue;
+        float g = grad[i];
+        if (KIND == kSoftmaxScore && !p.renormalise && (row.present >> i & 1)) g -= dot * row.score(row.x[i]);
+        dx[r * p.dx_stride + e] = static_cast<S>(g);
     }
 }
 
+// f(lanes of a team, items of a lane): sixteen lanes while their items fit and the places leave the
+// border's one to spare, otherwise a wavefront.
 template <typename F>
-int dispatch_items(int64_t n, F&& f) {
-    if (n <= 64) return f(std::integral_constant<int, 1>());
-    if (n <= 128) return f(std::integral_constant<int, 2>());
-    if (n <= 256) return f(std::integral_constant<int, 4>());
-    if (n <= 512) return f(std::integral_constant<int, 8>());
-    return f(std::integral_constant<int, 16>());
+int dispatch_team(int64_t n, int64_t k, F&& f) {
+    using std::integral_constant;
+    if (k < 16) {
+        if (n <= 64) return f(integral_constant<int, 16>(), integral_constant<int, 4>());
+        if (n <= 128) return f(integral_constant<int, 16>(), integral_constant<int, 8>());
+        if (n <= 256) return f(integral_constant<int, 16>(), integral_constant<int, 16>());
+    }
+    if (n <= 256) return f(integral_constant<int, kWave>(), integral_constant<int, 4>());
+    return f(integral_constant<int, kWave>(), integral_constant<int, 16>());
 }
 
 int check(const char* name, int64_t m, int64_t n, int64_t k, const void* x, int64_t stride, int* kind) {
@@ -243,19 +569,23 @@ extern "C" int dlfx_route(dlfx_stream_t stream, const char* name, int dtype, int
     if (int e = check(name, m, n, k, x, row_stride, &kind)) return e;
     if (!weights || !indices) return DLFX_ERR_INVALID_ARGUMENT;
     if (groups <= 0 || n % groups || kept_groups <= 0 || kept_groups > groups || (group_best != 1 && group_best != 2)) return DLFX_ERR_INVALID_ARGUMENT;
-    if (kept_groups * (n / groups) < k) return DLFX_ERR_INVALID_ARGUMENT;
+    const int64_t size = n / groups;
+    if (kept_groups * size < k) return DLFX_ERR_INVALID_ARGUMENT;
+    RouteCall p{m, row_stride, static_cast<int>(n), static_cast<int>(groups), static_cast<int>(kept_groups), group_best, static_cast<int>(size),
+                static_cast<int>(ceil_div(1 << 20, size)), static_cast<int>(k), renormalise, scale, bias, weights, indices, loads};
     return dispatch_sequence_dtype(dtype, [&](auto tag) {
         using S = decltype(tag);
-        return dispatch_items(n, [&](auto items) {
-            constexpr int ITEMS = decltype(items)::value;
+        return dispatch_team(n, k, [&](auto lanes, auto items) {
+            constexpr int L = decltype(lanes)::value, ITEMS = decltype(items)::value;
             auto run = [&](auto kernel) {
-                kernel<<<dim3(static_cast<unsigned>(ceil_div(m, 4))), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
-                    static_cast<const S*>(x) + x_offset, m, static_cast<int>(n), row_stride, bias, static_cast<int>(groups),
-                    static_cast<int>(kept_groups), group_best, static_cast<int>(k), renormalise, scale, weights, indices, loads);
+                // counting: a workgroup takes many rows, or adding up its counters costs more than the rows
+                const int64_t blocks = ceil_div(m, 256 / L), most = loads ? 512 : 0x7fffffffLL;
+                kernel<<<dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+                    static_cast<const S*>(x) + x_offset, p);
                 DLFX_CHECK_LAUNCH();
                 return static_cast<int>(DLFX_OK);
             };
-            return kind == kSoftmaxScore ? run(route_rows<S, kSoftmaxScore, ITEMS>) : run(route_rows<S, kSigmoidScore, ITEMS>);
+            return kind == kSoftmaxScore ? run(route_rows<S, kSoftmaxScore, L, ITEMS>) : run(route_rows<S, kSigmoidScore, L, ITEMS>);
         });
     });
 }
@@ -267,18 +597,18 @@ extern "C" int dlfx_route_grad(dlfx_stream_t stream, const char* name, int dtype
     int kind;
     if (int e = check(name, m, n, k, x, row_stride, &kind)) return e;
     if (!indices || !dweights || !dx || dx_row_stride < n) return DLFX_ERR_INVALID_ARGUMENT;
+    RouteGradCall p{m, row_stride, dx_row_stride, static_cast<int>(n), static_cast<int>(k), renormalise, scale, indices, dweights};
     return dispatch_sequence_dtype(dtype, [&](auto tag) {
         using S = decltype(tag);
-        return dispatch_items(n, [&](auto items) {
-            constexpr int ITEMS = decltype(items)::value;
+        return dispatch_team(n, 1, [&](auto lanes, auto items) {
+            constexpr int L = decltype(lanes)::value, ITEMS = decltype(items)::value;
             auto run = [&](auto kernel) {
-                kernel<<<dim3(static_cast<unsigned>(ceil_div(m, 4))), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
-                    static_cast<const S*>(x) + x_offset, m, static_cast<int>(n), row_stride, static_cast<int>(k), indices, dweights, renormalise,
-                    scale, static_cast<S*>(dx) + dx_offset, dx_row_stride);
+                kernel<<<dim3(static_cast<unsigned>(ceil_div(m, 256 / L))), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+                    static_cast<const S*>(x) + x_offset, static_cast<S*>(dx) + dx_offset, p);
                 DLFX_CHECK_LAUNCH();
                 return static_cast<int>(DLFX_OK);
             };
-            return kind == kSoftmaxScore ? run(route_grad_rows<S, kSoftmaxScore, ITEMS>) : run(route_grad_rows<S, kSigmoidScore, ITEMS>);
+            return kind == kSoftmaxScore ? run(route_grad_rows<S, kSoftmaxScore, L, ITEMS>) : run(route_grad_rows<S, kSigmoidScore, L, ITEMS>);
         });
     });
 }
