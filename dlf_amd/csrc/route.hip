@@ -8,10 +8,11 @@
 //   * choices in fp32.  A bound from the lanes' largest items (the (k+1)-th largest of them) leaves
 //     little more than k candidates; those are gathered through LDS, one or two to a lane, and
 //     ordered by a bitonic network of (choice, index) words.
-//   * where fp32 cannot tell two neighbours of the result apart (a gap under twice the scores' error
-//     bound, about one row in a hundred with random scores), where candidates are too many, or
-//     k >= L, the wavefront does its rows over in 64 bits, picking one expert after the other.
-// Without a bias the logits order the experts exactly, and only sums of two scores can need 64 bits.
+//   * where fp32 cannot tell two neighbours of the result apart (a gap under their errors, one row in
+//     hundreds with random scores), the row is marked and a second launch does it over in 64 bits,
+//     picking one expert after the other.
+// Without a bias the logits order the experts exactly, and only sums of two scores can need 64 bits:
+// other calls are one launch.
 #include <cstring>
 
 #include "sequence.hip.h"
@@ -67,11 +68,13 @@ struct RouteCall {
     int32_t* loads;
 };
 
-// Errors of fp32 scores: an exponential within (d + 3) u of itself at a distance d below the maximum
-// (exp(-d) d < 0.4), sums of 1024 terms in lanes of 16 and a tree within 24 u, a division: under 32 u
-// for scores up to 1, a rounding of the sum with the bias besides.  Two choices are told apart when
-// they differ by more than both errors.
-__device__ __forceinline__ float border(float a, float b) { return 0x1p-18f * (2.0f + fmaxf(fabsf(a), fabsf(b))); }
+// How far apart two fp32 choices a and b have to be to be told apart: both errors together, with
+// u = 2^-24.  `scores` is the scores' part: the logistic function is off by under 1 u from its
+// exponential (1.5 |x| + 2 u of it, times s (1 - s)) and a rounding each in its sum, quotient and
+// product, 4 u in all, 16 u is taken; a softmax score by under 28 u of itself (terms (1.5 d + 2) u at a
+// distance d below the maximum, up to 22 roundings of the sum, two more), and no score is larger than
+// the row's 1 / sum: 64 u of that is taken.  The sum with the bias rounds once: 2 u, 4 u taken.
+__device__ __forceinline__ float border(float scores, float a, float b) { return scores + 0x1p-22f * fmaxf(fabsf(a), fabsf(b)); }
 
 // LDS of a team: the items' values and the groups' (fp32), or the groups' (64 bits), or the candidates;
 // then a byte per group.  (8 of 32 doubles left over: the teams of a wavefront start 16 banks apart.)
@@ -149,7 +152,7 @@ __device__ __forceinline__ void group_values(const RouteCall& p, const double (&
 // Which items lie in a kept group, a bit per item of the lane.  `unsure` when the values are not exact
 // and a kept group's lies too close to one that was left.
 template <typename C, int L, int ITEMS>
-__device__ __forceinline__ uint32_t kept_items(const RouteCall& p, const C* sums, uint8_t* kept, bool exact, int lane, bool& unsure) {
+__device__ __forceinline__ uint32_t kept_items(const RouteCall& p, const C* sums, uint8_t* kept, bool exact, float scores, int lane, bool& unsure) {
     const C none = -std::numeric_limits<C>::infinity();
     C worst_kept = -none, best_left = none;
     for (int g = lane; g < p.groups; g += L) {
@@ -180,7 +183,7 @@ __device__ __forceinline__ uint32_t kept_items(const RouteCall& p, const C* sums
         best_left = team_reduce<L>(best_left, [](C a, C b) { return b > a ? b : a; });
         // (a sum of two choices carries two errors)
         const float a = static_cast<float>(worst_kept), b = static_cast<float>(best_left);
-        if (best_left != none && !(a - b > 2.0f * border(a, b))) unsure = true;
+        if (best_left != none && !(a - b > 2.0f * border(scores, a, b))) unsure = true;
     }
     return open;
 }
@@ -191,10 +194,10 @@ struct RouteRow {
     uint32_t present;
     float mx, inverse;        // softmax: the largest present logit, 1 / sum of exp(x - mx)
 
-    __device__ __forceinline__ void load(const S* row, int n, int lane, bool live) {
+    __device__ __forceinline__ void load(const S* row, int n, int lane) {
         present = 0;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) x[i] = live && i * L + lane < n ? static_cast<float>(row[i * L + lane]) : kMinusInfinity;
+        for (int i = 0; i < ITEMS; ++i) x[i] = i * L + lane < n ? static_cast<float>(row[i * L + lane]) : kMinusInfinity;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) present |= (x[i] <= lowest_of<S>() ? 0u : 1u) << i;
         mx = kMinusInfinity;
@@ -216,6 +219,7 @@ struct RouteRow {
             inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
         }
     }
+    __device__ __forceinline__ float error() const { return KIND == kSoftmaxScore ? 0x1p-18f * inverse : 0x1p-20f; }      // see border()
     __device__ __forceinline__ float power(float v) const { return __builtin_amdgcn_exp2f((v - mx) * kLog2E); }
     __device__ __forceinline__ float score(float v) const {
         if constexpr (KIND == kSoftmaxScore) {
@@ -259,7 +263,7 @@ __device__ __forceinline__ int choose_exactly(const RouteCall& p, const RouteRow
         }
         wave_sync();
         group_values<L, ITEMS>(p, value, row.present, lds, lane);
-        open = kept_items<double, L, ITEMS>(p, lds, reinterpret_cast<uint8_t*>(lds + L * ITEMS), true, lane, unsure);
+        open = kept_items<double, L, ITEMS>(p, lds, reinterpret_cast<uint8_t*>(lds + L * ITEMS), true, 0.0f, lane, unsure);
     }
     uint64_t image[ITEMS];
 #pragma unroll
@@ -284,7 +288,7 @@ __device__ __forceinline__ int choose_exactly(const RouteCall& p, const RouteRow
     return mine;
 }
 
-// The k choices in fp32 (k < L): place t ends in lane t.  `unsure` when they may not be the exact ones.
+// The k choices in fp32: place t ends in lane t.  `unsure` when they may not be the exact ones.
 template <typename S, int KIND, int L, int ITEMS>
 __device__ __forceinline__ int choose(const RouteCall& p, const RouteRow<S, KIND, L, ITEMS>& row, const S* x, float* lds, int lane, bool& unsure) {
     uint32_t image[ITEMS];
@@ -304,7 +308,7 @@ __device__ __forceinline__ int choose(const RouteCall& p, const RouteRow<S, KIND
             for (int i = 0; i < ITEMS; ++i) v[i] = p.bias || exact ? c[i] : row.score(row.x[i]);
             wave_sync();
             group_values<L, ITEMS>(p, v, row.present, lds, lds + L * ITEMS, lane);
-            open = kept_items<float, L, ITEMS>(p, lds + L * ITEMS, reinterpret_cast<uint8_t*>(lds + 2 * L * ITEMS), exact, lane, unsure);
+            open = kept_items<float, L, ITEMS>(p, lds + L * ITEMS, reinterpret_cast<uint8_t*>(lds + 2 * L * ITEMS), exact, row.error(), lane, unsure);
         }
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
@@ -319,7 +323,7 @@ __device__ __forceinline__ int choose(const RouteCall& p, const RouteRow<S, KIND
         most = keep_better == (other > most) ? other : most;
     });
     const int base = lane_id() & ~(L - 1);
-    uint32_t bound = lane_get(most, base + p.k);
+    uint32_t bound = p.k < L ? lane_get(most, base + p.k) : 0;
     if (bound == 0) bound = 1;
     int count = 0;
 #pragma unroll
@@ -370,14 +374,33 @@ __device__ __forceinline__ int choose(const RouteCall& p, const RouteRow<S, KIND
         mine = other > mine ? other : mine;
         sort(mine);
     }
-    if (total > SLOTS) unsure = true;
+    if (__any(total > SLOTS)) {
+        // (equal logits in masses) one after the other
+        uint64_t word = 0;
+        for (int t = 0; t <= p.k; ++t) {
+            uint64_t best = 0;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const uint64_t w = static_cast<uint64_t>(image[i]) << 32 | (0xffffffffu - static_cast<uint32_t>(i * L + lane));
+                if (image[i] && w > best) best = w;
+            }
+            best = team_reduce<L>(best, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+            const int e = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                if (i * L + lane == e) image[i] = 0;
+            if (lane == t) word = best;
+        }
+        if (total > SLOTS) mine = word;
+    }
     if (p.bias) {
         // neighbours too close for fp32; equal logits with equal biases are equal, whatever the precision
         const uint64_t next = lane_get(mine, base + ((lane + 1) & (L - 1)));
         const uint32_t a = static_cast<uint32_t>(mine >> 32), b = static_cast<uint32_t>(next >> 32);
-        if (lane < p.k && a > 1 && b > 1) {
+        if (p.k == L && lane == p.k - 1) unsure = true;           // (no lane for the place behind the last)
+        else if (lane < p.k && a > 1 && b > 1) {
             const float va = value_of(a), vb = value_of(b);
-            if (!(va - vb > border(va, vb))) {
+            if (!(va - vb > border(row.error(), va, vb))) {
                 const int ea = static_cast<int>(0xffffffffu - static_cast<uint32_t>(mine)), eb = static_cast<int>(0xffffffffu - static_cast<uint32_t>(next));
                 const bool equal = static_cast<float>(x[ea]) == static_cast<float>(x[eb]) && p.bias[ea] == p.bias[eb];
                 // (the last place against the first one left out: others of that value may follow unseen)
@@ -388,53 +411,90 @@ __device__ __forceinline__ int choose(const RouteCall& p, const RouteRow<S, KIND
     return static_cast<int>(0xffffffffu - static_cast<uint32_t>(mine));
 }
 
+// What place `lane` < k of row r gets once its expert e is settled.
+constexpr int32_t kUnsettled = -1;
+template <typename S, int KIND, int L, int ITEMS>
+__device__ __forceinline__ void settle(const RouteCall& p, const RouteRow<S, KIND, L, ITEMS>& row, const S* xr, int e, int64_t r, bool live, int lane,
+                                       int32_t* histogram) {
+    float s = 0.0f, total = 1.0f;
+    const bool place = lane < p.k;
+    const float v = place ? static_cast<float>(xr[e]) : kMinusInfinity;
+    const bool there = place && !(v <= lowest_of<S>());
+    if (KIND == kSoftmaxScore && p.renormalise) {
+        // the chosen logits' own softmax: what all scores have in common cancels
+        const float top = team_reduce<L>(there ? v : kMinusInfinity, [](float a, float b) { return fmaxf(a, b); });
+        if (there) s = __builtin_amdgcn_exp2f((v - top) * kLog2E);
+    } else if (there) {
+        s = row.score(v);
+    }
+    if (p.renormalise) {
+        total = team_reduce<L>(s, [](float a, float b) { return a + b; });
+        if (total == 0.0f) total = 1.0f;
+    }
+    if (live && place) {
+        p.weights[r * p.k + lane] = p.renormalise ? s / total * p.scale : s * p.scale;
+        p.indices[r * p.k + lane] = e;
+        if (p.loads) atomicAdd(&histogram[e], 1);
+    }
+}
+
+__device__ __forceinline__ void clear_loads(const RouteCall& p, int32_t* histogram) {
+    if (!p.loads) return;
+    for (int e = threadIdx.x; e < p.n; e += 256) histogram[e] = 0;
+    __syncthreads();
+}
+__device__ __forceinline__ void flush_loads(const RouteCall& p, int32_t* histogram) {
+    if (!p.loads) return;
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.n; e += 256)
+        if (histogram[e]) atomicAdd(&p.loads[e], histogram[e]);
+}
+
 template <typename S, int KIND, int L, int ITEMS>
 __global__ __launch_bounds__(256) void route_rows(const S* x, RouteCall p) {
     constexpr int TEAMS = 256 / L;
     __shared__ double lds[TEAMS][team_doubles<L, ITEMS>()];
     __shared__ int32_t histogram[L * ITEMS];
     const int lane = threadIdx.x % L, team = threadIdx.x / L;
-    if (p.loads) {
-        for (int e = threadIdx.x; e < p.n; e += 256) histogram[e] = 0;
-        __syncthreads();
-    }
+    clear_loads(p, histogram);
     for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * TEAMS; r0 < p.m; r0 += static_cast<int64_t>(gridDim.x) * TEAMS) {
         const int64_t r = r0 + team;
         const bool live = r < p.m;
         const S* xr = x + (live ? r : 0) * p.stride;
         RouteRow<S, KIND, L, ITEMS> row;
-        row.load(xr, p.n, lane, true);
+        row.load(xr, p.n, lane);
         if (p.bias || p.kept_groups < p.groups || !p.renormalise) row.normalise();
-        bool unsure = p.k >= L;
-        int e = 0;
-        if (p.k < L) e = choose<S, KIND, L, ITEMS>(p, row, xr, reinterpret_cast<float*>(lds[team]), lane, unsure);
-        if (__any(unsure)) e = choose_exactly<S, KIND, L, ITEMS>(p, row, lds[team], lane);
-        float s = 0.0f, total = 1.0f;
-        const bool place = lane < p.k;
-        const float v = place ? static_cast<float>(xr[e]) : kMinusInfinity;
-        const bool there = place && !(v <= lowest_of<S>());
-        if (KIND == kSoftmaxScore && p.renormalise) {
-            // the chosen logits' own softmax: what all scores have in common cancels
-            const float top = team_reduce<L>(there ? v : kMinusInfinity, [](float a, float b) { return fmaxf(a, b); });
-            if (there) s = __builtin_amdgcn_exp2f((v - top) * kLog2E);
-        } else if (there) {
-            s = row.score(v);
+        bool unsure = false;
+        const int e = choose<S, KIND, L, ITEMS>(p, row, xr, reinterpret_cast<float*>(lds[team]), lane, unsure);
+        if (team_reduce<L>(static_cast<int>(unsure), [](int a, int b) { return a | b; })) {
+            if (live && lane == 0) p.indices[r * p.k] = kUnsettled;
+            continue;
         }
-        if (p.renormalise) {
-            total = team_reduce<L>(s, [](float a, float b) { return a + b; });
-            if (total == 0.0f) total = 1.0f;
-        }
-        if (live && place) {
-            p.weights[r * p.k + lane] = p.renormalise ? s / total * p.scale : s * p.scale;
-            p.indices[r * p.k + lane] = e;
-            if (p.loads) atomicAdd(&histogram[e], 1);
-        }
+        settle<S, KIND, L, ITEMS>(p, row, xr, e, r, live, lane, histogram);
     }
-    if (p.loads) {
-        __syncthreads();
-        for (int e = threadIdx.x; e < p.n; e += 256)
-            if (histogram[e]) atomicAdd(&p.loads[e], histogram[e]);
+    flush_loads(p, histogram);
+}
+
+// Rows that route_rows left marked: kRowsPerWave neighbouring rows to a wavefront.
+constexpr int kRowsPerWave = 16;
+template <typename S, int KIND, int ITEMS>
+__global__ __launch_bounds__(256) void route_unsettled(const S* x, RouteCall p) {
+    __shared__ double lds[4][kWave * ITEMS + kWave * ITEMS / 8];
+    __shared__ int32_t histogram[kWave * ITEMS];
+    const int lane = lane_id(), wave = threadIdx.x / kWave;
+    clear_loads(p, histogram);
+    const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * 4 + wave) * kRowsPerWave;
+    const bool marked = lane < kRowsPerWave && r0 + lane < p.m && p.indices[(r0 + lane) * p.k] == kUnsettled;
+    for (uint64_t rows = __ballot(marked); rows; rows &= rows - 1) {
+        const int64_t r = r0 + __builtin_ctzll(rows);
+        const S* xr = x + r * p.stride;
+        RouteRow<S, KIND, kWave, ITEMS> row;
+        row.load(xr, p.n, lane);
+        row.normalise();
+        const int e = choose_exactly<S, KIND, kWave, ITEMS>(p, row, lds[wave], lane);
+        settle<S, KIND, kWave, ITEMS>(p, row, xr, e, r, true, lane, histogram);
     }
+    flush_loads(p, histogram);
 }
 
 struct RouteGradCall {
@@ -464,7 +524,7 @@ __global__ __launch_bounds__(256) void route_grad_rows(const S* x, S* dx, RouteG
 
     RouteRow<S, KIND, L, ITEMS> row;
     if (!(KIND == kSoftmaxScore && p.renormalise)) {
-        row.load(xr, p.n, lane, true);
+        row.load(xr, p.n, lane);
         row.normalise();
     }
     float grad[ITEMS];
@@ -585,7 +645,18 @@ extern "C" int dlfx_route(dlfx_stream_t stream, const char* name, int dtype, int
                 DLFX_CHECK_LAUNCH();
                 return static_cast<int>(DLFX_OK);
             };
-            return kind == kSoftmaxScore ? run(route_rows<S, kSoftmaxScore, L, ITEMS>) : run(route_rows<S, kSigmoidScore, L, ITEMS>);
+            auto again = [&](auto kernel) {
+                kernel<<<dim3(static_cast<unsigned>(ceil_div(m, 4 * kRowsPerWave))), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+                    static_cast<const S*>(x) + x_offset, p);
+                DLFX_CHECK_LAUNCH();
+                return static_cast<int>(DLFX_OK);
+            };
+            const bool exact = !bias && (kept_groups == groups || group_best == 1);
+            int status = kind == kSoftmaxScore ? run(route_rows<S, kSoftmaxScore, L, ITEMS>) : run(route_rows<S, kSigmoidScore, L, ITEMS>);
+            if (status != DLFX_OK || exact) return status;
+            // (a team of 16 lanes has up to 256 experts: four to a lane of a wavefront)
+            constexpr int MANY = L == 16 ? 4 : ITEMS;
+            return kind == kSoftmaxScore ? again(route_unsettled<S, kSoftmaxScore, MANY>) : again(route_unsettled<S, kSigmoidScore, MANY>);
         });
     });
 }
