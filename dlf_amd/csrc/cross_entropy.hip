@@ -1,5 +1,16 @@
 // Softmax cross entropy of the rows of a matrix of logits, whole or in pieces of the vocabulary,
 // and its gradient.
+//
+// Bandwidth bound: a loss reads the logits once, a gradient reads them once and writes as many.
+//   * Loss and gradient in one call, rows that fit a workgroup's registers: the row is read once, its
+//     maximum and sum go over the workgroup, the gradient leaves from the registers; a register that
+//     has been stored takes the next row's elements at once, so loads and stores overlap.
+//   * Everything else is cut into tiles of a row: a tile leaves its maximum and sum (a record, or the
+//     row's result where it has one tile), and the gradient of a tile folds the row's few records.
+// Sums and maxima are fp32; exponentials are the hardware's 2^x of (x - maximum) log2(e), where the
+// difference comes first: it is exact for neighbours, whatever the logits' common offset.
+#include <atomic>
+
 #include "sequence.hip.h"
 
 namespace dlfx {
@@ -10,40 +21,51 @@ struct MaxSum {
     float mx, sum;
 };
 constexpr float kNone = -std::numeric_limits<float>::infinity();
+constexpr float kLargest = std::numeric_limits<float>::max();
+
+__device__ __forceinline__ float exp_diff(float x, float mx) { return __builtin_amdgcn_exp2f((x - mx) * kLog2E); }
 
 __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b) {
     const float mx = fmaxf(a.mx, b.mx);
     // an empty side (maximum -inf) adds its sum of 0, or the NaN that the side has met
-    const float fa = a.mx == mx ? 1.0f : expf(a.mx - mx);
-    const float fb = b.mx == mx ? 1.0f : expf(b.mx - mx);
+    const float fa = a.mx == mx ? 1.0f : exp_diff(a.mx, mx);
+    const float fb = b.mx == mx ? 1.0f : exp_diff(b.mx, mx);
     return {mx, a.sum * fa + b.sum * fb};
 }
-__device__ __forceinline__ void fold(MaxSum& s, float x) {
-    if (x > s.mx) {
-        s.sum = s.sum * expf(s.mx - x) + 1.0f;
-        s.mx = x;
-    } else if (x != kNone) {
-        s.sum += x == s.mx ? 1.0f : expf(x - s.mx);        // NaN: the sum is NaN from here on
-    }
+
+// Folds N values in.  Differences are taken to a finite maximum: -inf adds 0 to an empty row, +inf
+// makes the sum infinite, a NaN stays.
+template <int N>
+__device__ __forceinline__ void fold(MaxSum& s, const float (&v)[N]) {
+    float mx = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) mx = fmaxf(mx, v[i]);
+    mx = fmaxf(mx, s.mx);
+    const float to = fminf(fmaxf(mx, -kLargest), kLargest);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum += exp_diff(v[i], to);
+    s.sum = (s.mx == mx ? s.sum : s.sum * exp_diff(s.mx, to)) + sum;
+    s.mx = mx;
 }
 
-template <int WAVES>
+// Over the T threads of a workgroup; every thread gets the result.  Two uses in a row need different
+// `lds` or a barrier between them.
+template <int T>
 __device__ __forceinline__ MaxSum block_join(MaxSum v, MaxSum* lds) {
+    constexpr int WAVES = T / kWave;
     v = wave_reduce(v, join);
-    __syncthreads();
     if (lane_id() == 0) lds[threadIdx.x / kWave] = v;
     __syncthreads();
-    v = lds[0];
-#pragma unroll
-    for (int i = 1; i < WAVES; ++i) v = join(v, lds[i]);
-    return v;
+    v = lds[lane_id() % WAVES];
+    return group_reduce(v, WAVES, join);
 }
 
 // Loss of a finished row.  log(sum) + (maximum - logit) in this order: the difference is exact for
 // nearby values, maximum + log(sum) would round at the maximum's size.
 __device__ __forceinline__ float loss_of(MaxSum s, float logit, float z) {
-    const float log_sum = logf(s.sum);
     if (s.sum == 0.0f) return std::numeric_limits<float>::infinity();
+    const float log_sum = logf(s.sum);
     float loss = log_sum + (s.mx - logit);
     if (z != 0.0f) {
         const float lse = s.mx + log_sum;
@@ -52,60 +74,187 @@ __device__ __forceinline__ float loss_of(MaxSum s, float logit, float z) {
     return loss;
 }
 
-// What the elements of a row's gradient have in common: dx = up (factor exp(x - mx) - [target]).
+// What the elements of a row's gradient have in common: dx = p * exp(x - mx) - [target] * up.
 struct RowGrad {
-    float mx, factor, up;
-    int64_t target;
+    float mx, p, up;
+    bool zero;                // a row without a target, or of nothing but -inf
 };
-__device__ __forceinline__ RowGrad row_grad(MaxSum s, int64_t target, float weight, float z) {
-    RowGrad g = {s.mx, 0.0f, weight, target};
-    if (target < 0) g.up = 0.0f;
-    else if (s.sum == 0.0f) g.up = 0.0f;          // nothing but -inf
-    else {
-        g.factor = 1.0f / s.sum;
-        if (z != 0.0f) g.factor *= 1.0f + 2.0f * z * (s.mx + logf(s.sum));
-    }
+__device__ __forceinline__ RowGrad row_grad(MaxSum s, bool live, float weight, float z) {
+    RowGrad g = {fminf(fmaxf(s.mx, -kLargest), kLargest), 0.0f, weight, !live || s.sum == 0.0f};
+    float factor = 1.0f / s.sum;
+    if (z != 0.0f) factor *= 1.0f + 2.0f * z * (s.mx + logf(s.sum));
+    g.p = weight * factor;
     return g;
 }
-__device__ __forceinline__ float grad_of(const RowGrad& g, float x, int64_t j) {
-    if (g.up == 0.0f && (g.target < 0 || g.factor == 0.0f)) return 0.0f;
-    float p = g.factor * expf(x - g.mx);
-    if (j == g.target) p -= 1.0f;
-    return g.up * p;
+
+template <typename S> constexpr int vector_width() { return 16 / static_cast<int>(sizeof(S)); }
+
+// V elements from position e0 of a row of n, as they are stored; -inf past the end.
+template <typename S>
+__device__ __forceinline__ typename AnyVec<S, vector_width<S>()>::type load_part(const S* row, int64_t e0, int64_t n) {
+    constexpr int V = vector_width<S>();
+    using VecT = typename AnyVec<S, V>::type;
+    if (e0 + V <= n) return __builtin_nontemporal_load(reinterpret_cast<const VecT*>(row + e0));
+    VecT v;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = e0 + i < n ? row[e0 + i] : static_cast<S>(kNone);
+    return v;
+}
+template <typename S>
+__device__ __forceinline__ void grad_part(S* row, int64_t e0, int64_t n, const typename AnyVec<S, vector_width<S>()>::type& x, const RowGrad& g,
+                                          int64_t target) {
+    constexpr int V = vector_width<S>();
+    using VecT = typename AnyVec<S, V>::type;
+    float v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = g.p * exp_diff(static_cast<float>(x[i]), g.mx);
+    const uint64_t at = static_cast<uint64_t>(target - e0);
+    if (at < V) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (at == static_cast<uint64_t>(i)) v[i] -= g.up;
+    }
+    VecT out;
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = static_cast<S>(g.zero ? 0.0f : v[i]);
+    if (e0 + V <= n) {
+        __builtin_nontemporal_store(out, reinterpret_cast<VecT*>(row + e0));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (e0 + i < n) row[e0 + i] = out[i];
+    }
 }
 
-// One workgroup per row.
-template <typename S, typename I>
-__global__ __launch_bounds__(256) void loss_rows(const S* x, int64_t n, int64_t stride, const I* targets, int64_t first, int resume,
-                                                 float* state, int64_t m, float z, float* loss) {
-    __shared__ MaxSum lds[4];
-    const int64_t r = blockIdx.x;
-    const S* xr = x + r * stride;
-    const int64_t target = static_cast<int64_t>(targets[r]);
-    if (target < 0) {
-        if (threadIdx.x == 0) {
-            if (loss) loss[r] = 0.0f;
-            else if (!resume) state[r] = kNone, state[m + r] = 0.0f, state[2 * m + r] = std::numeric_limits<float>::quiet_NaN();
+// Loss and gradient of whole rows held in registers, NV vectors to a thread; a workgroup takes every
+// gridDim-th row.
+template <typename S, typename I, int NV, int T>
+__global__ __launch_bounds__(T) void grad_rows_held(const S* x, int64_t m, int64_t n, int64_t stride, const I* targets, const float* weights, float z,
+                                                    float* loss, S* dx, int64_t dx_stride) {
+    constexpr int V = vector_width<S>();
+    using VecT = typename AnyVec<S, V>::type;
+    __shared__ MaxSum lds[2][T / kWave];
+    VecT raw[NV];
+    int64_t r = blockIdx.x;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) raw[j] = load_part(x + r * stride, (j * T + static_cast<int64_t>(threadIdx.x)) * V, n);
+    for (int parity = 0; r < m; r += gridDim.x, parity ^= 1) {
+        const int64_t target = static_cast<int64_t>(targets[r]);
+        const float weight = weights ? weights[r] : 1.0f;
+        float logit = std::numeric_limits<float>::quiet_NaN();
+        if (threadIdx.x == 0 && loss && target >= 0 && target < n) logit = static_cast<float>(x[r * stride + target]);
+        MaxSum s = {kNone, 0.0f};
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float v[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = static_cast<float>(raw[j][i]);
+            fold(s, v);
         }
-        return;
+        asm volatile("" : "+v"(logit));             // (here, not later: dx may be x, and others store after the barrier)
+        s = block_join<T>(s, lds[parity]);
+        if (threadIdx.x == 0 && loss) loss[r] = target < 0 ? 0.0f : loss_of(s, logit, z);
+        const RowGrad g = row_grad(s, target >= 0, weight, z);
+        S* dr = dx + r * dx_stride;
+        const int64_t next = r + gridDim.x;
+        const S* xn = x + next * stride;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t e0 = (j * T + static_cast<int64_t>(threadIdx.x)) * V;
+            grad_part(dr, e0, n, raw[j], g, target);
+            if (next < m) raw[j] = load_part(xn, e0, n);
+        }
     }
-    MaxSum v = {kNone, 0.0f};
-    for (int64_t j = threadIdx.x; j < n; j += 256) fold(v, static_cast<float>(xr[j]));
-    v = block_join<4>(v, lds);
-    if (threadIdx.x) return;
+}
+
+// A row cut into tiles, a workgroup each: blockIdx = row * tiles + tile.
+constexpr int kTileThreads = 256;
+constexpr int kTileBatch = 4;                       // vectors of a thread in flight
+template <typename S> constexpr int64_t tile_unit() { return static_cast<int64_t>(kTileThreads) * vector_width<S>(); }
+
+struct Tiles {
+    int64_t count, length;
+};
+
+// What a call on a matrix of logits works on; state or loss is where a finished row goes.
+template <typename S, typename I>
+struct LossCall {
+    const S* x;
+    int64_t m, n, stride;
+    const I* targets;
+    int64_t first;               // column of the whole vocabulary that column 0 is
+    int resume;
+    float* state;
+    float z;
+    float* loss;
+    Tiles tiles;
+    MaxSum* records;             // tiles.count per row
+};
+
+template <typename S, typename I>
+__device__ __forceinline__ void finish_row(const LossCall<S, I>& p, int64_t r, MaxSum v) {
+    const int64_t target = static_cast<int64_t>(p.targets[r]);
     float logit = std::numeric_limits<float>::quiet_NaN();
-    if (!loss && resume) {
-        v = join({state[r], state[m + r]}, v);
-        logit = state[2 * m + r];
+    if (!p.loss && p.resume) {
+        v = join({p.state[r], p.state[p.m + r]}, v);
+        logit = p.state[2 * p.m + r];
     }
-    if (target >= first && target - first < n) logit = static_cast<float>(xr[target - first]);
-    if (loss) {
-        loss[r] = loss_of(v, logit, z);
+    if (target >= p.first && target - p.first < p.n) logit = static_cast<float>(p.x[r * p.stride + (target - p.first)]);
+    if (p.loss) {
+        p.loss[r] = target < 0 ? 0.0f : loss_of(v, logit, p.z);
     } else {
-        state[r] = v.mx;
-        state[m + r] = v.sum;
-        state[2 * m + r] = logit;
+        p.state[r] = v.mx;
+        p.state[p.m + r] = v.sum;
+        p.state[2 * p.m + r] = logit;
     }
+}
+
+// A tile's record, or with one tile to a row the row's result.
+template <typename S, typename I>
+__global__ __launch_bounds__(kTileThreads) void loss_tiles(LossCall<S, I> p) {
+    constexpr int V = vector_width<S>();
+    __shared__ MaxSum lds[kTileThreads / kWave];
+    const uint32_t tiles = static_cast<uint32_t>(p.tiles.count);
+    const int64_t r = blockIdx.x / tiles, tile = blockIdx.x % tiles;
+    const S* xr = p.x + r * p.stride;
+    const int64_t begin = tile * p.tiles.length;
+    const int64_t end = begin + p.tiles.length < p.n ? begin + p.tiles.length : p.n;
+    MaxSum s = {kNone, 0.0f};
+    for (int64_t e0 = begin + static_cast<int64_t>(threadIdx.x) * V; e0 < end; e0 += kTileBatch * tile_unit<S>()) {
+        typename AnyVec<S, V>::type raw[kTileBatch];
+#pragma unroll
+        for (int u = 0; u < kTileBatch; ++u) {
+            const int64_t e = e0 + u * tile_unit<S>();
+            if (e < end) raw[u] = load_part(xr, e, end);
+        }
+#pragma unroll
+        for (int u = 0; u < kTileBatch; ++u) {
+            if (e0 + u * tile_unit<S>() >= end) break;
+            float v[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = static_cast<float>(raw[u][i]);
+            fold(s, v);
+        }
+    }
+    s = block_join<kTileThreads>(s, lds);
+    if (threadIdx.x) return;
+    if (p.tiles.count > 1 || !(p.loss || p.state)) p.records[blockIdx.x] = s;
+    else finish_row(p, r, s);
+}
+
+__device__ __forceinline__ MaxSum join_records(const MaxSum* records, int64_t count) {
+    MaxSum s = {kNone, 0.0f};
+    for (int64_t t = lane_id(); t < count; t += kWave) s = join(s, records[t]);
+    return wave_reduce(s, join);
+}
+
+// One wavefront per row joins its records.
+template <typename S, typename I>
+__global__ __launch_bounds__(256) void loss_join_tiles(LossCall<S, I> p) {
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
+    if (r >= p.m) return;
+    const MaxSum s = join_records(p.records + r * p.tiles.count, p.tiles.count);
+    if (lane_id() == 0) finish_row(p, r, s);
 }
 
 template <typename I>
@@ -115,27 +264,36 @@ __global__ __launch_bounds__(256) void loss_join(int64_t m, const I* targets, co
     loss[r] = targets[r] < 0 ? 0.0f : loss_of({state[r], state[m + r]}, state[2 * m + r], z);
 }
 
+// Gradient of a tile: the row's maximum and sum come from the state or from the records.
 template <typename S, typename I>
-__global__ __launch_bounds__(256) void grad_rows(const S* x, int64_t n, int64_t stride, const I* targets, int64_t first, const float* state,
-                                                 const float* weights, float z, int64_t m, float* loss, S* dx, int64_t dx_stride) {
-    __shared__ MaxSum lds[4];
-    const int64_t r = blockIdx.x;
-    const S* xr = x + r * stride;
+__global__ __launch_bounds__(kTileThreads) void grad_tiles(LossCall<S, I> p, int64_t record_count, const float* weights, S* dx, int64_t dx_stride) {
+    constexpr int V = vector_width<S>();
+    const uint32_t tiles = static_cast<uint32_t>(p.tiles.count);
+    const int64_t r = blockIdx.x / tiles, tile = blockIdx.x % tiles;
+    const S* xr = p.x + r * p.stride;
     S* dr = dx + r * dx_stride;
-    const int64_t target = static_cast<int64_t>(targets[r]);
-    MaxSum v = {kNone, 0.0f};
-    if (state) {
-        v = {state[r], state[m + r]};
-    } else if (target >= 0) {
-        for (int64_t j = threadIdx.x; j < n; j += 256) fold(v, static_cast<float>(xr[j]));
-        v = block_join<4>(v, lds);
-        if (loss && threadIdx.x == 0) loss[r] = loss_of(v, target < n ? static_cast<float>(xr[target]) : std::numeric_limits<float>::quiet_NaN(), z);
-        __syncthreads();
-    } else if (loss && threadIdx.x == 0) {
-        loss[r] = 0.0f;
+    const int64_t begin = tile * p.tiles.length;
+    const int64_t end = begin + p.tiles.length < p.n ? begin + p.tiles.length : p.n;
+    const int64_t target = static_cast<int64_t>(p.targets[r]);
+    const float weight = weights ? weights[r] : 1.0f;
+    MaxSum s;
+    if (p.state) s = {p.state[r], p.state[p.m + r]};
+    else s = join_records(p.records + r * record_count, record_count);
+    const RowGrad g = row_grad(s, target >= 0, weight, p.z);
+    const int64_t here = target < 0 ? -1 : target - p.first;
+    for (int64_t e0 = begin + static_cast<int64_t>(threadIdx.x) * V; e0 < end; e0 += kTileBatch * tile_unit<S>()) {
+        typename AnyVec<S, V>::type raw[kTileBatch];
+#pragma unroll
+        for (int u = 0; u < kTileBatch; ++u) {
+            const int64_t e = e0 + u * tile_unit<S>();
+            if (e < end && !g.zero) raw[u] = load_part(xr, e, end);
+        }
+#pragma unroll
+        for (int u = 0; u < kTileBatch; ++u) {
+            const int64_t e = e0 + u * tile_unit<S>();
+            if (e < end) grad_part(dr, e, end, raw[u], g, here);
+        }
     }
-    const RowGrad g = row_grad(v, target, weights ? weights[r] : 1.0f, z);
-    for (int64_t j = threadIdx.x; j < n; j += 256) dr[j] = static_cast<S>(grad_of(g, static_cast<float>(xr[j]), first + j));
 }
 
 template <typename F>
@@ -151,27 +309,151 @@ int check(int64_t m, int64_t n, const void* x, int64_t row_stride, const void* t
     return DLFX_OK;
 }
 
+// Tiles of a pass that joins (records of scratch: about 2048 workgroups, none under 8 KB) and of one
+// that only writes gradients (16 KB each, whatever their number).
+template <typename S>
+Tiles joining_tiles(int64_t m, int64_t n) {
+    constexpr int64_t unit = tile_unit<S>();
+    int64_t count = ceil_div(2048, m);
+    const int64_t most = ceil_div(n, 2 * unit);
+    if (count > most) count = most;
+    if (count < 1) count = 1;
+    const int64_t length = ceil_div(ceil_div(n, count), unit) * unit;
+    return {ceil_div(n, length), length};
+}
+template <typename S>
+Tiles writing_tiles(int64_t n) {
+    const int64_t length = kTileBatch * tile_unit<S>();
+    return {ceil_div(n, length), length};
+}
+
+// Longest row that a workgroup's registers hold.
+template <typename S> constexpr int64_t held_most() { return 16 * 1024 * vector_width<S>(); }
+
+// Records of the tiles; calls that make none ask for nothing.
+template <typename S>
+size_t scratch_of(int64_t m, int64_t n) {
+    const int64_t count = joining_tiles<S>(m, n).count;
+    return count > 1 || n > held_most<S>() ? static_cast<size_t>(m * count) * sizeof(MaxSum) : 0;
+}
+
+// Workgroups of a kernel that the current device holds at once, asked for once per device.
+template <auto KERNEL>
+int64_t resident(int threads) {
+    static std::atomic<int64_t> known[64];
+    int device = 0;
+    if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64) return resident_workgroups(KERNEL, threads);
+    int64_t n = known[device].load(std::memory_order_relaxed);
+    if (n == 0) known[device].store(n = resident_workgroups(KERNEL, threads), std::memory_order_relaxed);
+    return n;
+}
+
+template <typename S, typename I>
+int launch_loss(LossCall<S, I> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
+    p.tiles = joining_tiles<S>(p.m, p.n);
+    if (p.tiles.count > 1 && (!scratch || scratch_bytes < scratch_of<S>(p.m, p.n))) p.tiles = {1, p.n};
+    if (p.m * p.tiles.count > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
+    p.records = static_cast<MaxSum*>(scratch);
+    loss_tiles<S, I><<<dim3(static_cast<unsigned>(p.m * p.tiles.count)), dim3(kTileThreads), 0, stream>>>(p);
+    DLFX_CHECK_LAUNCH();
+    if (p.tiles.count > 1) {
+        loss_join_tiles<S, I><<<dim3(static_cast<unsigned>(ceil_div(p.m, 4))), dim3(256), 0, stream>>>(p);
+        DLFX_CHECK_LAUNCH();
+    }
+    return DLFX_OK;
+}
+
+template <typename S, typename I>
+int launch_grad_tiles(LossCall<S, I> p, int64_t record_count, const float* weights, S* dx, int64_t dx_stride, hipStream_t stream) {
+    p.tiles = writing_tiles<S>(p.n);
+    if (p.m * p.tiles.count > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
+    grad_tiles<S, I><<<dim3(static_cast<unsigned>(p.m * p.tiles.count)), dim3(kTileThreads), 0, stream>>>(p, record_count, weights, dx, dx_stride);
+    DLFX_CHECK_LAUNCH();
+    return DLFX_OK;
+}
+
+template <typename S, typename I>
+int launch_grad(LossCall<S, I> p, const float* weights, S* dx, int64_t dx_stride, void* scratch, size_t scratch_bytes, hipStream_t stream) {
+    auto held = [&](auto vectors, auto team) {
+        constexpr int NV = decltype(vectors)::value, T = decltype(team)::value;
+        // as many workgroups as the device holds: each goes on to its next row while it stores the last
+        const int64_t most = resident<grad_rows_held<S, I, NV, T>>(T);
+        const int64_t blocks = most > 0 && most < p.m ? most : p.m;
+        grad_rows_held<S, I, NV, T><<<dim3(static_cast<unsigned>(blocks)), dim3(T), 0, stream>>>(p.x, p.m, p.n, p.stride, p.targets, weights, p.z, p.loss,
+                                                                                              dx, dx_stride);
+        DLFX_CHECK_LAUNCH();
+        return static_cast<int>(DLFX_OK);
+    };
+    using std::integral_constant;
+    constexpr int64_t V = vector_width<S>();
+    const size_t need = scratch_of<S>(p.m, p.n);
+    const bool has_scratch = need && scratch && scratch_bytes >= need;
+    const integral_constant<int, 256> few;
+    const integral_constant<int, 1024> many;
+    if (p.n <= 256 * V) return held(integral_constant<int, 1>(), few);
+    if (p.n <= 512 * V) return held(integral_constant<int, 2>(), few);
+    if (p.n <= 1024 * V) return held(integral_constant<int, 4>(), few);
+    if (p.n <= held_most<S>() && (p.m >= 192 || !has_scratch)) {
+        if (p.n <= 2 * 1024 * V) return held(integral_constant<int, 2>(), many);
+        if (p.n <= 3 * 1024 * V) return held(integral_constant<int, 3>(), many);
+        if (p.n <= 4 * 1024 * V) return held(integral_constant<int, 4>(), many);
+        if (p.n <= 6 * 1024 * V) return held(integral_constant<int, 6>(), many);
+        if (p.n <= 8 * 1024 * V) return held(integral_constant<int, 8>(), many);
+        if (p.n <= 12 * 1024 * V) return held(integral_constant<int, 12>(), many);
+        return held(integral_constant<int, 16>(), many);
+    }
+    if (!has_scratch) return DLFX_ERR_SCRATCH_TOO_SMALL;
+    // the records first, then the losses (the target's logit is read before dx, which may be x, is
+    // written), then the gradients tile by tile
+    LossCall<S, I> q = p;
+    q.tiles = joining_tiles<S>(p.m, p.n);
+    if (p.m * q.tiles.count > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
+    q.records = static_cast<MaxSum*>(scratch);
+    float* loss = q.loss;
+    q.loss = nullptr;
+    loss_tiles<S, I><<<dim3(static_cast<unsigned>(p.m * q.tiles.count)), dim3(kTileThreads), 0, stream>>>(q);
+    DLFX_CHECK_LAUNCH();
+    if (loss) {
+        q.loss = loss;
+        loss_join_tiles<S, I><<<dim3(static_cast<unsigned>(ceil_div(p.m, 4))), dim3(256), 0, stream>>>(q);
+        DLFX_CHECK_LAUNCH();
+    }
+    return launch_grad_tiles(q, q.tiles.count, weights, dx, dx_stride, stream);
+}
+
 }  // namespace
 }  // namespace dlfx
 
 using namespace dlfx;
 
-extern "C" size_t dlfx_cross_entropy_scratch_bytes(int, int64_t, int64_t) { return 0; }
+extern "C" size_t dlfx_cross_entropy_scratch_bytes(int dtype, int64_t m, int64_t n) {
+    if (m <= 0 || n <= 0 || m > 0x7fffffffLL || n > 0x7fffffffLL) return 0;
+    switch (dtype) {
+    case DLFX_F32: return scratch_of<float>(m, n);
+    case DLFX_F16: return scratch_of<half_t>(m, n);
+    case DLFX_BF16: return scratch_of<bf16_t>(m, n);
+    default: return 0;
+    }
+}
+
+// f(element, index, stream): dispatches a matrix call's types.
+template <typename F>
+static int with_types(dlfx_stream_t stream, int dtype, int index_dtype, F&& f) {
+    return dispatch_sequence_dtype(dtype, [&](auto tag) {
+        return dispatch_index(index_dtype, [&](auto index) { return static_cast<int>(f(tag, index, static_cast<hipStream_t>(stream))); });
+    });
+}
 
 extern "C" int dlfx_cross_entropy(dlfx_stream_t stream, int dtype, int index_dtype, int64_t m, int64_t n,
                                   const void* x, int64_t x_offset, int64_t row_stride, const void* targets,
                                   float z_loss, float* loss, void* scratch, size_t scratch_bytes) {
     if (int e = check(m, n, x, row_stride, targets)) return e;
     if (!loss) return DLFX_ERR_INVALID_ARGUMENT;
-    return dispatch_sequence_dtype(dtype, [&](auto tag) {
+    return with_types(stream, dtype, index_dtype, [&](auto tag, auto index, hipStream_t s) {
         using S = decltype(tag);
-        return dispatch_index(index_dtype, [&](auto index) {
-            using I = decltype(index);
-            loss_rows<S, I><<<dim3(static_cast<unsigned>(m)), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
-                static_cast<const S*>(x) + x_offset, n, row_stride, static_cast<const I*>(targets), 0, 0, nullptr, m, z_loss, loss);
-            DLFX_CHECK_LAUNCH();
-            return static_cast<int>(DLFX_OK);
-        });
+        using I = decltype(index);
+        LossCall<S, I> p{static_cast<const S*>(x) + x_offset, m, n, row_stride, static_cast<const I*>(targets), 0, 0, nullptr, z_loss, loss, {}, nullptr};
+        return launch_loss(p, scratch, scratch_bytes, s);
     });
 }
 
@@ -182,16 +464,11 @@ extern "C" int dlfx_cross_entropy_grad(dlfx_stream_t stream, int dtype, int inde
                                        void* scratch, size_t scratch_bytes) {
     if (int e = check(m, n, x, row_stride, targets)) return e;
     if (!dx || dx_row_stride < n) return DLFX_ERR_INVALID_ARGUMENT;
-    return dispatch_sequence_dtype(dtype, [&](auto tag) {
+    return with_types(stream, dtype, index_dtype, [&](auto tag, auto index, hipStream_t s) {
         using S = decltype(tag);
-        return dispatch_index(index_dtype, [&](auto index) {
-            using I = decltype(index);
-            grad_rows<S, I><<<dim3(static_cast<unsigned>(m)), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
-                static_cast<const S*>(x) + x_offset, n, row_stride, static_cast<const I*>(targets), 0, nullptr, weights, z_loss, m, loss,
-                static_cast<S*>(dx) + dx_offset, dx_row_stride);
-            DLFX_CHECK_LAUNCH();
-            return static_cast<int>(DLFX_OK);
-        });
+        using I = decltype(index);
+        LossCall<S, I> p{static_cast<const S*>(x) + x_offset, m, n, row_stride, static_cast<const I*>(targets), 0, 0, nullptr, z_loss, loss, {}, nullptr};
+        return launch_grad(p, weights, static_cast<S*>(dx) + dx_offset, dx_row_stride, scratch, scratch_bytes, s);
     });
 }
 
@@ -200,15 +477,11 @@ extern "C" int dlfx_cross_entropy_piece(dlfx_stream_t stream, int dtype, int ind
                                         int64_t first, int resume, float* state, void* scratch, size_t scratch_bytes) {
     if (int e = check(m, n, x, row_stride, targets)) return e;
     if (!state || first < 0) return DLFX_ERR_INVALID_ARGUMENT;
-    return dispatch_sequence_dtype(dtype, [&](auto tag) {
+    return with_types(stream, dtype, index_dtype, [&](auto tag, auto index, hipStream_t s) {
         using S = decltype(tag);
-        return dispatch_index(index_dtype, [&](auto index) {
-            using I = decltype(index);
-            loss_rows<S, I><<<dim3(static_cast<unsigned>(m)), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
-                static_cast<const S*>(x) + x_offset, n, row_stride, static_cast<const I*>(targets), first, resume, state, m, 0.0f, nullptr);
-            DLFX_CHECK_LAUNCH();
-            return static_cast<int>(DLFX_OK);
-        });
+        using I = decltype(index);
+        LossCall<S, I> p{static_cast<const S*>(x) + x_offset, m, n, row_stride, static_cast<const I*>(targets), first, resume, state, 0.0f, nullptr, {}, nullptr};
+        return launch_loss(p, scratch, scratch_bytes, s);
     });
 }
 
@@ -231,15 +504,11 @@ extern "C" int dlfx_cross_entropy_piece_grad(dlfx_stream_t stream, int dtype, in
                                              void* dx, int64_t dx_offset, int64_t dx_row_stride) {
     if (int e = check(m, n, x, row_stride, targets)) return e;
     if (!state || first < 0 || !dx || dx_row_stride < n) return DLFX_ERR_INVALID_ARGUMENT;
-    return dispatch_sequence_dtype(dtype, [&](auto tag) {
+    return with_types(stream, dtype, index_dtype, [&](auto tag, auto index, hipStream_t s) {
         using S = decltype(tag);
-        return dispatch_index(index_dtype, [&](auto index) {
-            using I = decltype(index);
-            grad_rows<S, I><<<dim3(static_cast<unsigned>(m)), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
-                static_cast<const S*>(x) + x_offset, n, row_stride, static_cast<const I*>(targets), first, state, weights, z_loss, m, nullptr,
-                static_cast<S*>(dx) + dx_offset, dx_row_stride);
-            DLFX_CHECK_LAUNCH();
-            return static_cast<int>(DLFX_OK);
-        });
+        using I = decltype(index);
+        LossCall<S, I> p{static_cast<const S*>(x) + x_offset, m, n, row_stride, static_cast<const I*>(targets), first, 0, const_cast<float*>(state), z_loss,
+                         nullptr, {}, nullptr};
+        return launch_grad_tiles(p, 0, weights, static_cast<S*>(dx) + dx_offset, dx_row_stride, s);
     });
 }

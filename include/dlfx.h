@@ -440,9 +440,10 @@ int dlfx_route_grad(dlfx_stream_t stream, const char* name, int dtype, int64_t m
  *   dlfx_cross_entropy_piece_grad  the gradient of a piece, from the finished state: the piece is
  *                                  computed a second time, or was kept; dx may be x.
  * The order of the pieces is free, and a state of columns seen elsewhere can be folded in (larger
- * maximum, sums scaled to it).  Scratch is optional (NULL): few long rows are cut into tiles for the
- * whole device when scratch of dlfx_cross_entropy_scratch_bytes() bytes is given, and walked by one
- * workgroup per row when it is not.
+ * maximum, sums scaled to it).  Scratch of dlfx_cross_entropy_scratch_bytes() bytes cuts few long
+ * rows into tiles for the whole device; without it (NULL) a workgroup walks each row.
+ * dlfx_cross_entropy_grad cannot do without it for rows of more than 131072 two-byte or 65536
+ * four-byte elements (DLFX_ERR_SCRATCH_TOO_SMALL).
  */
 size_t dlfx_cross_entropy_scratch_bytes(int dtype, int64_t m, int64_t n);
 int dlfx_cross_entropy(dlfx_stream_t stream, int dtype, int index_dtype, int64_t m, int64_t n,
