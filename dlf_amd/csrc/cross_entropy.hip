@@ -10,11 +10,21 @@
 // Sums and maxima are fp32; exponentials are the hardware's 2^x of (x - maximum) log2(e), where the
 // difference comes first: it is exact for neighbours, whatever the logits' common offset.
 #include <atomic>
+#include <utility>
 
 #include "sequence.hip.h"
 
 namespace dlfx {
 namespace {
+
+// The rows' target columns, 32 or 64 bits each.
+struct Targets {
+    const void* base;
+    bool wide;
+    __device__ __forceinline__ int64_t operator[](int64_t r) const {
+        return wide ? static_cast<const int64_t*>(base)[r] : static_cast<const int32_t*>(base)[r];
+    }
+};
 
 // Running maximum of a row and the sum of exp(x - maximum).
 struct MaxSum {
@@ -89,82 +99,144 @@ __device__ __forceinline__ RowGrad row_grad(MaxSum s, bool live, float weight, f
 
 template <typename S> constexpr int vector_width() { return 16 / static_cast<int>(sizeof(S)); }
 
+// A vector while it waits in registers: four words, whatever the type (vectors of 16-bit elements
+// carried round a loop would take a register per element).
+typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
+template <int BYTES> struct WordsAt;                 // in memory, on an element's boundary
+template <> struct WordsAt<2> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2), may_alias)); };
+template <> struct WordsAt<4> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4), may_alias)); };
+template <typename S>
+__device__ __forceinline__ Words4 load_words(const S* at) { return __builtin_nontemporal_load(reinterpret_cast<const typename WordsAt<sizeof(S)>::type*>(at)); }
+template <typename S>
+__device__ __forceinline__ void widen(const Words4& w, float (&v)[vector_width<S>()]) {
+    if constexpr (sizeof(S) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = bit_cast<float>(w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const Vec<S, 2> pair = bit_cast<Vec<S, 2>>(static_cast<uint32_t>(w[i]));
+            v[2 * i] = static_cast<float>(pair.v[0]);
+            v[2 * i + 1] = static_cast<float>(pair.v[1]);
+        }
+    }
+}
+
 // V elements from position e0 of a row of n, as they are stored; -inf past the end.
 template <typename S>
-__device__ __forceinline__ typename AnyVec<S, vector_width<S>()>::type load_part(const S* row, int64_t e0, int64_t n) {
+__device__ __forceinline__ Words4 load_part(const S* row, int64_t e0, int64_t n) {
     constexpr int V = vector_width<S>();
-    using VecT = typename AnyVec<S, V>::type;
-    if (e0 + V <= n) return __builtin_nontemporal_load(reinterpret_cast<const VecT*>(row + e0));
-    VecT v;
+    if (e0 + V <= n) return load_words(row + e0);
+    Vec<S, V> v;
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = e0 + i < n ? row[e0 + i] : static_cast<S>(kNone);
-    return v;
+    for (int i = 0; i < V; ++i) v.v[i] = e0 + i < n ? row[e0 + i] : static_cast<S>(kNone);
+    return bit_cast<Words4>(v);
 }
 template <typename S>
-__device__ __forceinline__ void grad_part(S* row, int64_t e0, int64_t n, const typename AnyVec<S, vector_width<S>()>::type& x, const RowGrad& g,
-                                          int64_t target) {
+__device__ __forceinline__ Vec<S, vector_width<S>()> grad_vector(int64_t e0, const Words4& x, const RowGrad& g, int64_t target) {
     constexpr int V = vector_width<S>();
-    using VecT = typename AnyVec<S, V>::type;
     float v[V];
+    widen<S>(x, v);
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = g.p * exp_diff(static_cast<float>(x[i]), g.mx);
+    for (int i = 0; i < V; ++i) v[i] = g.p * exp_diff(v[i], g.mx);
     const uint64_t at = static_cast<uint64_t>(target - e0);
     if (at < V) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if (at == static_cast<uint64_t>(i)) v[i] -= g.up;
     }
-    VecT out;
+    Vec<S, V> out;
 #pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = static_cast<S>(g.zero ? 0.0f : v[i]);
+    for (int i = 0; i < V; ++i) out.v[i] = static_cast<S>(g.zero ? 0.0f : v[i]);
+    return out;
+}
+template <typename S>
+__device__ __forceinline__ void store_whole(S* at, const Vec<S, vector_width<S>()>& v) {
+    const typename WordsAt<sizeof(S)>::type words = bit_cast<Words4>(v);
+    __builtin_nontemporal_store(words, reinterpret_cast<typename WordsAt<sizeof(S)>::type*>(at));
+}
+template <typename S>
+__device__ __forceinline__ void store_part(S* row, int64_t e0, int64_t n, const Vec<S, vector_width<S>()>& v) {
+    constexpr int V = vector_width<S>();
     if (e0 + V <= n) {
-        __builtin_nontemporal_store(out, reinterpret_cast<VecT*>(row + e0));
+        store_whole(row + e0, v);
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (e0 + i < n) row[e0 + i] = out[i];
+            if (e0 + i < n) row[e0 + i] = v.v[i];
     }
 }
 
-// Loss and gradient of whole rows held in registers, NV vectors to a thread; a workgroup takes every
-// gridDim-th row.
-template <typename S, typename I, int NV, int T>
-__global__ __launch_bounds__(T) void grad_rows_held(const S* x, int64_t m, int64_t n, int64_t stride, const I* targets, const float* weights, float z,
+// Loss and gradient of whole rows held in registers: NV vectors to a thread, the last of them at or
+// over the row's end for some; a workgroup takes every gridDim-th row.  All other loads and stores
+// are unconditional, so the next row's loads are still in flight while its first vectors are summed.
+template <typename S, int NV, int T>
+__global__ __launch_bounds__(T) void grad_rows_held(const S* x, int64_t m, int64_t n, int64_t stride, Targets targets, const float* weights, float z,
                                                     float* loss, S* dx, int64_t dx_stride) {
     constexpr int V = vector_width<S>();
-    using VecT = typename AnyVec<S, V>::type;
     __shared__ MaxSum lds[2][T / kWave];
-    VecT raw[NV];
+    const uint32_t mine = threadIdx.x * V;
+    const int64_t end = (NV - 1) * T * V + static_cast<int64_t>(mine);      // where the thread's last vector begins
+    auto load = [&](const S* row, int j) { return load_words(row + j * T * V + mine); };
+    Words4 raw[NV];
     int64_t r = blockIdx.x;
+    raw[NV - 1] = load_part(x + r * stride, end, n);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) raw[j] = load_part(x + r * stride, (j * T + static_cast<int64_t>(threadIdx.x)) * V, n);
+    for (int j = 0; j < NV - 1; ++j) raw[j] = load(x + r * stride, j);
     for (int parity = 0; r < m; r += gridDim.x, parity ^= 1) {
-        const int64_t target = static_cast<int64_t>(targets[r]);
+        const int64_t target = targets[r];
         const float weight = weights ? weights[r] : 1.0f;
-        float logit = std::numeric_limits<float>::quiet_NaN();
-        if (threadIdx.x == 0 && loss && target >= 0 && target < n) logit = static_cast<float>(x[r * stride + target]);
         MaxSum s = {kNone, 0.0f};
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             float v[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = static_cast<float>(raw[j][i]);
+            widen<S>(raw[j], v);
             fold(s, v);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        float logit = std::numeric_limits<float>::quiet_NaN();
+        if (threadIdx.x == 0 && loss && target >= 0 && target < n) logit = static_cast<float>(x[r * stride + target]);
         asm volatile("" : "+v"(logit));             // (here, not later: dx may be x, and others store after the barrier)
         s = block_join<T>(s, lds[parity]);
         if (threadIdx.x == 0 && loss) loss[r] = target < 0 ? 0.0f : loss_of(s, logit, z);
         const RowGrad g = row_grad(s, target >= 0, weight, z);
         S* dr = dx + r * dx_stride;
-        const int64_t next = r + gridDim.x;
+        const int64_t next = r + gridDim.x < m ? r + gridDim.x : r;      // (past the last row: values that nobody uses)
         const S* xn = x + next * stride;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int64_t e0 = (j * T + static_cast<int64_t>(threadIdx.x)) * V;
-            grad_part(dr, e0, n, raw[j], g, target);
-            if (next < m) raw[j] = load_part(xn, e0, n);
+        for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(raw[j]));      // (the words are kept, not the floats the sum was made of)
+#pragma unroll
+        for (int j = 0; j < NV - 1; ++j) {
+            store_whole(dr + j * T * V + mine, grad_vector<S>(j * T * V + static_cast<int64_t>(mine), raw[j], g, target));
+            raw[j] = load(xn, j);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        store_part(dr, end, n, grad_vector<S>(end, raw[NV - 1], g, target));
+        raw[NV - 1] = load_part(xn, end, n);
     }
+}
+
+// Rows shorter than a vector: a thread each.
+template <typename S>
+__global__ __launch_bounds__(256) void grad_rows_tiny(const S* x, int64_t m, int n, int64_t stride, Targets targets, const float* weights, float z,
+                                                      float* loss, S* dx, int64_t dx_stride) {
+    constexpr int V = vector_width<S>();
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (r >= m) return;
+    const int64_t target = targets[r];
+    float v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = i < n ? static_cast<float>(x[r * stride + i]) : kNone;
+    MaxSum s = {kNone, 0.0f};
+    fold(s, v);
+    float logit = std::numeric_limits<float>::quiet_NaN();
+#pragma unroll
+    for (int i = 0; i < V; ++i) logit = i == target && i < n ? v[i] : logit;
+    if (loss) loss[r] = target < 0 ? 0.0f : loss_of(s, logit, z);
+    const RowGrad g = row_grad(s, target >= 0, weights ? weights[r] : 1.0f, z);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (i < n) dx[r * dx_stride + i] = static_cast<S>(g.zero ? 0.0f : g.p * exp_diff(v[i], g.mx) - (i == target ? g.up : 0.0f));
 }
 
 // A row cut into tiles, a workgroup each: blockIdx = row * tiles + tile.
@@ -177,11 +249,11 @@ struct Tiles {
 };
 
 // What a call on a matrix of logits works on; state or loss is where a finished row goes.
-template <typename S, typename I>
+template <typename S>
 struct LossCall {
     const S* x;
     int64_t m, n, stride;
-    const I* targets;
+    Targets targets;
     int64_t first;               // column of the whole vocabulary that column 0 is
     int resume;
     float* state;
@@ -191,9 +263,9 @@ struct LossCall {
     MaxSum* records;             // tiles.count per row
 };
 
-template <typename S, typename I>
-__device__ __forceinline__ void finish_row(const LossCall<S, I>& p, int64_t r, MaxSum v) {
-    const int64_t target = static_cast<int64_t>(p.targets[r]);
+template <typename S>
+__device__ __forceinline__ void finish_row(const LossCall<S>& p, int64_t r, MaxSum v) {
+    const int64_t target = p.targets[r];
     float logit = std::numeric_limits<float>::quiet_NaN();
     if (!p.loss && p.resume) {
         v = join({p.state[r], p.state[p.m + r]}, v);
@@ -210,8 +282,8 @@ __device__ __forceinline__ void finish_row(const LossCall<S, I>& p, int64_t r, M
 }
 
 // A tile's record, or with one tile to a row the row's result.
-template <typename S, typename I>
-__global__ __launch_bounds__(kTileThreads) void loss_tiles(LossCall<S, I> p) {
+template <typename S>
+__global__ __launch_bounds__(kTileThreads) void loss_tiles(LossCall<S> p) {
     constexpr int V = vector_width<S>();
     __shared__ MaxSum lds[kTileThreads / kWave];
     const uint32_t tiles = static_cast<uint32_t>(p.tiles.count);
@@ -221,7 +293,7 @@ __global__ __launch_bounds__(kTileThreads) void loss_tiles(LossCall<S, I> p) {
     const int64_t end = begin + p.tiles.length < p.n ? begin + p.tiles.length : p.n;
     MaxSum s = {kNone, 0.0f};
     for (int64_t e0 = begin + static_cast<int64_t>(threadIdx.x) * V; e0 < end; e0 += kTileBatch * tile_unit<S>()) {
-        typename AnyVec<S, V>::type raw[kTileBatch];
+        Words4 raw[kTileBatch];
 #pragma unroll
         for (int u = 0; u < kTileBatch; ++u) {
             const int64_t e = e0 + u * tile_unit<S>();
@@ -231,8 +303,7 @@ __global__ __launch_bounds__(kTileThreads) void loss_tiles(LossCall<S, I> p) {
         for (int u = 0; u < kTileBatch; ++u) {
             if (e0 + u * tile_unit<S>() >= end) break;
             float v[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = static_cast<float>(raw[u][i]);
+            widen<S>(raw[u], v);
             fold(s, v);
         }
     }
@@ -249,24 +320,23 @@ __device__ __forceinline__ MaxSum join_records(const MaxSum* records, int64_t co
 }
 
 // One wavefront per row joins its records.
-template <typename S, typename I>
-__global__ __launch_bounds__(256) void loss_join_tiles(LossCall<S, I> p) {
+template <typename S>
+__global__ __launch_bounds__(256) void loss_join_tiles(LossCall<S> p) {
     const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
     if (r >= p.m) return;
     const MaxSum s = join_records(p.records + r * p.tiles.count, p.tiles.count);
     if (lane_id() == 0) finish_row(p, r, s);
 }
 
-template <typename I>
-__global__ __launch_bounds__(256) void loss_join(int64_t m, const I* targets, const float* state, float z, float* loss) {
+__global__ __launch_bounds__(256) void loss_join(int64_t m, Targets targets, const float* state, float z, float* loss) {
     const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (r >= m) return;
     loss[r] = targets[r] < 0 ? 0.0f : loss_of({state[r], state[m + r]}, state[2 * m + r], z);
 }
 
 // Gradient of a tile: the row's maximum and sum come from the state or from the records.
-template <typename S, typename I>
-__global__ __launch_bounds__(kTileThreads) void grad_tiles(LossCall<S, I> p, int64_t record_count, const float* weights, S* dx, int64_t dx_stride) {
+template <typename S>
+__global__ __launch_bounds__(kTileThreads) void grad_tiles(LossCall<S> p, int64_t record_count, const float* weights, S* dx, int64_t dx_stride) {
     constexpr int V = vector_width<S>();
     const uint32_t tiles = static_cast<uint32_t>(p.tiles.count);
     const int64_t r = blockIdx.x / tiles, tile = blockIdx.x % tiles;
@@ -274,7 +344,7 @@ __global__ __launch_bounds__(kTileThreads) void grad_tiles(LossCall<S, I> p, int
     S* dr = dx + r * dx_stride;
     const int64_t begin = tile * p.tiles.length;
     const int64_t end = begin + p.tiles.length < p.n ? begin + p.tiles.length : p.n;
-    const int64_t target = static_cast<int64_t>(p.targets[r]);
+    const int64_t target = p.targets[r];
     const float weight = weights ? weights[r] : 1.0f;
     MaxSum s;
     if (p.state) s = {p.state[r], p.state[p.m + r]};
@@ -282,7 +352,7 @@ __global__ __launch_bounds__(kTileThreads) void grad_tiles(LossCall<S, I> p, int
     const RowGrad g = row_grad(s, target >= 0, weight, p.z);
     const int64_t here = target < 0 ? -1 : target - p.first;
     for (int64_t e0 = begin + static_cast<int64_t>(threadIdx.x) * V; e0 < end; e0 += kTileBatch * tile_unit<S>()) {
-        typename AnyVec<S, V>::type raw[kTileBatch];
+        Words4 raw[kTileBatch];
 #pragma unroll
         for (int u = 0; u < kTileBatch; ++u) {
             const int64_t e = e0 + u * tile_unit<S>();
@@ -291,17 +361,12 @@ __global__ __launch_bounds__(kTileThreads) void grad_tiles(LossCall<S, I> p, int
 #pragma unroll
         for (int u = 0; u < kTileBatch; ++u) {
             const int64_t e = e0 + u * tile_unit<S>();
-            if (e < end) grad_part(dr, e, end, raw[u], g, here);
+            if (e < end) store_part(dr, e, end, grad_vector<S>(e, raw[u], g, here));
         }
     }
 }
 
-template <typename F>
-int dispatch_index(int index_dtype, F&& f) {
-    if (index_dtype == DLFX_I32) return f(int32_t());
-    if (index_dtype == DLFX_I64) return f(int64_t());
-    return DLFX_ERR_UNSUPPORTED_DTYPE;
-}
+bool index_ok(int index_dtype) { return index_dtype == DLFX_I32 || index_dtype == DLFX_I64; }
 
 int check(int64_t m, int64_t n, const void* x, int64_t row_stride, const void* targets) {
     if (m <= 0 || n <= 0 || !x || !targets || row_stride < n) return DLFX_ERR_INVALID_ARGUMENT;
@@ -337,6 +402,9 @@ size_t scratch_of(int64_t m, int64_t n) {
     return count > 1 || n > held_most<S>() ? static_cast<size_t>(m * count) * sizeof(MaxSum) : 0;
 }
 
+template <int... I, typename F>
+void for_each_of(std::integer_sequence<int, I...>, F&& f) { (f(std::integral_constant<int, I + 2>()), ...); }
+
 // Workgroups of a kernel that the current device holds at once, asked for once per device.
 template <auto KERNEL>
 int64_t resident(int threads) {
@@ -348,38 +416,38 @@ int64_t resident(int threads) {
     return n;
 }
 
-template <typename S, typename I>
-int launch_loss(LossCall<S, I> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
+template <typename S>
+int launch_loss(LossCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     p.tiles = joining_tiles<S>(p.m, p.n);
     if (p.tiles.count > 1 && (!scratch || scratch_bytes < scratch_of<S>(p.m, p.n))) p.tiles = {1, p.n};
     if (p.m * p.tiles.count > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
     p.records = static_cast<MaxSum*>(scratch);
-    loss_tiles<S, I><<<dim3(static_cast<unsigned>(p.m * p.tiles.count)), dim3(kTileThreads), 0, stream>>>(p);
+    loss_tiles<S><<<dim3(static_cast<unsigned>(p.m * p.tiles.count)), dim3(kTileThreads), 0, stream>>>(p);
     DLFX_CHECK_LAUNCH();
     if (p.tiles.count > 1) {
-        loss_join_tiles<S, I><<<dim3(static_cast<unsigned>(ceil_div(p.m, 4))), dim3(256), 0, stream>>>(p);
+        loss_join_tiles<S><<<dim3(static_cast<unsigned>(ceil_div(p.m, 4))), dim3(256), 0, stream>>>(p);
         DLFX_CHECK_LAUNCH();
     }
     return DLFX_OK;
 }
 
-template <typename S, typename I>
-int launch_grad_tiles(LossCall<S, I> p, int64_t record_count, const float* weights, S* dx, int64_t dx_stride, hipStream_t stream) {
+template <typename S>
+int launch_grad_tiles(LossCall<S> p, int64_t record_count, const float* weights, S* dx, int64_t dx_stride, hipStream_t stream) {
     p.tiles = writing_tiles<S>(p.n);
     if (p.m * p.tiles.count > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
-    grad_tiles<S, I><<<dim3(static_cast<unsigned>(p.m * p.tiles.count)), dim3(kTileThreads), 0, stream>>>(p, record_count, weights, dx, dx_stride);
+    grad_tiles<S><<<dim3(static_cast<unsigned>(p.m * p.tiles.count)), dim3(kTileThreads), 0, stream>>>(p, record_count, weights, dx, dx_stride);
     DLFX_CHECK_LAUNCH();
     return DLFX_OK;
 }
 
-template <typename S, typename I>
-int launch_grad(LossCall<S, I> p, const float* weights, S* dx, int64_t dx_stride, void* scratch, size_t scratch_bytes, hipStream_t stream) {
+template <typename S>
+int launch_grad(LossCall<S> p, const float* weights, S* dx, int64_t dx_stride, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     auto held = [&](auto vectors, auto team) {
         constexpr int NV = decltype(vectors)::value, T = decltype(team)::value;
         // as many workgroups as the device holds: each goes on to its next row while it stores the last
-        const int64_t most = resident<grad_rows_held<S, I, NV, T>>(T);
+        const int64_t most = resident<grad_rows_held<S, NV, T>>(T);
         const int64_t blocks = most > 0 && most < p.m ? most : p.m;
-        grad_rows_held<S, I, NV, T><<<dim3(static_cast<unsigned>(blocks)), dim3(T), 0, stream>>>(p.x, p.m, p.n, p.stride, p.targets, weights, p.z, p.loss,
+        grad_rows_held<S, NV, T><<<dim3(static_cast<unsigned>(blocks)), dim3(T), 0, stream>>>(p.x, p.m, p.n, p.stride, p.targets, weights, p.z, p.loss,
                                                                                               dx, dx_stride);
         DLFX_CHECK_LAUNCH();
         return static_cast<int>(DLFX_OK);
@@ -388,34 +456,39 @@ int launch_grad(LossCall<S, I> p, const float* weights, S* dx, int64_t dx_stride
     constexpr int64_t V = vector_width<S>();
     const size_t need = scratch_of<S>(p.m, p.n);
     const bool has_scratch = need && scratch && scratch_bytes >= need;
-    const integral_constant<int, 256> few;
-    const integral_constant<int, 1024> many;
-    if (p.n <= 256 * V) return held(integral_constant<int, 1>(), few);
-    if (p.n <= 512 * V) return held(integral_constant<int, 2>(), few);
-    if (p.n <= 1024 * V) return held(integral_constant<int, 4>(), few);
+    if (p.n < V) {
+        grad_rows_tiny<S><<<dim3(static_cast<unsigned>(ceil_div(p.m, 256))), dim3(256), 0, stream>>>(p.x, p.m, static_cast<int>(p.n), p.stride, p.targets,
+                                                                                                     weights, p.z, p.loss, dx, dx_stride);
+        DLFX_CHECK_LAUNCH();
+        return DLFX_OK;
+    }
+    if (p.n <= 256 * V) return held(integral_constant<int, 1>(), integral_constant<int, 256>());
+    if (p.n <= 512 * V) return held(integral_constant<int, 2>(), integral_constant<int, 256>());
+    if (p.n <= 768 * V) return held(integral_constant<int, 3>(), integral_constant<int, 256>());
+    if (p.n <= 1024 * V) return held(integral_constant<int, 4>(), integral_constant<int, 256>());
     if (p.n <= held_most<S>() && (p.m >= 192 || !has_scratch)) {
-        if (p.n <= 2 * 1024 * V) return held(integral_constant<int, 2>(), many);
-        if (p.n <= 3 * 1024 * V) return held(integral_constant<int, 3>(), many);
-        if (p.n <= 4 * 1024 * V) return held(integral_constant<int, 4>(), many);
-        if (p.n <= 6 * 1024 * V) return held(integral_constant<int, 6>(), many);
-        if (p.n <= 8 * 1024 * V) return held(integral_constant<int, 8>(), many);
-        if (p.n <= 12 * 1024 * V) return held(integral_constant<int, 12>(), many);
-        return held(integral_constant<int, 16>(), many);
+        int status = DLFX_OK;
+        const int64_t vectors = ceil_div(p.n, 1024 * V);
+        auto one = [&](auto c) {
+            if (vectors == decltype(c)::value) status = held(c, integral_constant<int, 1024>());
+        };
+        for_each_of(std::make_integer_sequence<int, 15>(), one);      // 2 to 16
+        return status;
     }
     if (!has_scratch) return DLFX_ERR_SCRATCH_TOO_SMALL;
     // the records first, then the losses (the target's logit is read before dx, which may be x, is
     // written), then the gradients tile by tile
-    LossCall<S, I> q = p;
+    LossCall<S> q = p;
     q.tiles = joining_tiles<S>(p.m, p.n);
     if (p.m * q.tiles.count > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
     q.records = static_cast<MaxSum*>(scratch);
     float* loss = q.loss;
     q.loss = nullptr;
-    loss_tiles<S, I><<<dim3(static_cast<unsigned>(p.m * q.tiles.count)), dim3(kTileThreads), 0, stream>>>(q);
+    loss_tiles<S><<<dim3(static_cast<unsigned>(p.m * q.tiles.count)), dim3(kTileThreads), 0, stream>>>(q);
     DLFX_CHECK_LAUNCH();
     if (loss) {
         q.loss = loss;
-        loss_join_tiles<S, I><<<dim3(static_cast<unsigned>(ceil_div(p.m, 4))), dim3(256), 0, stream>>>(q);
+        loss_join_tiles<S><<<dim3(static_cast<unsigned>(ceil_div(p.m, 4))), dim3(256), 0, stream>>>(q);
         DLFX_CHECK_LAUNCH();
     }
     return launch_grad_tiles(q, q.tiles.count, weights, dx, dx_stride, stream);
@@ -436,23 +509,16 @@ extern "C" size_t dlfx_cross_entropy_scratch_bytes(int dtype, int64_t m, int64_t
     }
 }
 
-// f(element, index, stream): dispatches a matrix call's types.
-template <typename F>
-static int with_types(dlfx_stream_t stream, int dtype, int index_dtype, F&& f) {
-    return dispatch_sequence_dtype(dtype, [&](auto tag) {
-        return dispatch_index(index_dtype, [&](auto index) { return static_cast<int>(f(tag, index, static_cast<hipStream_t>(stream))); });
-    });
-}
-
 extern "C" int dlfx_cross_entropy(dlfx_stream_t stream, int dtype, int index_dtype, int64_t m, int64_t n,
                                   const void* x, int64_t x_offset, int64_t row_stride, const void* targets,
                                   float z_loss, float* loss, void* scratch, size_t scratch_bytes) {
     if (int e = check(m, n, x, row_stride, targets)) return e;
     if (!loss) return DLFX_ERR_INVALID_ARGUMENT;
-    return with_types(stream, dtype, index_dtype, [&](auto tag, auto index, hipStream_t s) {
+    if (!index_ok(index_dtype)) return DLFX_ERR_UNSUPPORTED_DTYPE;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return dispatch_sequence_dtype(dtype, [&](auto tag) {
         using S = decltype(tag);
-        using I = decltype(index);
-        LossCall<S, I> p{static_cast<const S*>(x) + x_offset, m, n, row_stride, static_cast<const I*>(targets), 0, 0, nullptr, z_loss, loss, {}, nullptr};
+        LossCall<S> p{static_cast<const S*>(x) + x_offset, m, n, row_stride, Targets{targets, index_dtype == DLFX_I64}, 0, 0, nullptr, z_loss, loss, {}, nullptr};
         return launch_loss(p, scratch, scratch_bytes, s);
     });
 }
@@ -464,10 +530,11 @@ extern "C" int dlfx_cross_entropy_grad(dlfx_stream_t stream, int dtype, int inde
                                        void* scratch, size_t scratch_bytes) {
     if (int e = check(m, n, x, row_stride, targets)) return e;
     if (!dx || dx_row_stride < n) return DLFX_ERR_INVALID_ARGUMENT;
-    return with_types(stream, dtype, index_dtype, [&](auto tag, auto index, hipStream_t s) {
+    if (!index_ok(index_dtype)) return DLFX_ERR_UNSUPPORTED_DTYPE;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return dispatch_sequence_dtype(dtype, [&](auto tag) {
         using S = decltype(tag);
-        using I = decltype(index);
-        LossCall<S, I> p{static_cast<const S*>(x) + x_offset, m, n, row_stride, static_cast<const I*>(targets), 0, 0, nullptr, z_loss, loss, {}, nullptr};
+        LossCall<S> p{static_cast<const S*>(x) + x_offset, m, n, row_stride, Targets{targets, index_dtype == DLFX_I64}, 0, 0, nullptr, z_loss, loss, {}, nullptr};
         return launch_grad(p, weights, static_cast<S*>(dx) + dx_offset, dx_row_stride, scratch, scratch_bytes, s);
     });
 }
@@ -477,10 +544,11 @@ extern "C" int dlfx_cross_entropy_piece(dlfx_stream_t stream, int dtype, int ind
                                         int64_t first, int resume, float* state, void* scratch, size_t scratch_bytes) {
     if (int e = check(m, n, x, row_stride, targets)) return e;
     if (!state || first < 0) return DLFX_ERR_INVALID_ARGUMENT;
-    return with_types(stream, dtype, index_dtype, [&](auto tag, auto index, hipStream_t s) {
+    if (!index_ok(index_dtype)) return DLFX_ERR_UNSUPPORTED_DTYPE;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return dispatch_sequence_dtype(dtype, [&](auto tag) {
         using S = decltype(tag);
-        using I = decltype(index);
-        LossCall<S, I> p{static_cast<const S*>(x) + x_offset, m, n, row_stride, static_cast<const I*>(targets), first, resume, state, 0.0f, nullptr, {}, nullptr};
+        LossCall<S> p{static_cast<const S*>(x) + x_offset, m, n, row_stride, Targets{targets, index_dtype == DLFX_I64}, first, resume, state, 0.0f, nullptr, {}, nullptr};
         return launch_loss(p, scratch, scratch_bytes, s);
     });
 }
@@ -489,13 +557,11 @@ extern "C" int dlfx_cross_entropy_join(dlfx_stream_t stream, int index_dtype, in
                                        const float* state, float z_loss, float* loss) {
     if (m <= 0 || !targets || !state || !loss) return DLFX_ERR_INVALID_ARGUMENT;
     if (m > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
-    return dispatch_index(index_dtype, [&](auto index) {
-        using I = decltype(index);
-        loss_join<I><<<dim3(static_cast<unsigned>(ceil_div(m, 256))), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
-            m, static_cast<const I*>(targets), state, z_loss, loss);
-        DLFX_CHECK_LAUNCH();
-        return static_cast<int>(DLFX_OK);
-    });
+    if (!index_ok(index_dtype)) return DLFX_ERR_UNSUPPORTED_DTYPE;
+    loss_join<<<dim3(static_cast<unsigned>(ceil_div(m, 256))), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+        m, Targets{targets, index_dtype == DLFX_I64}, state, z_loss, loss);
+    DLFX_CHECK_LAUNCH();
+    return DLFX_OK;
 }
 
 extern "C" int dlfx_cross_entropy_piece_grad(dlfx_stream_t stream, int dtype, int index_dtype, int64_t m, int64_t n,
@@ -504,10 +570,11 @@ extern "C" int dlfx_cross_entropy_piece_grad(dlfx_stream_t stream, int dtype, in
                                              void* dx, int64_t dx_offset, int64_t dx_row_stride) {
     if (int e = check(m, n, x, row_stride, targets)) return e;
     if (!state || first < 0 || !dx || dx_row_stride < n) return DLFX_ERR_INVALID_ARGUMENT;
-    return with_types(stream, dtype, index_dtype, [&](auto tag, auto index, hipStream_t s) {
+    if (!index_ok(index_dtype)) return DLFX_ERR_UNSUPPORTED_DTYPE;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return dispatch_sequence_dtype(dtype, [&](auto tag) {
         using S = decltype(tag);
-        using I = decltype(index);
-        LossCall<S, I> p{static_cast<const S*>(x) + x_offset, m, n, row_stride, static_cast<const I*>(targets), first, 0, const_cast<float*>(state), z_loss,
+        LossCall<S> p{static_cast<const S*>(x) + x_offset, m, n, row_stride, Targets{targets, index_dtype == DLFX_I64}, first, 0, const_cast<float*>(state), z_loss,
                          nullptr, {}, nullptr};
         return launch_grad_tiles(p, 0, weights, static_cast<S*>(dx) + dx_offset, dx_row_stride, s);
     });
