@@ -37,6 +37,14 @@ __device__ __forceinline__ void gate_of(float g, float& a, float& keep) {
     }
 }
 
+// The gate that leaves a state as it is when x is 0 (a = 1).
+template <typename S, int KIND>
+__device__ __forceinline__ S neutral_gate() {
+    if constexpr (KIND == kGated) return static_cast<S>(1.0f);
+    else if constexpr (KIND == kGatedExp) return static_cast<S>(0.0f);
+    else return static_cast<S>(std::numeric_limits<float>::infinity());
+}
+
 // What a stretch of steps does to the state that enters it: h -> a h + b.  The product of many
 // gates can leave the range of fp32 where the states do not (growth from a tiny state, decay of a
 // large one), so it is held in 64 bits; an exact zero stays one under any growth.
@@ -49,7 +57,8 @@ __device__ __forceinline__ float through(const Stretch& s, float h) {
 }
 __device__ __forceinline__ Stretch join(const Stretch& first, const Stretch& then) { return {first.a * then.a, through(then, first.b)}; }
 
-// V neighbouring elements at base + off bytes.
+// V neighbouring elements at base + off bytes.  The base is the same for the whole wavefront and the
+// offset a lane's own: with 32 bits of it an access takes both as they are, without address arithmetic.
 template <typename S, int V, typename OFF>
 __device__ __forceinline__ Vec<S, V> load_at(const S* base, OFF off) {
     if constexpr (sizeof(S) == 2 && V == 1) {
@@ -67,6 +76,13 @@ __device__ __forceinline__ void store_at(S* base, OFF off, const Vec<S, V>& v) {
         constexpr int WORDS = sizeof(S) * V / 4;
         store_stream(reinterpret_cast<Vec<uint32_t, WORDS>*>(reinterpret_cast<char*>(base) + off), bit_cast<Vec<uint32_t, WORDS>>(v));
     }
+}
+
+// Keeps the compiler from adding a loop's changing base to the lane's offset beforehand.
+template <typename OFF>
+__device__ __forceinline__ OFF as_it_is(OFF off) {
+    if constexpr (sizeof(OFF) == 4) asm volatile("" : "+v"(off));
+    return off;
 }
 
 // A wavefront takes 64 groups of V neighbouring rows and S consecutive steps of a pass, W wavefronts

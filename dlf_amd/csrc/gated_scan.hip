@@ -79,11 +79,25 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
 
     Vec<S, V> graw[kSteps], xraw[kSteps];
     auto fetch = [&](int64_t t0) {
+        const S* gp = p.g.base + t0 * p.g.step;
+        const S* xp = p.x.base + t0 * p.x.step;
+        const OFF gi = as_it_is(go), xi = as_it_is(xo);
+        if (t0 + kSteps <= end) {
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            const int64_t t = t0 + i < end ? t0 + i : end - 1;          // past the end: any step's values, dropped later
-            graw[i] = load_at<S, V>(p.g.base + t * p.g.step, go);
-            xraw[i] = load_at<S, V>(p.x.base + t * p.x.step, xo);
+            for (int i = 0; i < kSteps; ++i, gp += p.g.step, xp += p.x.step) {
+                graw[i] = load_at<S, V>(gp, gi);
+                xraw[i] = load_at<S, V>(xp, xi);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i, gp += p.g.step, xp += p.x.step) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) graw[i].v[v] = neutral_gate<S, KIND>(), xraw[i].v[v] = static_cast<S>(0.0f);
+                if (t0 + i < end) {
+                    graw[i] = load_at<S, V>(gp, gi);
+                    xraw[i] = load_at<S, V>(xp, xi);
+                }
+            }
         }
     };
     int64_t t0 = begin + wave * kSteps;
@@ -99,14 +113,6 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
                 b[i][v] = static_cast<float>(xraw[i].v[v]);
                 gate_of<S, KIND>(static_cast<float>(graw[i].v[v]), a[i][v], keep);
                 if constexpr (KIND == kGatedBlend) b[i][v] *= keep;
-            }
-        }
-        if (t0 + kSteps > end) {
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                if (t0 + i < end) continue;
-#pragma unroll
-                for (int v = 0; v < V; ++v) a[i][v] = 1.0f, b[i][v] = 0.0f;
             }
         }
         if (pass + W * kSteps < end) fetch(t0 + W * kSteps);
@@ -143,15 +149,26 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
             h[v] = mine;
         }
         if constexpr (!PARTIAL) {
+            Vec<S, V> out[kSteps];
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
-                Vec<S, V> out;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     h[v] = fmaf(a[i][v], h[v], b[i][v]);
-                    out.v[v] = static_cast<S>(h[v]);
+                    out[i].v[v] = static_cast<S>(h[v]);
                 }
-                if (live && t0 + i < end) store_at<S, V>(p.y.base + (t0 + i) * p.y.step, yo, out);
+            }
+            S* yp = p.y.base + t0 * p.y.step;
+            const OFF yi = as_it_is(yo);
+            if (t0 + kSteps <= end) {
+                if (live) {
+#pragma unroll
+                    for (int i = 0; i < kSteps; ++i, yp += p.y.step) store_at<S, V>(yp, yi, out[i]);
+                }
+            } else if (live) {
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i, yp += p.y.step)
+                    if (t0 + i < end) store_at<S, V>(yp, yi, out[i]);
             }
         }
     }

@@ -99,14 +99,38 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
 
     Vec<S, V> graw[N], dyraw[N], yraw[N], xraw[N];
     auto fetch = [&](int64_t i0) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int64_t t = top - (i0 + i < end ? i0 + i : end - 1);
-            graw[i] = load_at<S, V>(p.g.base + t * p.g.step, go);
-            dyraw[i] = load_at<S, V>(p.dy.base + t * p.dy.step, dyo);
+        const int64_t t0 = top - i0;
+        const S* gp = p.g.base + t0 * p.g.step;
+        const S* dyp = p.dy.base + t0 * p.dy.step;
+        const S* yp = p.y.base + (t0 - 1) * p.y.step;
+        const S* xp = KIND == kGatedBlend ? p.x.base + t0 * p.x.step : nullptr;
+        const OFF gi = as_it_is(go), dyi = as_it_is(dyo), yi = as_it_is(yo), xi = as_it_is(xo);
+        auto one = [&](int i, bool first_step) {
+            graw[i] = load_at<S, V>(gp, gi);
+            dyraw[i] = load_at<S, V>(dyp, dyi);
             if constexpr (!PARTIAL) {
-                yraw[i] = load_at<S, V>(p.y.base + (t > 0 ? t - 1 : 0) * p.y.step, yo);      // (step 0: initial, below)
-                if constexpr (KIND == kGatedBlend) xraw[i] = load_at<S, V>(p.x.base + t * p.x.step, xo);
+                if (!first_step) yraw[i] = load_at<S, V>(yp, yi);
+                if constexpr (KIND == kGatedBlend) xraw[i] = load_at<S, V>(xp, xi);
+            }
+        };
+        auto on = [&] {
+            gp -= p.g.step;
+            dyp -= p.dy.step;
+            yp -= p.y.step;
+            if constexpr (KIND == kGatedBlend) xp -= p.x.step;
+        };
+        if (i0 + N <= end && i0 + N <= top) {
+#pragma unroll
+            for (int i = 0; i < N; ++i, on()) one(i, false);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i, on()) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    graw[i].v[v] = neutral_gate<S, KIND>();
+                    dyraw[i].v[v] = yraw[i].v[v] = xraw[i].v[v] = static_cast<S>(0.0f);
+                }
+                if (i0 + i < end) one(i, i0 + i == top);          // (before the first step: initial, below)
             }
         }
     };
@@ -122,18 +146,11 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
                 d[i][v] = static_cast<float>(dyraw[i].v[v]);
                 float before = 0.0f, x = 0.0f;
                 if constexpr (!PARTIAL) {
-                    before = i0 + i == top ? h0[v] : static_cast<float>(yraw[i].v[v]);
+                    before = static_cast<float>(yraw[i].v[v]);
+                    if (i0 + i == top) before = h0[v];
                     if constexpr (KIND == kGatedBlend) x = static_cast<float>(xraw[i].v[v]);
                 }
                 step_of<S, KIND>(static_cast<float>(graw[i].v[v]), x, before, a[i][v], keep[i][v], side[i][v]);
-            }
-        }
-        if (i0 + N > end) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                if (i0 + i < end) continue;
-#pragma unroll
-                for (int v = 0; v < V; ++v) a[i][v] = 1.0f, d[i][v] = 0.0f;
             }
         }
         if (pass + W * N < end) fetch(i0 + W * N);
@@ -164,19 +181,35 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
             mu[v] = mine;
         }
         if constexpr (!PARTIAL) {
+            Vec<S, V> dg[N], dx[N];
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                Vec<S, V> dg, dx;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     const float lam = d[i][v] + mu[v];
                     mu[v] = a[i][v] * lam;
-                    dg.v[v] = static_cast<S>(lam * side[i][v]);
-                    dx.v[v] = static_cast<S>(KIND == kGatedBlend ? lam * keep[i][v] : lam);
+                    dg[i].v[v] = static_cast<S>(lam * side[i][v]);
+                    dx[i].v[v] = static_cast<S>(KIND == kGatedBlend ? lam * keep[i][v] : lam);
                 }
-                if (live && i0 + i < end) {
-                    store_at<S, V>(p.dg.base + (top - i0 - i) * p.dg.step, dgo, dg);
-                    store_at<S, V>(p.dx.base + (top - i0 - i) * p.dx.step, dxo, dx);
+            }
+            S* dgp = p.dg.base + (top - i0) * p.dg.step;
+            S* dxp = p.dx.base + (top - i0) * p.dx.step;
+            const OFF dgi = as_it_is(dgo), dxi = as_it_is(dxo);
+            if (i0 + N <= end) {
+                if (live) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i, dgp -= p.dg.step, dxp -= p.dx.step) {
+                        store_at<S, V>(dgp, dgi, dg[i]);
+                        store_at<S, V>(dxp, dxi, dx[i]);
+                    }
+                }
+            } else if (live) {
+#pragma unroll
+                for (int i = 0; i < N; ++i, dgp -= p.dg.step, dxp -= p.dx.step) {
+                    if (i0 + i < end) {
+                        store_at<S, V>(dgp, dgi, dg[i]);
+                        store_at<S, V>(dxp, dxi, dx[i]);
+                    }
                 }
             }
         }
