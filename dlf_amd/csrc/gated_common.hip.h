@@ -93,8 +93,14 @@ struct Cut {
     int64_t segments, length;    // of the axis; length steps each, the last one shorter
 };
 
-constexpr int kSegmentsMost = 64;
 constexpr int64_t kBlocksWanted = 512;
+constexpr int kColumnSegments = 64, kRowSegments = 512;      // the most
+
+// Workgroups go round the eight XCDs in turn, each with a cache of its own: neighbouring pieces of work
+// (groups of rows that share cache lines where a row of columns is no whole number of them) go to one
+// XCD side by side.  The grid is rounded up to a multiple of 8.
+__device__ __forceinline__ int64_t work_of(uint32_t block, uint32_t grid) { return static_cast<int64_t>(block % 8) * (grid / 8) + block / 8; }
+inline int64_t grid_of(int64_t work) { return ceil_div(work, 8) * 8; }
 
 // ---- rows along memory: a lane takes kRun consecutive positions of its row in two 128-bit accesses
 template <typename S>
@@ -140,28 +146,43 @@ __device__ __forceinline__ void store_run(S* row, int64_t i0, int64_t end, const
     }
 }
 
-// The stretches of a group of G lanes (16 or 64, in order) joined from the group's first lane up to
-// each; `before` is what lies before the lane, `all` the whole group's.
+// The stretches of a group of G lanes (4, 16, 32 or 64, in order) joined from the group's first lane up
+// to each; `before` is what lies before the lane, `all` the whole group's.
 template <int G>
 __device__ __forceinline__ void join_lanes(Stretch s, Stretch& before, Stretch& all) {
-    auto step = [&](double pa, float pb) {
+    const int lane = lane_id();
+    auto step = [&](double pa, float pb, bool mine) {
+        if (!mine) pa = 1.0, pb = 0.0f;
         s.b = through(s, pb);
         s.a *= pa;
     };
-    step(dpp_fetch<kRowShr1>(s.a, 1.0), dpp_fetch<kRowShr1>(s.b, 0.0f));
-    step(dpp_fetch<kRowShr2>(s.a, 1.0), dpp_fetch<kRowShr2>(s.b, 0.0f));
-    step(dpp_fetch<kRowShr4>(s.a, 1.0), dpp_fetch<kRowShr4>(s.b, 0.0f));
-    step(dpp_fetch<kRowShr8>(s.a, 1.0), dpp_fetch<kRowShr8>(s.b, 0.0f));
-    if constexpr (G == kWave) {
-        step(dpp_fetch<kRowBcast15, 0xa>(s.a, 1.0), dpp_fetch<kRowBcast15, 0xa>(s.b, 0.0f));
-        step(dpp_fetch<kRowBcast31, 0xc>(s.a, 1.0), dpp_fetch<kRowBcast31, 0xc>(s.b, 0.0f));
+    // (a row shift reaches over a group of four: what comes from the group before is dropped)
+    step(dpp_fetch<kRowShr1>(s.a, 1.0), dpp_fetch<kRowShr1>(s.b, 0.0f), G >= 16 || lane % G >= 1);
+    step(dpp_fetch<kRowShr2>(s.a, 1.0), dpp_fetch<kRowShr2>(s.b, 0.0f), G >= 16 || lane % G >= 2);
+    if constexpr (G >= 16) {
+        step(dpp_fetch<kRowShr4>(s.a, 1.0), dpp_fetch<kRowShr4>(s.b, 0.0f), true);
+        step(dpp_fetch<kRowShr8>(s.a, 1.0), dpp_fetch<kRowShr8>(s.b, 0.0f), true);
     }
-    const int lane = lane_id();
+    if constexpr (G >= 32) step(dpp_fetch<kRowBcast15, 0xa>(s.a, 1.0), dpp_fetch<kRowBcast15, 0xa>(s.b, 0.0f), true);
+    if constexpr (G >= 64) step(dpp_fetch<kRowBcast31, 0xc>(s.a, 1.0), dpp_fetch<kRowBcast31, 0xc>(s.b, 0.0f), true);
     before.a = lane_get(s.a, (lane + kWave - 1) % kWave);
     before.b = lane_get(s.b, (lane + kWave - 1) % kWave);
     if (lane % G == 0) before = {1.0, 0.0f};
     if constexpr (G == kWave) all = {lane_read(s.a, kWave - 1), lane_read(s.b, kWave - 1)};
     else all = {lane_get(s.a, lane | (G - 1)), lane_get(s.b, lane | (G - 1))};
+}
+
+// The state that enters segment `count` of row r, by a whole wavefront: a lane joins neighbouring records.
+__device__ __forceinline__ float enter_segment(const Stretch* records, int64_t m, int64_t r, int64_t count, float state) {
+    const int per = static_cast<int>((count + kWave - 1) / kWave);
+    Stretch mine = {1.0, 0.0f};
+    for (int i = 0; i < per; ++i) {
+        const int64_t s = static_cast<int64_t>(lane_id()) * per + i;
+        if (s < count) mine = join(mine, records[s * m + r]);
+    }
+    Stretch before, all;
+    join_lanes<kWave>(mine, before, all);
+    return through(all, state);
 }
 
 // +1 or -1 when a track's steps lie one element apart in memory, 0 otherwise.
@@ -170,10 +191,10 @@ int direction(const Track<S>& t) { return t.step == 1 ? 1 : t.step == -1 ? -1 : 
 
 // How many segments: one while the groups of rows alone give the device its workgroups, otherwise
 // about kBlocksWanted workgroups in all, none shorter than `shortest` steps.
-inline int64_t segments_of(int64_t groups, int64_t n, int64_t shortest, int64_t enough) {
+inline int64_t segments_of(int64_t groups, int64_t n, int64_t shortest, int64_t enough, int64_t limit) {
     if (groups >= enough) return 1;
     int64_t s = ceil_div(kBlocksWanted, groups);
-    if (s > kSegmentsMost) s = kSegmentsMost;
+    if (s > limit) s = limit;
     const int64_t most = n / shortest;
     return s < most ? s : (most < 1 ? 1 : most);
 }

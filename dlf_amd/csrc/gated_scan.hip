@@ -47,8 +47,11 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
     __shared__ float lds[2][W][kWave][2 * V];
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int64_t segment = PARTIAL ? blockIdx.x / p.cut.blocks : p.cut.segments - 1 - blockIdx.x / p.cut.blocks;
-    const int64_t block = blockIdx.x % p.cut.blocks;
+    const int64_t work = work_of(blockIdx.x, gridDim.x);
+    if (work >= p.cut.blocks * (PARTIAL ? p.cut.segments - 1 : p.cut.segments)) return;
+    // (segments from the last one on after PARTIAL went from the first: what it read last may still be cached)
+    const int64_t segment = PARTIAL ? work / p.cut.blocks : p.cut.segments - 1 - work / p.cut.blocks;
+    const int64_t block = work % p.cut.blocks;
     const int64_t r = (block * kWave + lane) * V;
     const bool live = r < p.cut.m;
     const int64_t rr = live ? r : p.cut.m - V;
@@ -184,23 +187,23 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
 template <typename S, int KIND, int V, int W, typename OFF>
 int launch_cols(ScanCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     p.cut.blocks = ceil_div(p.cut.m, kWave * V);
-    int64_t segments = segments_of(p.cut.blocks, p.cut.n, 2 * W * kSteps, 192);
+    int64_t segments = segments_of(p.cut.blocks, p.cut.n, W * kSteps, 192, kColumnSegments);
     if (segments > 1 && (!scratch || scratch_bytes < records_bytes(p.cut.m, segments))) return DLFX_ERR_SCRATCH_TOO_SMALL;
     p.cut.length = align_up(ceil_div(p.cut.n, segments), W * kSteps);
     segments = p.cut.segments = ceil_div(p.cut.n, p.cut.length);
-    if (p.cut.blocks * segments > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
+    if (p.cut.blocks * segments > 0x7ffffff0LL) return DLFX_ERR_TOO_LARGE;
     if (segments > 1) {
         p.records = static_cast<Stretch*>(scratch);
         p.entering = reinterpret_cast<float*>(static_cast<char*>(scratch) + align_up(static_cast<size_t>(p.cut.m * (segments - 1)) * sizeof(Stretch), 256));
-        gated_cols<S, KIND, V, W, OFF, true><<<dim3(static_cast<unsigned>(p.cut.blocks * (segments - 1))), dim3(W * kWave), 0, stream>>>(p);
+        gated_cols<S, KIND, V, W, OFF, true><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * (segments - 1)))), dim3(W * kWave), 0, stream>>>(p);
         DLFX_CHECK_LAUNCH();
     }
-    gated_cols<S, KIND, V, W, OFF, false><<<dim3(static_cast<unsigned>(p.cut.blocks * segments)), dim3(W * kWave), 0, stream>>>(p);
+    gated_cols<S, KIND, V, W, OFF, false><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * segments))), dim3(W * kWave), 0, stream>>>(p);
     DLFX_CHECK_LAUNCH();
     return DLFX_OK;
 }
 
-// Rows along memory: G lanes (16 or 64) or W wavefronts per row, a run of consecutive steps to a
+// Rows along memory: G lanes (4, 16, 32 or 64) or W wavefronts per row, a run of consecutive steps to a
 // lane; the lanes' stretches are joined by DPP, the wavefronts' through LDS, pass after pass.
 template <typename S, int KIND, int G, int W, int DIR, bool PARTIAL>
 __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_rows(ScanCall<S> p) {
@@ -231,7 +234,7 @@ __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_rows(ScanCall<S
         }
     } else if (!PARTIAL) {
         carry = p.entering[rr];
-        for (int64_t s = 0; s < segment; ++s) carry = through(p.records[s * p.cut.m + rr], carry);
+        if constexpr (W > 4) carry = enter_segment(p.records, p.cut.m, rr, segment, carry);
     }
 
     S graw[N], xraw[N];
@@ -303,7 +306,7 @@ template <typename S, int KIND, int G, int W, int DIR>
 int launch_rows(ScanCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     constexpr int BLOCK = W > 4 ? W * kWave : 256, PASS = W * G * run_length<S>();
     p.cut.blocks = ceil_div(p.cut.m, BLOCK / (W * G));
-    int64_t segments = W > 4 ? segments_of(p.cut.blocks, p.cut.n, PASS, 192) : 1;
+    int64_t segments = W > 4 ? segments_of(p.cut.blocks, p.cut.n, PASS, 192, kRowSegments) : 1;
     if (segments > 1 && (!scratch || scratch_bytes < records_bytes(p.cut.m, segments))) return DLFX_ERR_SCRATCH_TOO_SMALL;
     p.cut.length = align_up(ceil_div(p.cut.n, segments), PASS);
     segments = p.cut.segments = ceil_div(p.cut.n, p.cut.length);
@@ -323,7 +326,9 @@ int launch_rows(ScanCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t 
 
 template <typename S, int KIND, int DIR>
 int launch_direction(const ScanCall<S>& p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
+    if (p.cut.n <= 4 * run_length<S>()) return launch_rows<S, KIND, 4, 1, DIR>(p, scratch, scratch_bytes, stream);
     if (p.cut.n <= 16 * run_length<S>()) return launch_rows<S, KIND, 16, 1, DIR>(p, scratch, scratch_bytes, stream);
+    if (p.cut.n <= 32 * run_length<S>()) return launch_rows<S, KIND, 32, 1, DIR>(p, scratch, scratch_bytes, stream);
     if (p.cut.m >= 2048) return launch_rows<S, KIND, kWave, 1, DIR>(p, scratch, scratch_bytes, stream);
     if (p.cut.m >= 512 || p.cut.n <= 4 * kWave * run_length<S>()) return launch_rows<S, KIND, kWave, 4, DIR>(p, scratch, scratch_bytes, stream);
     return launch_rows<S, KIND, kWave, 16, DIR>(p, scratch, scratch_bytes, stream);
@@ -359,7 +364,7 @@ using namespace dlfx;
 // (an upper bound over every layout of m rows of n steps, forward and backward: the query does not see the strides)
 extern "C" size_t dlfx_gated_scan_scratch_bytes(int dtype, int64_t m, int64_t n) {
     if (m <= 0 || n <= 0 || (dtype != DLFX_F32 && dtype != DLFX_F16 && dtype != DLFX_BF16)) return 0;
-    return records_bytes(m, std::max(segments_of(ceil_div(m, kWave), n, 256, 192), segments_of(m, n, 8192, 192)));
+    return records_bytes(m, std::max(segments_of(ceil_div(m, kWave), n, 32, 192, kColumnSegments), segments_of(m, n, 8192, 192, kRowSegments)));
 }
 
 extern "C" int dlfx_gated_scan(dlfx_stream_t stream, const char* name, int dtype, int64_t m, int64_t n,

@@ -62,8 +62,11 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
     __shared__ float lds[2][W][kWave][2 * V];
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int64_t segment = PARTIAL ? blockIdx.x / p.cut.blocks : p.cut.segments - 1 - blockIdx.x / p.cut.blocks;
-    const int64_t block = blockIdx.x % p.cut.blocks;
+    const int64_t work = work_of(blockIdx.x, gridDim.x);
+    if (work >= p.cut.blocks * (PARTIAL ? p.cut.segments - 1 : p.cut.segments)) return;
+    // (segments from the last one on after PARTIAL went from the first: what it read last may still be cached)
+    const int64_t segment = PARTIAL ? work / p.cut.blocks : p.cut.segments - 1 - work / p.cut.blocks;
+    const int64_t block = work % p.cut.blocks;
     const int64_t r = (block * kWave + lane) * V;
     const bool live = r < p.cut.m;
     const int64_t rr = live ? r : p.cut.m - V;
@@ -226,18 +229,18 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
 template <typename S, int KIND, int V, int W, typename OFF>
 int launch_cols(GradCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     p.cut.blocks = ceil_div(p.cut.m, kWave * V);
-    int64_t segments = segments_of(p.cut.blocks, p.cut.n, 2 * W * kGradSteps, 192);
+    int64_t segments = segments_of(p.cut.blocks, p.cut.n, W * kGradSteps, 192, kColumnSegments);
     if (segments > 1 && (!scratch || scratch_bytes < records_bytes(p.cut.m, segments))) return DLFX_ERR_SCRATCH_TOO_SMALL;
     p.cut.length = align_up(ceil_div(p.cut.n, segments), W * kGradSteps);
     segments = p.cut.segments = ceil_div(p.cut.n, p.cut.length);
-    if (p.cut.blocks * segments > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
+    if (p.cut.blocks * segments > 0x7ffffff0LL) return DLFX_ERR_TOO_LARGE;
     if (segments > 1) {
         p.records = static_cast<Stretch*>(scratch);
         p.entering = reinterpret_cast<float*>(static_cast<char*>(scratch) + align_up(static_cast<size_t>(p.cut.m * (segments - 1)) * sizeof(Stretch), 256));
-        gated_grad_cols<S, KIND, V, W, OFF, true><<<dim3(static_cast<unsigned>(p.cut.blocks * (segments - 1))), dim3(W * kWave), 0, stream>>>(p);
+        gated_grad_cols<S, KIND, V, W, OFF, true><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * (segments - 1)))), dim3(W * kWave), 0, stream>>>(p);
         DLFX_CHECK_LAUNCH();
     }
-    gated_grad_cols<S, KIND, V, W, OFF, false><<<dim3(static_cast<unsigned>(p.cut.blocks * segments)), dim3(W * kWave), 0, stream>>>(p);
+    gated_grad_cols<S, KIND, V, W, OFF, false><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * segments))), dim3(W * kWave), 0, stream>>>(p);
     DLFX_CHECK_LAUNCH();
     return DLFX_OK;
 }
@@ -282,7 +285,7 @@ __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_grad_rows(GradC
         }
     } else if (!PARTIAL) {
         carry = p.entering[rr];
-        for (int64_t s = 0; s < segment; ++s) carry = through(p.records[s * p.cut.m + rr], carry);
+        if constexpr (W > 4) carry = enter_segment(p.records, p.cut.m, rr, segment, carry);
     }
 
     S graw[N], dyraw[N], yraw[N], xraw[N];
@@ -366,7 +369,7 @@ template <typename S, int KIND, int G, int W, int DIR>
 int launch_rows(GradCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     constexpr int BLOCK = W > 4 ? W * kWave : 256, PASS = W * G * run_length<S>();
     p.cut.blocks = ceil_div(p.cut.m, BLOCK / (W * G));
-    int64_t segments = W > 4 ? segments_of(p.cut.blocks, p.cut.n, PASS, 192) : 1;
+    int64_t segments = W > 4 ? segments_of(p.cut.blocks, p.cut.n, PASS, 192, kRowSegments) : 1;
     if (segments > 1 && (!scratch || scratch_bytes < records_bytes(p.cut.m, segments))) return DLFX_ERR_SCRATCH_TOO_SMALL;
     p.cut.length = align_up(ceil_div(p.cut.n, segments), PASS);
     segments = p.cut.segments = ceil_div(p.cut.n, p.cut.length);
@@ -386,7 +389,9 @@ int launch_rows(GradCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t 
 
 template <typename S, int KIND, int DIR>
 int launch_direction(const GradCall<S>& p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
+    if (p.cut.n <= 4 * run_length<S>()) return launch_rows<S, KIND, 4, 1, DIR>(p, scratch, scratch_bytes, stream);
     if (p.cut.n <= 16 * run_length<S>()) return launch_rows<S, KIND, 16, 1, DIR>(p, scratch, scratch_bytes, stream);
+    if (p.cut.n <= 32 * run_length<S>()) return launch_rows<S, KIND, 32, 1, DIR>(p, scratch, scratch_bytes, stream);
     if (p.cut.m >= 2048) return launch_rows<S, KIND, kWave, 1, DIR>(p, scratch, scratch_bytes, stream);
     if (p.cut.m >= 512 || p.cut.n <= 4 * kWave * run_length<S>()) return launch_rows<S, KIND, kWave, 4, DIR>(p, scratch, scratch_bytes, stream);
     return launch_rows<S, KIND, kWave, 16, DIR>(p, scratch, scratch_bytes, stream);
