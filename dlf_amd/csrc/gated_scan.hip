@@ -41,9 +41,13 @@ constexpr int kSteps = 16;       // of a wavefront in a pass
 // Rows side by side: lanes run along the rows, wavefronts along the axis.  Every wavefront holds its
 // steps of a pass in registers, leaves what they do to the state in LDS, and walks them again from
 // the state that the wavefronts before it make of the pass's; the next pass is loaded meanwhile.
+// The loop over whole passes has no branch beside its loads and stores: behind one, the wait for the
+// next pass's loads would be a wait for this pass's stores.  Lanes past the last row do the last row's
+// work over, value for value.
 // PARTIAL: only what the segment does to the state, for the segments behind it.
-template <typename S, int KIND, int V, int W, typename OFF, bool PARTIAL>
+template <typename S, int KIND, int V, int W, typename OFF, bool NT, bool PARTIAL>
 __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
+    constexpr int N = kSteps;
     __shared__ float lds[2][W][kWave][2 * V];
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -52,12 +56,11 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
     // (segments from the last one on after PARTIAL went from the first: what it read last may still be cached)
     const int64_t segment = PARTIAL ? work / p.cut.blocks : p.cut.segments - 1 - work / p.cut.blocks;
     const int64_t block = work % p.cut.blocks;
-    const int64_t r = (block * kWave + lane) * V;
-    const bool live = r < p.cut.m;
-    const int64_t rr = live ? r : p.cut.m - V;
-    const OFF go = static_cast<OFF>(p.g.row.at(rr) * static_cast<int64_t>(sizeof(S)));
-    const OFF xo = static_cast<OFF>(p.x.row.at(rr) * static_cast<int64_t>(sizeof(S)));
-    const OFF yo = static_cast<OFF>(p.y.row.at(rr) * static_cast<int64_t>(sizeof(S)));
+    const int64_t wanted = (block * kWave + lane) * V;
+    const int64_t r = wanted < p.cut.m ? wanted : p.cut.m - V;
+    const OFF go = static_cast<OFF>(p.g.row.at(r) * static_cast<int64_t>(sizeof(S)));
+    const OFF xo = static_cast<OFF>(p.x.row.at(r) * static_cast<int64_t>(sizeof(S)));
+    const OFF yo = static_cast<OFF>(p.y.row.at(r) * static_cast<int64_t>(sizeof(S)));
     const int64_t begin = segment * p.cut.length;
     const int64_t end = begin + p.cut.length < p.cut.n ? begin + p.cut.length : p.cut.n;
 
@@ -68,48 +71,33 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
         product[v] = 1.0;
         carry[v] = 0.0f;
         if (p.cut.segments == 1 || (PARTIAL && segment == 0)) {
-            const float h = p.initial.base ? p.initial.base[p.initial.row.at(rr + v)] : 0.0f;
+            const float h = p.initial.base ? p.initial.base[p.initial.row.at(r + v)] : 0.0f;
             if constexpr (PARTIAL) {
-                if (wave == 0 && live) p.entering[rr + v] = h;
+                if (wave == 0) p.entering[r + v] = h;
             } else {
                 carry[v] = h;
             }
         } else if (!PARTIAL) {
-            carry[v] = p.entering[rr + v];
-            for (int64_t s = 0; s < segment; ++s) carry[v] = through(p.records[s * p.cut.m + rr + v], carry[v]);
+            carry[v] = p.entering[r + v];
+            for (int64_t s = 0; s < segment; ++s) carry[v] = through(p.records[s * p.cut.m + r + v], carry[v]);
         }
     }
 
-    Vec<S, V> graw[kSteps], xraw[kSteps];
+    Vec<S, V> graw[N], xraw[N];
+    float a[N][V], b[N][V];
     auto fetch = [&](int64_t t0) {
         const S* gp = p.g.base + t0 * p.g.step;
         const S* xp = p.x.base + t0 * p.x.step;
         const OFF gi = as_it_is(go), xi = as_it_is(xo);
-        if (t0 + kSteps <= end) {
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i, gp += p.g.step, xp += p.x.step) {
-                graw[i] = load_at<S, V>(gp, gi);
-                xraw[i] = load_at<S, V>(xp, xi);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i, gp += p.g.step, xp += p.x.step) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) graw[i].v[v] = neutral_gate<S, KIND>(), xraw[i].v[v] = static_cast<S>(0.0f);
-                if (t0 + i < end) {
-                    graw[i] = load_at<S, V>(gp, gi);
-                    xraw[i] = load_at<S, V>(xp, xi);
-                }
-            }
+        for (int i = 0; i < N; ++i, gp += p.g.step, xp += p.x.step) {
+            graw[i] = load_at<NT, S, V>(gp, gi);
+            xraw[i] = load_at<NT, S, V>(xp, xi);
         }
     };
-    int64_t t0 = begin + wave * kSteps;
-    fetch(t0);
-    int parity = 0;
-    for (int64_t pass = begin; pass < end; pass += W * kSteps, t0 += W * kSteps, parity ^= 1) {
-        float a[kSteps][V], b[kSteps][V];
+    auto widen = [&] {
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
+        for (int i = 0; i < N; ++i) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 float keep = 1.0f;
@@ -118,26 +106,22 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
                 if constexpr (KIND == kGatedBlend) b[i][v] *= keep;
             }
         }
-        if (pass + W * kSteps < end) fetch(t0 + W * kSteps);
-        float whole_a[V], whole_b[V];
+    };
+    // The pass's states from the stretches of all wavefronts; h: the state that enters this one's steps.
+    int parity = 0;
+    auto enter = [&](float (&h)[V]) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            float pa = a[0][v], h = b[0][v];
+            float pa = a[0][v], pb = b[0][v];
 #pragma unroll
-            for (int i = 1; i < kSteps; ++i) {
+            for (int i = 1; i < N; ++i) {
                 pa *= a[i][v];
-                h = fmaf(a[i][v], h, b[i][v]);
+                pb = fmaf(a[i][v], pb, b[i][v]);
             }
-            whole_a[v] = pa;
-            whole_b[v] = h;
-        }
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            lds[parity][wave][lane][2 * v] = whole_a[v];
-            lds[parity][wave][lane][2 * v + 1] = whole_b[v];
+            lds[parity][wave][lane][2 * v] = pa;
+            lds[parity][wave][lane][2 * v + 1] = pb;
         }
         __syncthreads();
-        float h[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float c = carry[v], mine = carry[v];
@@ -151,31 +135,58 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
             carry[v] = c;
             h[v] = mine;
         }
+        parity ^= 1;
+    };
+    auto state = [&](int i, float (&h)[V]) {
+        Vec<S, V> out;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            h[v] = fmaf(a[i][v], h[v], b[i][v]);
+            out.v[v] = static_cast<S>(h[v]);
+        }
+        return out;
+    };
+
+    const int64_t passes = (end - begin) / (W * N);
+    int64_t t0 = begin + wave * N;
+    if (passes > 0) fetch(t0);
+    for (int64_t pass = 0; pass < passes; ++pass, t0 += W * N) {
+        widen();
+        fetch(pass + 1 < passes ? t0 + W * N : t0);       // (after the last whole pass: values that nobody uses)
+        float h[V];
+        enter(h);
         if constexpr (!PARTIAL) {
-            Vec<S, V> out[kSteps];
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    h[v] = fmaf(a[i][v], h[v], b[i][v]);
-                    out[i].v[v] = static_cast<S>(h[v]);
-                }
-            }
             S* yp = p.y.base + t0 * p.y.step;
             const OFF yi = as_it_is(yo);
-            if (t0 + kSteps <= end) {
-                if (live) {
 #pragma unroll
-                    for (int i = 0; i < kSteps; ++i, yp += p.y.step) store_at<S, V>(yp, yi, out[i]);
-                }
-            } else if (live) {
+            for (int i = 0; i < N; ++i, yp += p.y.step) store_at<NT, S, V>(yp, yi, state(i, h));
+        }
+    }
+    if (begin + passes * (W * N) < end) {
+        const S* gp = p.g.base + t0 * p.g.step;
+        const S* xp = p.x.base + t0 * p.x.step;
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i, yp += p.y.step)
-                    if (t0 + i < end) store_at<S, V>(yp, yi, out[i]);
+        for (int i = 0; i < N; ++i, gp += p.g.step, xp += p.x.step) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) graw[i].v[v] = neutral_gate<S, KIND>(), xraw[i].v[v] = static_cast<S>(0.0f);
+            if (t0 + i < end) {
+                graw[i] = load_at<NT, S, V>(gp, go);
+                xraw[i] = load_at<NT, S, V>(xp, xo);
+            }
+        }
+        widen();
+        float h[V];
+        enter(h);
+        if constexpr (!PARTIAL) {
+            S* yp = p.y.base + t0 * p.y.step;
+#pragma unroll
+            for (int i = 0; i < N; ++i, yp += p.y.step) {
+                const Vec<S, V> out = state(i, h);
+                if (t0 + i < end) store_at<NT, S, V>(yp, yo, out);
             }
         }
     }
-    if (wave == 0 && live) {
+    if (wave == 0) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             if constexpr (PARTIAL) p.records[segment * p.cut.m + r + v] = {product[v], carry[v]};
@@ -184,7 +195,7 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
     }
 }
 
-template <typename S, int KIND, int V, int W, typename OFF>
+template <typename S, int KIND, int V, int W, typename OFF, bool NT>
 int launch_cols(ScanCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     p.cut.blocks = ceil_div(p.cut.m, kWave * V);
     int64_t segments = segments_of(p.cut.blocks, p.cut.n, W * kSteps, 192, kColumnSegments);
@@ -195,10 +206,10 @@ int launch_cols(ScanCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t 
     if (segments > 1) {
         p.records = static_cast<Stretch*>(scratch);
         p.entering = reinterpret_cast<float*>(static_cast<char*>(scratch) + align_up(static_cast<size_t>(p.cut.m * (segments - 1)) * sizeof(Stretch), 256));
-        gated_cols<S, KIND, V, W, OFF, true><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * (segments - 1)))), dim3(W * kWave), 0, stream>>>(p);
+        gated_cols<S, KIND, V, W, OFF, NT, true><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * (segments - 1)))), dim3(W * kWave), 0, stream>>>(p);
         DLFX_CHECK_LAUNCH();
     }
-    gated_cols<S, KIND, V, W, OFF, false><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * segments))), dim3(W * kWave), 0, stream>>>(p);
+    gated_cols<S, KIND, V, W, OFF, NT, false><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * segments))), dim3(W * kWave), 0, stream>>>(p);
     DLFX_CHECK_LAUNCH();
     return DLFX_OK;
 }
@@ -214,36 +225,34 @@ __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_rows(ScanCall<S
     __shared__ Stretch lds[W > 1 ? 2 : 1][W > 1 ? TEAMS : 1][W];
     const int team = threadIdx.x / TEAM, place = threadIdx.x % TEAM, wave = place / kWave;
     const int64_t segment = PARTIAL ? blockIdx.x / p.cut.blocks : p.cut.segments - 1 - blockIdx.x / p.cut.blocks;
-    const int64_t r = (blockIdx.x % p.cut.blocks) * TEAMS + team;
-    const bool live = r < p.cut.m;
-    const int64_t rr = live ? r : p.cut.m - 1;
-    const S* gp = p.g.base + p.g.row.at(rr);
-    const S* xp = p.x.base + p.x.row.at(rr);
-    S* yp = p.y.base + p.y.row.at(rr);
+    const int64_t wanted = (blockIdx.x % p.cut.blocks) * TEAMS + team;
+    // a wavefront past the last row has nothing to do; groups past it beside others do the last row's work
+    // over, value for value and in step with the wavefront's group that owns it
+    if (wanted - (W == 1 ? threadIdx.x % kWave / G : 0) >= p.cut.m) return;
+    const int64_t r = wanted < p.cut.m ? wanted : p.cut.m - 1;
+    const S* gp = p.g.base + p.g.row.at(r);
+    const S* xp = p.x.base + p.x.row.at(r);
+    S* yp = p.y.base + p.y.row.at(r);
     const int64_t begin = segment * p.cut.length;
     const int64_t end = begin + p.cut.length < p.cut.n ? begin + p.cut.length : p.cut.n;
 
     float carry = 0.0f;
     double product = 1.0;
     if (p.cut.segments == 1 || (PARTIAL && segment == 0)) {
-        const float h = p.initial.base ? p.initial.base[p.initial.row.at(rr)] : 0.0f;
+        const float h = p.initial.base ? p.initial.base[p.initial.row.at(r)] : 0.0f;
         if constexpr (PARTIAL) {
-            if (place == 0 && live) p.entering[rr] = h;
+            if (place == 0) p.entering[r] = h;
         } else {
             carry = h;
         }
     } else if (!PARTIAL) {
-        carry = p.entering[rr];
-        if constexpr (W > 4) carry = enter_segment(p.records, p.cut.m, rr, segment, carry);
+        carry = p.entering[r];
+        if constexpr (W > 4) carry = enter_segment(p.records, p.cut.m, r, segment, carry);
     }
 
     S graw[N], xraw[N];
-    int64_t i0 = begin + place * N;
-    load_run<DIR>(gp, i0, end, graw);
-    load_run<DIR>(xp, i0, end, xraw);
-    int parity = 0;
-    for (int64_t pass = begin; pass < end; pass += PASS, i0 += PASS, parity ^= 1) {
-        float a[N], b[N];
+    float a[N], b[N];
+    auto widen = [&] {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float keep = 1.0f;
@@ -251,52 +260,76 @@ __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_rows(ScanCall<S
             gate_of<S, KIND>(static_cast<float>(graw[i]), a[i], keep);
             if constexpr (KIND == kGatedBlend) b[i] *= keep;
         }
-        if (i0 + N > end) {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (i0 + i >= end) a[i] = 1.0f, b[i] = 0.0f;
-        }
-        if (pass + PASS < end) {
-            load_run<DIR>(gp, i0 + PASS, end, graw);
-            load_run<DIR>(xp, i0 + PASS, end, xraw);
-        }
-        float pa = a[0], h = b[0];
+    };
+    int parity = 0;
+    auto enter = [&]() -> float {
+        float pa = a[0], pb = b[0];
 #pragma unroll
         for (int i = 1; i < N; ++i) {
             pa *= a[i];
-            h = fmaf(a[i], h, b[i]);
+            pb = fmaf(a[i], pb, b[i]);
         }
         Stretch before, all;
-        join_lanes<G>({pa, h}, before, all);
-        float enter = carry;
+        join_lanes<G>({pa, pb}, before, all);
+        float h = carry;
         if constexpr (W > 1) {
             if (lane_id() == 0) lds[parity][team][wave] = all;
             __syncthreads();
             float c = carry;
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                if (w == wave) enter = c;
+                if (w == wave) h = c;
                 const Stretch s = lds[parity][team][w];
                 c = through(s, c);
                 if constexpr (PARTIAL) product *= s.a;
             }
             carry = c;
+            parity ^= 1;
         } else {
             carry = through(all, carry);
             if constexpr (PARTIAL) product *= all.a;
         }
-        if constexpr (!PARTIAL) {
-            h = through(before, enter);
-            S out[N];
+        return through(before, h);
+    };
+    auto states = [&](float h, S (&out)[N]) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                h = fmaf(a[i], h, b[i]);
-                out[i] = static_cast<S>(h);
-            }
-            if (live) store_run<DIR>(yp, i0, end, out);
+        for (int i = 0; i < N; ++i) {
+            h = fmaf(a[i], h, b[i]);
+            out[i] = static_cast<S>(h);
+        }
+    };
+
+    const int64_t passes = (end - begin) / PASS;
+    int64_t i0 = begin + place * N;
+    auto fetch = [&](int64_t i) {
+        load_run<true, DIR>(gp, i, end, graw);
+        load_run<true, DIR>(xp, i, end, xraw);
+    };
+    if (passes > 0) fetch(i0);
+    for (int64_t pass = 0; pass < passes; ++pass, i0 += PASS) {
+        widen();
+        fetch(pass + 1 < passes ? i0 + PASS : i0);        // (after the last whole pass: values that nobody uses)
+        const float h = enter();
+        if constexpr (!PARTIAL) {
+            S out[N];
+            states(h, out);
+            store_run<true, DIR>(yp, i0, end, out);
         }
     }
-    if (place == 0 && live) {
+    if (begin + passes * PASS < end) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) graw[i] = neutral_gate<S, KIND>(), xraw[i] = static_cast<S>(0.0f);
+        load_run<false, DIR>(gp, i0, end, graw);
+        load_run<false, DIR>(xp, i0, end, xraw);
+        widen();
+        const float h = enter();
+        if constexpr (!PARTIAL) {
+            S out[N];
+            states(h, out);
+            store_run<false, DIR>(yp, i0, end, out);
+        }
+    }
+    if (place == 0) {
         if constexpr (PARTIAL) p.records[segment * p.cut.m + r] = {product, carry};
         else if (p.last.base && segment == p.cut.segments - 1) p.last.base[p.last.row.at(r)] = carry;
     }
@@ -347,13 +380,16 @@ int launch_scan(const ScanCall<S>& p, void* scratch, size_t scratch_bytes, hipSt
     if (d != 0 && d == direction(p.g) && d == direction(p.x))
         return d > 0 ? launch_direction<S, KIND, 1>(p, scratch, scratch_bytes, stream) : launch_direction<S, KIND, -1>(p, scratch, scratch_bytes, stream);
     if (!(short_offsets(p.g) && short_offsets(p.x) && short_offsets(p.y)))
-        return launch_cols<S, KIND, 1, 16, int64_t>(p, scratch, scratch_bytes, stream);
-    if (n <= 64) return launch_cols<S, KIND, 1, 4, uint32_t>(p, scratch, scratch_bytes, stream);
+        return launch_cols<S, KIND, 1, 16, int64_t, false>(p, scratch, scratch_bytes, stream);
+    if (n <= 64) return launch_cols<S, KIND, 1, 4, uint32_t, false>(p, scratch, scratch_bytes, stream);
+    const bool lines = whole_lines(p.g) && whole_lines(p.x) && whole_lines(p.y);
     if constexpr (sizeof(S) == 2) {
         if (ceil_div(m, 2 * kWave) >= 512 && pairs_of_rows(p.g) && pairs_of_rows(p.x) && pairs_of_rows(p.y))
-            return launch_cols<S, KIND, 2, 8, uint32_t>(p, scratch, scratch_bytes, stream);
+            return lines ? launch_cols<S, KIND, 2, 8, uint32_t, true>(p, scratch, scratch_bytes, stream)
+                         : launch_cols<S, KIND, 2, 8, uint32_t, false>(p, scratch, scratch_bytes, stream);
     }
-    return launch_cols<S, KIND, 1, 16, uint32_t>(p, scratch, scratch_bytes, stream);
+    return lines ? launch_cols<S, KIND, 1, 16, uint32_t, true>(p, scratch, scratch_bytes, stream)
+                 : launch_cols<S, KIND, 1, 16, uint32_t, false>(p, scratch, scratch_bytes, stream);
 }
 
 }  // namespace

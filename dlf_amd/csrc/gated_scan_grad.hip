@@ -56,7 +56,7 @@ constexpr int kGradSteps = 8;       // of a wavefront in a pass
 
 // Rows side by side, as in the forward kernel, from the last step to the first: position i of the
 // walk is step n - 1 - i.
-template <typename S, int KIND, int V, int W, typename OFF, bool PARTIAL>
+template <typename S, int KIND, int V, int W, typename OFF, bool NT, bool PARTIAL>
 __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
     constexpr int N = kGradSteps;
     __shared__ float lds[2][W][kWave][2 * V];
@@ -67,10 +67,9 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
     // (segments from the last one on after PARTIAL went from the first: what it read last may still be cached)
     const int64_t segment = PARTIAL ? work / p.cut.blocks : p.cut.segments - 1 - work / p.cut.blocks;
     const int64_t block = work % p.cut.blocks;
-    const int64_t r = (block * kWave + lane) * V;
-    const bool live = r < p.cut.m;
-    const int64_t rr = live ? r : p.cut.m - V;
-    auto offset = [&](const auto& track) { return static_cast<OFF>(track.row.at(rr) * static_cast<int64_t>(sizeof(S))); };
+    const int64_t wanted = (block * kWave + lane) * V;
+    const int64_t r = wanted < p.cut.m ? wanted : p.cut.m - V;
+    auto offset = [&](const auto& track) { return static_cast<OFF>(track.row.at(r) * static_cast<int64_t>(sizeof(S))); };
     const OFF go = offset(p.g), dyo = offset(p.dy);
     const OFF xo = KIND == kGatedBlend ? offset(p.x) : OFF(0);
     const OFF yo = offset(p.y), dgo = offset(p.dg), dxo = offset(p.dx);
@@ -85,22 +84,32 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
         product[v] = 1.0;
         carry[v] = h0[v] = 0.0f;
         if constexpr (!PARTIAL) {
-            if (segment == p.cut.segments - 1 && p.initial.base) h0[v] = p.initial.base[p.initial.row.at(rr + v)];
+            if (segment == p.cut.segments - 1 && p.initial.base) h0[v] = p.initial.base[p.initial.row.at(r + v)];
         }
         if (p.cut.segments == 1 || (PARTIAL && segment == 0)) {
-            const float d = p.dlast.base ? p.dlast.base[p.dlast.row.at(rr + v)] : 0.0f;
+            const float d = p.dlast.base ? p.dlast.base[p.dlast.row.at(r + v)] : 0.0f;
             if constexpr (PARTIAL) {
-                if (wave == 0 && live) p.entering[rr + v] = d;
+                if (wave == 0) p.entering[r + v] = d;
             } else {
                 carry[v] = d;
             }
         } else if (!PARTIAL) {
-            carry[v] = p.entering[rr + v];
-            for (int64_t s = 0; s < segment; ++s) carry[v] = through(p.records[s * p.cut.m + rr + v], carry[v]);
+            carry[v] = p.entering[r + v];
+            for (int64_t s = 0; s < segment; ++s) carry[v] = through(p.records[s * p.cut.m + r + v], carry[v]);
         }
     }
 
     Vec<S, V> graw[N], dyraw[N], yraw[N], xraw[N];
+    float a[N][V], d[N][V], keep[N][V], side[N][V];
+    // Position i0 + i: the state before it is the next position's, for the axis's last one `initial`.
+    auto fetch_one = [&](int i, const S* gp, const S* dyp, const S* yp, const S* xp, OFF gi, OFF dyi, OFF yi, OFF xi) {
+        graw[i] = load_at<NT, S, V>(gp, gi);
+        dyraw[i] = load_at<NT, S, V>(dyp, dyi);
+        if constexpr (!PARTIAL) {
+            yraw[i] = load_at<NT, S, V>(yp, yi);
+            if constexpr (KIND == kGatedBlend) xraw[i] = load_at<NT, S, V>(xp, xi);
+        }
+    };
     auto fetch = [&](int64_t i0) {
         const int64_t t0 = top - i0;
         const S* gp = p.g.base + t0 * p.g.step;
@@ -108,40 +117,16 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
         const S* yp = p.y.base + (t0 - 1) * p.y.step;
         const S* xp = KIND == kGatedBlend ? p.x.base + t0 * p.x.step : nullptr;
         const OFF gi = as_it_is(go), dyi = as_it_is(dyo), yi = as_it_is(yo), xi = as_it_is(xo);
-        auto one = [&](int i, bool first_step) {
-            graw[i] = load_at<S, V>(gp, gi);
-            dyraw[i] = load_at<S, V>(dyp, dyi);
-            if constexpr (!PARTIAL) {
-                if (!first_step) yraw[i] = load_at<S, V>(yp, yi);
-                if constexpr (KIND == kGatedBlend) xraw[i] = load_at<S, V>(xp, xi);
-            }
-        };
-        auto on = [&] {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            fetch_one(i, gp, dyp, yp, xp, gi, dyi, yi, xi);
             gp -= p.g.step;
             dyp -= p.dy.step;
             yp -= p.y.step;
             if constexpr (KIND == kGatedBlend) xp -= p.x.step;
-        };
-        if (i0 + N <= end && i0 + N <= top) {
-#pragma unroll
-            for (int i = 0; i < N; ++i, on()) one(i, false);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i, on()) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    graw[i].v[v] = neutral_gate<S, KIND>();
-                    dyraw[i].v[v] = yraw[i].v[v] = xraw[i].v[v] = static_cast<S>(0.0f);
-                }
-                if (i0 + i < end) one(i, i0 + i == top);          // (before the first step: initial, below)
-            }
         }
     };
-    int64_t i0 = begin + wave * N;
-    fetch(i0);
-    int parity = 0;
-    for (int64_t pass = begin; pass < end; pass += W * N, i0 += W * N, parity ^= 1) {
-        float a[N][V], d[N][V], keep[N][V], side[N][V];
+    auto widen = [&](int64_t i0, bool last) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
 #pragma unroll
@@ -150,26 +135,27 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
                 float before = 0.0f, x = 0.0f;
                 if constexpr (!PARTIAL) {
                     before = static_cast<float>(yraw[i].v[v]);
-                    if (i0 + i == top) before = h0[v];
+                    if (last && i0 + i == top) before = h0[v];
                     if constexpr (KIND == kGatedBlend) x = static_cast<float>(xraw[i].v[v]);
                 }
                 step_of<S, KIND>(static_cast<float>(graw[i].v[v]), x, before, a[i][v], keep[i][v], side[i][v]);
             }
         }
-        if (pass + W * N < end) fetch(i0 + W * N);
+    };
+    int parity = 0;
+    auto enter = [&](float (&mu)[V]) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            float pa = a[0][v], mu = a[0][v] * d[0][v];
+            float pa = a[0][v], pb = a[0][v] * d[0][v];
 #pragma unroll
             for (int i = 1; i < N; ++i) {
                 pa *= a[i][v];
-                mu = a[i][v] * (d[i][v] + mu);
+                pb = a[i][v] * (d[i][v] + pb);
             }
             lds[parity][wave][lane][2 * v] = pa;
-            lds[parity][wave][lane][2 * v + 1] = mu;
+            lds[parity][wave][lane][2 * v + 1] = pb;
         }
         __syncthreads();
-        float mu[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float c = carry[v], mine = carry[v];
@@ -183,41 +169,72 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
             carry[v] = c;
             mu[v] = mine;
         }
+        parity ^= 1;
+    };
+    auto gradient = [&](int i, float (&mu)[V], Vec<S, V>& dg, Vec<S, V>& dx) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const float lam = d[i][v] + mu[v];
+            mu[v] = a[i][v] * lam;
+            dg.v[v] = static_cast<S>(lam * side[i][v]);
+            dx.v[v] = static_cast<S>(KIND == kGatedBlend ? lam * keep[i][v] : lam);
+        }
+    };
+
+    // whole passes, but for one that holds the axis's last position
+    const int64_t reach = end < top ? end : top;
+    const int64_t passes = reach > begin ? (reach - begin) / (W * N) : 0;
+    int64_t i0 = begin + wave * N;
+    if (passes > 0) fetch(i0);
+    for (int64_t pass = 0; pass < passes; ++pass, i0 += W * N) {
+        widen(i0, false);
+        fetch(pass + 1 < passes ? i0 + W * N : i0);       // (after the last whole pass: values that nobody uses)
+        float mu[V];
+        enter(mu);
         if constexpr (!PARTIAL) {
-            Vec<S, V> dg[N], dx[N];
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const float lam = d[i][v] + mu[v];
-                    mu[v] = a[i][v] * lam;
-                    dg[i].v[v] = static_cast<S>(lam * side[i][v]);
-                    dx[i].v[v] = static_cast<S>(KIND == kGatedBlend ? lam * keep[i][v] : lam);
-                }
-            }
             S* dgp = p.dg.base + (top - i0) * p.dg.step;
             S* dxp = p.dx.base + (top - i0) * p.dx.step;
             const OFF dgi = as_it_is(dgo), dxi = as_it_is(dxo);
-            if (i0 + N <= end) {
-                if (live) {
 #pragma unroll
-                    for (int i = 0; i < N; ++i, dgp -= p.dg.step, dxp -= p.dx.step) {
-                        store_at<S, V>(dgp, dgi, dg[i]);
-                        store_at<S, V>(dxp, dxi, dx[i]);
-                    }
-                }
-            } else if (live) {
+            for (int i = 0; i < N; ++i, dgp -= p.dg.step, dxp -= p.dx.step) {
+                Vec<S, V> dg, dx;
+                gradient(i, mu, dg, dx);
+                store_at<NT, S, V>(dgp, dgi, dg);
+                store_at<NT, S, V>(dxp, dxi, dx);
+            }
+        }
+    }
+    if (begin + passes * (W * N) < end) {
 #pragma unroll
-                for (int i = 0; i < N; ++i, dgp -= p.dg.step, dxp -= p.dx.step) {
-                    if (i0 + i < end) {
-                        store_at<S, V>(dgp, dgi, dg[i]);
-                        store_at<S, V>(dxp, dxi, dx[i]);
-                    }
+        for (int i = 0; i < N; ++i) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                graw[i].v[v] = neutral_gate<S, KIND>();
+                dyraw[i].v[v] = yraw[i].v[v] = xraw[i].v[v] = static_cast<S>(0.0f);
+            }
+            const int64_t t = top - i0 - i;
+            if (i0 + i < end)
+                fetch_one(i, p.g.base + t * p.g.step, p.dy.base + t * p.dy.step, p.y.base + (t > 0 ? t - 1 : 0) * p.y.step,
+                          KIND == kGatedBlend ? p.x.base + t * p.x.step : nullptr, go, dyo, yo, xo);
+        }
+        widen(i0, true);
+        float mu[V];
+        enter(mu);
+        if constexpr (!PARTIAL) {
+            S* dgp = p.dg.base + (top - i0) * p.dg.step;
+            S* dxp = p.dx.base + (top - i0) * p.dx.step;
+#pragma unroll
+            for (int i = 0; i < N; ++i, dgp -= p.dg.step, dxp -= p.dx.step) {
+                Vec<S, V> dg, dx;
+                gradient(i, mu, dg, dx);
+                if (i0 + i < end) {
+                    store_at<NT, S, V>(dgp, dgo, dg);
+                    store_at<NT, S, V>(dxp, dxo, dx);
                 }
             }
         }
     }
-    if (wave == 0 && live) {
+    if (wave == 0) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             if constexpr (PARTIAL) p.records[segment * p.cut.m + r + v] = {product[v], carry[v]};
@@ -226,7 +243,7 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
     }
 }
 
-template <typename S, int KIND, int V, int W, typename OFF>
+template <typename S, int KIND, int V, int W, typename OFF, bool NT>
 int launch_cols(GradCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     p.cut.blocks = ceil_div(p.cut.m, kWave * V);
     int64_t segments = segments_of(p.cut.blocks, p.cut.n, W * kGradSteps, 192, kColumnSegments);
@@ -237,10 +254,10 @@ int launch_cols(GradCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t 
     if (segments > 1) {
         p.records = static_cast<Stretch*>(scratch);
         p.entering = reinterpret_cast<float*>(static_cast<char*>(scratch) + align_up(static_cast<size_t>(p.cut.m * (segments - 1)) * sizeof(Stretch), 256));
-        gated_grad_cols<S, KIND, V, W, OFF, true><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * (segments - 1)))), dim3(W * kWave), 0, stream>>>(p);
+        gated_grad_cols<S, KIND, V, W, OFF, NT, true><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * (segments - 1)))), dim3(W * kWave), 0, stream>>>(p);
         DLFX_CHECK_LAUNCH();
     }
-    gated_grad_cols<S, KIND, V, W, OFF, false><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * segments))), dim3(W * kWave), 0, stream>>>(p);
+    gated_grad_cols<S, KIND, V, W, OFF, NT, false><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * segments))), dim3(W * kWave), 0, stream>>>(p);
     DLFX_CHECK_LAUNCH();
     return DLFX_OK;
 }
@@ -256,12 +273,12 @@ __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_grad_rows(GradC
     __shared__ Stretch lds[W > 1 ? 2 : 1][W > 1 ? TEAMS : 1][W];
     const int team = threadIdx.x / TEAM, place = threadIdx.x % TEAM, wave = place / kWave;
     const int64_t segment = PARTIAL ? blockIdx.x / p.cut.blocks : p.cut.segments - 1 - blockIdx.x / p.cut.blocks;
-    const int64_t r = (blockIdx.x % p.cut.blocks) * TEAMS + team;
-    const bool live = r < p.cut.m;
-    const int64_t rr = live ? r : p.cut.m - 1;
+    const int64_t wanted = (blockIdx.x % p.cut.blocks) * TEAMS + team;
+    if (wanted - (W == 1 ? threadIdx.x % kWave / G : 0) >= p.cut.m) return;      // (as in the forward kernel)
+    const int64_t r = wanted < p.cut.m ? wanted : p.cut.m - 1;
     const int64_t n = p.cut.n, top = n - 1;
     // position i of the walk is step n - 1 - i, DIR elements further on in memory each
-    auto start = [&](const auto& track) { return track.base + track.row.at(rr) - DIR * top; };
+    auto start = [&](const auto& track) { return track.base + track.row.at(r) - DIR * top; };
     const S* gp = start(p.g);
     const S* dyp = start(p.dy);
     const S* xp = KIND == kGatedBlend ? start(p.x) : nullptr;
@@ -274,92 +291,121 @@ __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_grad_rows(GradC
     float carry = 0.0f, h0 = 0.0f;
     double product = 1.0;
     if constexpr (!PARTIAL) {
-        if (segment == p.cut.segments - 1 && p.initial.base) h0 = p.initial.base[p.initial.row.at(rr)];
+        if (segment == p.cut.segments - 1 && p.initial.base) h0 = p.initial.base[p.initial.row.at(r)];
     }
     if (p.cut.segments == 1 || (PARTIAL && segment == 0)) {
-        const float d = p.dlast.base ? p.dlast.base[p.dlast.row.at(rr)] : 0.0f;
+        const float d = p.dlast.base ? p.dlast.base[p.dlast.row.at(r)] : 0.0f;
         if constexpr (PARTIAL) {
-            if (place == 0 && live) p.entering[rr] = d;
+            if (place == 0) p.entering[r] = d;
         } else {
             carry = d;
         }
     } else if (!PARTIAL) {
-        carry = p.entering[rr];
-        if constexpr (W > 4) carry = enter_segment(p.records, p.cut.m, rr, segment, carry);
+        carry = p.entering[r];
+        if constexpr (W > 4) carry = enter_segment(p.records, p.cut.m, r, segment, carry);
     }
 
     S graw[N], dyraw[N], yraw[N], xraw[N];
-    auto fetch = [&](int64_t i0) {
-        load_run<DIR>(gp, i0, end, graw);
-        load_run<DIR>(dyp, i0, end, dyraw);
+    float a[N], d[N], keep[N], side[N];
+    auto fetch = [&](int64_t i) {
+        load_run<true, DIR>(gp, i, end, graw);
+        load_run<true, DIR>(dyp, i, end, dyraw);
         if constexpr (!PARTIAL) {
-            load_run<DIR>(before_p, i0, end < top ? end : top, yraw);      // (the last position: initial, below)
-            if constexpr (KIND == kGatedBlend) load_run<DIR>(xp, i0, end, xraw);
+            load_run<true, DIR>(before_p, i, end, yraw);
+            if constexpr (KIND == kGatedBlend) load_run<true, DIR>(xp, i, end, xraw);
         }
     };
-    int64_t i0 = begin + place * N;
-    fetch(i0);
-    int parity = 0;
-    for (int64_t pass = begin; pass < end; pass += PASS, i0 += PASS, parity ^= 1) {
-        float a[N], d[N], keep[N], side[N];
+    auto widen = [&](int64_t i0, bool last) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             d[i] = static_cast<float>(dyraw[i]);
             float before = 0.0f, x = 0.0f;
             if constexpr (!PARTIAL) {
-                before = i0 + i == top ? h0 : static_cast<float>(yraw[i]);
+                before = static_cast<float>(yraw[i]);
+                if (last && i0 + i == top) before = h0;
                 if constexpr (KIND == kGatedBlend) x = static_cast<float>(xraw[i]);
             }
             step_of<S, KIND>(static_cast<float>(graw[i]), x, before, a[i], keep[i], side[i]);
         }
-        if (i0 + N > end) {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (i0 + i >= end) a[i] = 1.0f, d[i] = 0.0f;
-        }
-        if (pass + PASS < end) fetch(i0 + PASS);
-        float pa = a[0], mu = a[0] * d[0];
+    };
+    int parity = 0;
+    auto enter = [&]() -> float {
+        float pa = a[0], pb = a[0] * d[0];
 #pragma unroll
         for (int i = 1; i < N; ++i) {
             pa *= a[i];
-            mu = a[i] * (d[i] + mu);
+            pb = a[i] * (d[i] + pb);
         }
         Stretch before, all;
-        join_lanes<G>({pa, mu}, before, all);
-        float enter = carry;
+        join_lanes<G>({pa, pb}, before, all);
+        float mu = carry;
         if constexpr (W > 1) {
             if (lane_id() == 0) lds[parity][team][wave] = all;
             __syncthreads();
             float c = carry;
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                if (w == wave) enter = c;
+                if (w == wave) mu = c;
                 const Stretch s = lds[parity][team][w];
                 c = through(s, c);
                 if constexpr (PARTIAL) product *= s.a;
             }
             carry = c;
+            parity ^= 1;
         } else {
             carry = through(all, carry);
             if constexpr (PARTIAL) product *= all.a;
         }
-        if constexpr (!PARTIAL) {
-            mu = through(before, enter);
-            S dg[N], dx[N];
+        return through(before, mu);
+    };
+    auto gradients = [&](float mu, S (&dg)[N], S (&dx)[N]) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float lam = d[i] + mu;
-                mu = a[i] * lam;
-                dg[i] = static_cast<S>(lam * side[i]);
-                dx[i] = static_cast<S>(KIND == kGatedBlend ? lam * keep[i] : lam);
-            }
-            if (live) {
-                store_run<DIR>(dgp, i0, end, dg);
-                store_run<DIR>(dxp, i0, end, dx);
-            }
+        for (int i = 0; i < N; ++i) {
+            const float lam = d[i] + mu;
+            mu = a[i] * lam;
+            dg[i] = static_cast<S>(lam * side[i]);
+            dx[i] = static_cast<S>(KIND == kGatedBlend ? lam * keep[i] : lam);
+        }
+    };
+
+    // whole passes, but for one that holds the axis's last position
+    const int64_t reach = end < top ? end : top;
+    const int64_t passes = reach > begin ? (reach - begin) / PASS : 0;
+    int64_t i0 = begin + place * N;
+    if (passes > 0) fetch(i0);
+    for (int64_t pass = 0; pass < passes; ++pass, i0 += PASS) {
+        widen(i0, false);
+        fetch(pass + 1 < passes ? i0 + PASS : i0);        // (after the last whole pass: values that nobody uses)
+        const float mu = enter();
+        if constexpr (!PARTIAL) {
+            S dg[N], dx[N];
+            gradients(mu, dg, dx);
+            store_run<true, DIR>(dgp, i0, end, dg);
+            store_run<true, DIR>(dxp, i0, end, dx);
         }
     }
-    if (place == 0 && live) {
+    if (begin + passes * PASS < end) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            graw[i] = neutral_gate<S, KIND>();
+            dyraw[i] = yraw[i] = xraw[i] = static_cast<S>(0.0f);
+        }
+        load_run<false, DIR>(gp, i0, end, graw);
+        load_run<false, DIR>(dyp, i0, end, dyraw);
+        if constexpr (!PARTIAL) {
+            load_run<false, DIR>(before_p, i0, reach, yraw);
+            if constexpr (KIND == kGatedBlend) load_run<false, DIR>(xp, i0, end, xraw);
+        }
+        widen(i0, true);
+        const float mu = enter();
+        if constexpr (!PARTIAL) {
+            S dg[N], dx[N];
+            gradients(mu, dg, dx);
+            store_run<false, DIR>(dgp, i0, end, dg);
+            store_run<false, DIR>(dxp, i0, end, dx);
+        }
+    }
+    if (place == 0) {
         if constexpr (PARTIAL) p.records[segment * p.cut.m + r] = {product, carry};
         else if (p.dinitial.base && segment == p.cut.segments - 1) p.dinitial.base[p.dinitial.row.at(r)] = carry;
     }
@@ -410,14 +456,17 @@ int launch_grad(const GradCall<S>& p, void* scratch, size_t scratch_bytes, hipSt
     if (d != 0 && d == direction(p.g) && d == direction(p.dy) && d == direction(p.dg) && d == direction(p.dx) && (KIND != kGatedBlend || d == direction(p.x)))
         return d > 0 ? launch_direction<S, KIND, -1>(p, scratch, scratch_bytes, stream) : launch_direction<S, KIND, 1>(p, scratch, scratch_bytes, stream);
     if (!(short_offsets(p.g) && short_offsets(p.x) && short_offsets(p.y) && short_offsets(p.dy) && short_offsets(p.dg) && short_offsets(p.dx)))
-        return launch_cols<S, KIND, 1, 16, int64_t>(p, scratch, scratch_bytes, stream);
-    if (n <= 64) return launch_cols<S, KIND, 1, 4, uint32_t>(p, scratch, scratch_bytes, stream);
+        return launch_cols<S, KIND, 1, 16, int64_t, false>(p, scratch, scratch_bytes, stream);
+    if (n <= 64) return launch_cols<S, KIND, 1, 4, uint32_t, false>(p, scratch, scratch_bytes, stream);
+    const bool lines = whole_lines(p.g) && whole_lines(p.x) && whole_lines(p.y) && whole_lines(p.dy) && whole_lines(p.dg) && whole_lines(p.dx);
     if constexpr (sizeof(S) == 2) {
         if (ceil_div(m, 2 * kWave) >= 512 && pairs_of_rows(p.g) && pairs_of_rows(p.x) && pairs_of_rows(p.y) && pairs_of_rows(p.dy) &&
             pairs_of_rows(p.dg) && pairs_of_rows(p.dx))
-            return launch_cols<S, KIND, 2, 8, uint32_t>(p, scratch, scratch_bytes, stream);
+            return lines ? launch_cols<S, KIND, 2, 8, uint32_t, true>(p, scratch, scratch_bytes, stream)
+                         : launch_cols<S, KIND, 2, 8, uint32_t, false>(p, scratch, scratch_bytes, stream);
     }
-    return launch_cols<S, KIND, 1, 16, uint32_t>(p, scratch, scratch_bytes, stream);
+    return lines ? launch_cols<S, KIND, 1, 16, uint32_t, true>(p, scratch, scratch_bytes, stream)
+                 : launch_cols<S, KIND, 1, 16, uint32_t, false>(p, scratch, scratch_bytes, stream);
 }
 
 }  // namespace
