@@ -167,6 +167,25 @@ def test_in_place(hip_backend, extents, axis):
         assert O.close(S.numpy().reshape(-1), want[-1], err[-1], "f32")
 
 
+@pytest.mark.parametrize("n", [15, 63, 64, 65, 257, 1023, 1025, 2049, 4097, 33001])
+@pytest.mark.parametrize("start", [0, 1, 2, 3])
+def test_rows_on_odd_elements(hip_backend, n, start):
+    # two-byte rows along memory that start on any element, at even and odd pitches
+    kind, dtype, m = "gated_blend", "f16", 5
+    for pitch in (n + 3, n + 4):
+        for reverse in (False, True):
+            wide = [stored(kind, 400 + i, (m, pitch + start), dtype, gate=i == 0) for i in range(3)]
+            T = [Tensor.from_numpy(hip_backend, w).slice([start], [start + n], [1]) for w in wide]
+            v = [np.ascontiguousarray(w[:, start:start + n]) for w in wide]
+            initial = normal(410, m).astype(np.float32)
+            rest = Tensor.from_numpy(hip_backend, np.zeros((m, pitch + start), np.float16))
+            out = rest.slice([start], [start + n], [1])
+            Y, _ = check_forward(hip_backend, kind, dtype, (T[0], v[0]), (T[1], v[1]), 1, reverse, initial, out=out)
+            got = rest.numpy()
+            assert (got[:, :start] == 0).all() and (got[:, start + n:] == 0).all()          # nothing beside the rows
+            check_grad(hip_backend, kind, dtype, (T[0], v[0]), (T[1], v[1]), (Y, Y.numpy()), (T[2], v[2]), 1, reverse, initial)
+
+
 def test_decoding_equals_the_long_call(hip_backend):
     kind, dtype, shape = "gated_sigmoid", "f32", (5, 12, 33)
     G, X = pair(hip_backend, stored(kind, 91, shape, dtype, gate=True)), pair(hip_backend, stored(kind, 92, shape, dtype))
