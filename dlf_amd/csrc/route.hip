@@ -76,8 +76,8 @@ struct RouteCall {
 // the row's 1 / sum: 64 u of that is taken.  The sum with the bias rounds once: 2 u, 4 u taken.
 __device__ __forceinline__ float border(float scores, float a, float b) { return scores + 0x1p-22f * fmaxf(fabsf(a), fabsf(b)); }
 
-// LDS of a team: the items' values and the groups' (fp32), or the groups' (64 bits), or the candidates;
-// then a byte per group.  (8 of 32 doubles left over: the teams of a wavefront start 16 banks apart.)
+// LDS of a team: the items' values and the groups', or the candidates, then a byte per group.  (8 of 32
+// doubles left over: the teams of a wavefront start 16 banks apart.)
 template <int L, int ITEMS>
 constexpr int team_doubles() { return L * ITEMS + L * ITEMS / 8 + (40 - (L * ITEMS + L * ITEMS / 8) % 32) % 32; }
 
@@ -105,14 +105,10 @@ struct Best {
     }
 };
 
-// Values of the groups in sums[]; value[i]: what a present item adds to its group.
-template <int L, int ITEMS>
-__device__ __forceinline__ void group_values(const RouteCall& p, const float (&value)[ITEMS], uint32_t present, float* items, float* sums, int lane) {
-    const float none = -std::numeric_limits<float>::infinity();
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-        if (i * L + lane < p.n) items[i * L + lane] = (present >> i & 1) ? value[i] : std::numeric_limits<float>::quiet_NaN();
-    wave_sync();
+// Values of the groups in sums[] from their experts' in items[] (NaN: absent), by a team of L lanes.
+template <int L, typename C>
+__device__ __forceinline__ void group_values(const RouteCall& p, const C* items, C* sums, int lane) {
+    const C none = -std::numeric_limits<C>::infinity();
     // lanes_per lanes (a power of two) to a group; a lane walks its part of the group's experts from a
     // place of its own, so that the lanes read different LDS banks
     int lanes_per = L;
@@ -120,7 +116,7 @@ __device__ __forceinline__ void group_values(const RouteCall& p, const float (&v
     const int part = lane & (lanes_per - 1), side_by_side = L / lanes_per;
     for (int g0 = 0; g0 < p.groups; g0 += side_by_side) {
         const int g = g0 + lane / lanes_per;
-        Best<float> best = {none, none, 0};
+        Best<C> best = {none, none, 0};
         if (g < p.groups) {
             const int from = g - p.size * ((g * p.size_magic) >> 20);
             for (int i = part; i < p.size; i += lanes_per) {
@@ -134,25 +130,11 @@ __device__ __forceinline__ void group_values(const RouteCall& p, const float (&v
     }
     wave_sync();
 }
-// The same in 64 bits, a group at a time (rows that fp32 does not settle).
-template <int L, int ITEMS>
-__device__ __forceinline__ void group_values(const RouteCall& p, const double (&value)[ITEMS], uint32_t present, double* sums, int lane) {
-    const double none = -std::numeric_limits<double>::infinity();
-    for (int g = 0; g < p.groups; ++g) {
-        Best<double> best = {none, none, 0};
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if ((present >> i & 1) && ((i * L + lane) * p.size_magic) >> 20 == g) best.add(value[i]);
-        for (int j = 1; j < L; j <<= 1) best.add({lane_xor(best.first, j), lane_xor(best.second, j), lane_xor(best.count, j)});
-        if (lane == 0) sums[g] = best.value(p.group_best);
-    }
-    wave_sync();
-}
 
-// Which items lie in a kept group, a bit per item of the lane.  `unsure` when the values are not exact
-// and a kept group's lies too close to one that was left.
-template <typename C, int L, int ITEMS>
-__device__ __forceinline__ uint32_t kept_items(const RouteCall& p, const C* sums, uint8_t* kept, bool exact, float scores, int lane, bool& unsure) {
+// Which groups are kept, a byte each.  `unsure` when the values are not exact and a kept group's lies too
+// close to one that was left.
+template <int L, typename C>
+__device__ __forceinline__ void keep_groups(const RouteCall& p, const C* sums, uint8_t* kept, bool exact, float scores, int lane, bool& unsure) {
     const C none = -std::numeric_limits<C>::infinity();
     C worst_kept = -none, best_left = none;
     for (int g = lane; g < p.groups; g += L) {
@@ -172,12 +154,6 @@ __device__ __forceinline__ uint32_t kept_items(const RouteCall& p, const C* sums
         }
     }
     wave_sync();
-    uint32_t open = 0;
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        const int e = i * L + lane;
-        if (e < p.n && kept[(e * p.size_magic) >> 20]) open |= 1u << i;
-    }
     if (!exact) {
         worst_kept = team_reduce<L>(worst_kept, [](C a, C b) { return b < a ? b : a; });
         best_left = team_reduce<L>(best_left, [](C a, C b) { return b > a ? b : a; });
@@ -185,27 +161,24 @@ __device__ __forceinline__ uint32_t kept_items(const RouteCall& p, const C* sums
         const float a = static_cast<float>(worst_kept), b = static_cast<float>(best_left);
         if (best_left != none && !(a - b > 2.0f * border(scores, a, b))) unsure = true;
     }
-    return open;
 }
 
+// A row's logits, the absent ones -inf.
 template <typename S, int KIND, int L, int ITEMS>
 struct RouteRow {
     float x[ITEMS];
-    uint32_t present;
-    float mx, inverse;        // softmax: the largest present logit, 1 / sum of exp(x - mx)
+    float mx, inverse;        // softmax: the largest logit (a finite number), 1 / sum of exp(x - mx)
 
     __device__ __forceinline__ void load(const S* row, int n, int lane) {
-        present = 0;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) x[i] = i * L + lane < n ? static_cast<float>(row[i * L + lane]) : kMinusInfinity;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) present |= (x[i] <= lowest_of<S>() ? 0u : 1u) << i;
-        mx = kMinusInfinity;
+        for (int i = 0; i < ITEMS; ++i) x[i] = x[i] <= lowest_of<S>() ? kMinusInfinity : x[i];
+        mx = -std::numeric_limits<float>::max();
         inverse = 0.0f;
         if constexpr (KIND == kSoftmaxScore) {
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i)
-                if (present >> i & 1) mx = fmaxf(mx, x[i]);
+            for (int i = 0; i < ITEMS; ++i) mx = fmaxf(mx, x[i]);
             mx = team_reduce<L>(mx, [](float a, float b) { return fmaxf(a, b); });
         }
     }
@@ -213,8 +186,7 @@ struct RouteRow {
         if constexpr (KIND == kSoftmaxScore) {
             float sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i)
-                if (present >> i & 1) sum += power(x[i]);
+            for (int i = 0; i < ITEMS; ++i) sum += power(x[i]);
             sum = team_reduce<L>(sum, [](float a, float b) { return a + b; });
             inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
         }
@@ -225,64 +197,75 @@ struct RouteRow {
         if constexpr (KIND == kSoftmaxScore) {
             return power(v) * inverse;
         } else {
-            const float e = __builtin_amdgcn_exp2f(-fabsf(v) * kLog2E), r = 1.0f / (1.0f + e);
+            const float e = __builtin_amdgcn_exp2f(-fabsf(v) * kLog2E), r = __builtin_amdgcn_rcpf(1.0f + e);
             return v < 0.0f ? e * r : r;
         }
     }
 };
 
-// The k choices in 64 bits, one after the other: place t ends in lane t.
-template <typename S, int KIND, int L, int ITEMS>
-__device__ __forceinline__ int choose_exactly(const RouteCall& p, const RouteRow<S, KIND, L, ITEMS>& row, double* lds, int lane) {
-    double value[ITEMS];
-    double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        const double v = row.x[i];
-        if constexpr (KIND == kSoftmaxScore) value[i] = (row.present >> i & 1) ? exp(v - static_cast<double>(row.mx)) : 0.0;
-        else value[i] = 1.0 / (1.0 + exp(-v));
-        sum += value[i];
-    }
+// The k choices of one row in 64 bits by a wavefront, one after the other: place t ends in lane t.
+template <typename S, int KIND>
+__device__ __forceinline__ int choose_exactly(const RouteCall& p, const S* x, double* items, int lane) {
+    double mx = -std::numeric_limits<float>::max(), sum = 0.0;
+    auto logit = [&](int e) {
+        const float v = static_cast<float>(x[e]);
+        return v <= lowest_of<S>() ? kMinusInfinity : v;
+    };
     if constexpr (KIND == kSoftmaxScore) {
-        sum = team_reduce<L>(sum, [](double a, double b) { return a + b; });
-        const double by = sum == 0.0 ? 0.0 : 1.0 / sum;
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) value[i] *= by;
+#pragma unroll 1
+        for (int e = lane; e < p.n; e += kWave) mx = fmax(mx, static_cast<double>(logit(e)));
+        mx = wave_reduce(mx, [](double a, double b) { return b > a ? b : a; });
     }
-    if (p.bias) {
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (i * L + lane < p.n) value[i] += static_cast<double>(p.bias[i * L + lane]);
+    wave_sync();
+#pragma unroll 1
+    for (int e = lane; e < p.n; e += kWave) {
+        const double v = logit(e);
+        const double s = KIND == kSoftmaxScore ? exp(v - mx) : 1.0 / (1.0 + exp(-v));
+        sum += s;
+        items[e] = s;
     }
-    uint32_t open = 0xffffffffu;
-    bool unsure = false;
-    if (p.kept_groups < p.groups) {
-        if (!p.bias && p.group_best == 1) {
-#pragma unroll
-            for (int i = 0; i < ITEMS; ++i) value[i] = row.x[i];
-        }
-        wave_sync();
-        group_values<L, ITEMS>(p, value, row.present, lds, lane);
-        open = kept_items<double, L, ITEMS>(p, lds, reinterpret_cast<uint8_t*>(lds + L * ITEMS), true, 0.0f, lane, unsure);
+    double by = 1.0;
+    if constexpr (KIND == kSoftmaxScore) {
+        sum = wave_reduce(sum, [](double a, double b) { return a + b; });
+        by = sum == 0.0 ? 0.0 : 1.0 / sum;
     }
-    uint64_t image[ITEMS];
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        const double c = p.bias ? value[i] : static_cast<double>(row.x[i]);
-        image[i] = i * L + lane >= p.n || !(open >> i & 1) ? 0 : (row.present >> i & 1) ? image_of(c) : 1;
+    // (a lane reads back what it wrote)
+#pragma unroll 1
+    for (int e = lane; e < p.n; e += kWave) {
+        const float v = logit(e);
+        double c = items[e] * by + (p.bias ? static_cast<double>(p.bias[e]) : 0.0);
+        if (!p.bias && (p.kept_groups == p.groups || p.group_best == 1)) c = v;
+        items[e] = v == kMinusInfinity ? std::numeric_limits<double>::quiet_NaN() : c;
+    }
+    wave_sync();
+    const bool grouped = p.kept_groups < p.groups;
+    uint8_t* flags = reinterpret_cast<uint8_t*>(items + p.n + p.n / 2);
+    if (grouped) {
+        double* sums = items;                                // (groups of one expert are their experts)
+        bool settled = false;
+        if (p.size > 1) group_values<kWave>(p, items, sums = items + p.n, lane);
+        keep_groups<kWave>(p, sums, flags, true, 0.0f, lane, settled);
+    }
+    uint64_t* images = reinterpret_cast<uint64_t*>(items);
+#pragma unroll 1
+    for (int e = lane; e < p.n; e += kWave) {
+        double c = items[e];
+        if (!p.bias && c == c) c = logit(e);
+        images[e] = grouped && !flags[(e * p.size_magic) >> 20] ? 0 : image_of(c);
     }
     int mine = 0;
+#pragma unroll 1
     for (int t = 0; t < p.k; ++t) {
         uint64_t best = 0;
         int at = 0x7fffffff;
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (image[i] > best) best = image[i], at = i * L + lane;
-        const uint64_t top = team_reduce<L>(best, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-        at = team_reduce<L>(best == top ? at : 0x7fffffff, [](int a, int b) { return a < b ? a : b; });
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (i * L + lane == at) image[i] = 0;
+#pragma unroll 1
+        for (int e = lane; e < p.n; e += kWave) {
+            const uint64_t v = images[e];
+            if (v > best) best = v, at = e;
+        }
+        const uint64_t top = wave_reduce(best, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+        at = wave_reduce(best == top ? at : 0x7fffffff, [](int a, int b) { return a < b ? a : b; });
+        if (at % kWave == lane) images[at] = 0;              // (its own lane's)
         if (lane == t) mine = at;
     }
     return mine;
@@ -292,7 +275,6 @@ __device__ __forceinline__ int choose_exactly(const RouteCall& p, const RouteRow
 template <typename S, int KIND, int L, int ITEMS>
 __device__ __forceinline__ int choose(const RouteCall& p, const RouteRow<S, KIND, L, ITEMS>& row, const S* x, float* lds, int lane, bool& unsure) {
     uint32_t image[ITEMS];
-    uint32_t open = 0xffffffffu;
     {
         float c[ITEMS];
 #pragma unroll
@@ -300,19 +282,34 @@ __device__ __forceinline__ int choose(const RouteCall& p, const RouteRow<S, KIND
             c[i] = row.x[i];
             if (p.bias) c[i] = row.score(c[i]) + (i * L + lane < p.n ? p.bias[i * L + lane] : 0.0f);
         }
-        if (p.kept_groups < p.groups) {
+        const bool grouped = p.kept_groups < p.groups;
+        uint8_t* flags = reinterpret_cast<uint8_t*>(lds + 2 * L * ITEMS);
+        if (grouped) {
             // (without a bias: by the scores where two are added, else by the logits themselves)
             const bool exact = !p.bias && p.group_best == 1;
-            float v[ITEMS];
-#pragma unroll
-            for (int i = 0; i < ITEMS; ++i) v[i] = p.bias || exact ? c[i] : row.score(row.x[i]);
             wave_sync();
-            group_values<L, ITEMS>(p, v, row.present, lds, lds + L * ITEMS, lane);
-            open = kept_items<float, L, ITEMS>(p, lds + L * ITEMS, reinterpret_cast<uint8_t*>(lds + 2 * L * ITEMS), exact, row.error(), lane, unsure);
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const float v = p.bias || exact ? c[i] : row.score(row.x[i]);
+                if (i * L + lane < p.n) lds[i * L + lane] = row.x[i] == kMinusInfinity ? std::numeric_limits<float>::quiet_NaN() : v;
+            }
+            wave_sync();
+            group_values<L>(p, lds, lds + L * ITEMS, lane);
+            keep_groups<L>(p, lds + L * ITEMS, flags, exact, row.error(), lane, unsure);
         }
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            image[i] = i * L + lane >= p.n || !(open >> i & 1) ? 0 : (row.present >> i & 1) ? image_of(c[i]) : 1;
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t there = row.x[i] == kMinusInfinity ? 1 : image_of(c[i]);
+            image[i] = i * L + lane < p.n ? there : 0;
+        }
+        if (grouped) {
+            // (every item reads a flag, those past the last expert one that nobody set)
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const uint32_t open = flags[((i * L + lane) * p.size_magic) >> 20];
+                image[i] = open ? image[i] : 0;
+            }
+        }
     }
     // candidates: everything from the (k+1)-th largest of the lanes' largest items on
     uint32_t most = image[0];
@@ -479,7 +476,7 @@ __global__ __launch_bounds__(256) void route_rows(const S* x, RouteCall p) {
 constexpr int kRowsPerWave = 16;
 template <typename S, int KIND, int ITEMS>
 __global__ __launch_bounds__(256) void route_unsettled(const S* x, RouteCall p) {
-    __shared__ double lds[4][kWave * ITEMS + kWave * ITEMS / 8];
+    __shared__ double lds[4][kWave * ITEMS * 13 / 8];          // the experts' values, the groups' (half as many), a byte per group
     __shared__ int32_t histogram[kWave * ITEMS];
     const int lane = lane_id(), wave = threadIdx.x / kWave;
     clear_loads(p, histogram);
@@ -491,7 +488,7 @@ __global__ __launch_bounds__(256) void route_unsettled(const S* x, RouteCall p) 
         RouteRow<S, KIND, kWave, ITEMS> row;
         row.load(xr, p.n, lane);
         row.normalise();
-        const int e = choose_exactly<S, KIND, kWave, ITEMS>(p, row, lds[wave], lane);
+        const int e = choose_exactly<S, KIND>(p, xr, lds[wave], lane);
         settle<S, KIND, kWave, ITEMS>(p, row, xr, e, r, true, lane, histogram);
     }
     flush_loads(p, histogram);
@@ -588,7 +585,7 @@ __global__ __launch_bounds__(256) void route_grad_rows(const S* x, S* dx, RouteG
         const int e = i * L + lane;
         if (e >= p.n) continue;
         float g = grad[i];
-        if (KIND == kSoftmaxScore && !p.renormalise && (row.present >> i & 1)) g -= dot * row.score(row.x[i]);
+        if (KIND == kSoftmaxScore && !p.renormalise) g -= dot * row.score(row.x[i]);
         dx[r * p.dx_stride + e] = static_cast<S>(g);
     }
 }
