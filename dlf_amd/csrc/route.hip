@@ -473,7 +473,7 @@ __global__ __launch_bounds__(256) void route_rows(const S* x, RouteCall p) {
 }
 
 // Rows that route_rows left marked: kRowsPerWave neighbouring rows to a wavefront.
-constexpr int kRowsPerWave = 16;
+constexpr int kRowsPerWave = 4;
 template <typename S, int KIND, int ITEMS>
 __global__ __launch_bounds__(256) void route_unsettled(const S* x, RouteCall p) {
     __shared__ double lds[4][kWave * ITEMS * 13 / 8];          // the experts' values, the groups' (half as many), a byte per group
