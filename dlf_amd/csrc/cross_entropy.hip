@@ -59,12 +59,19 @@ __device__ __forceinline__ void fold(MaxSum& s, const float (&v)[N]) {
     s.mx = mx;
 }
 
+// Over a wavefront: the maxima first, so that a lane scales its sum once.
+__device__ __forceinline__ MaxSum wave_join(MaxSum s) {
+    const float mx = wave_reduce(s.mx, [](float a, float b) { return fmaxf(a, b); });
+    if (s.mx != mx) s.sum *= exp_diff(s.mx, fminf(mx, kLargest));
+    return {mx, wave_reduce(s.sum, [](float a, float b) { return a + b; })};
+}
+
 // Over the T threads of a workgroup; every thread gets the result.  Two uses in a row need different
 // `lds` or a barrier between them.
 template <int T>
 __device__ __forceinline__ MaxSum block_join(MaxSum v, MaxSum* lds) {
     constexpr int WAVES = T / kWave;
-    v = wave_reduce(v, join);
+    v = wave_join(v);
     if (lane_id() == 0) lds[threadIdx.x / kWave] = v;
     __syncthreads();
     v = lds[lane_id() % WAVES];
@@ -294,17 +301,30 @@ __global__ __launch_bounds__(kTileThreads) void loss_tiles(LossCall<S> p) {
     MaxSum s = {kNone, 0.0f};
     for (int64_t e0 = begin + static_cast<int64_t>(threadIdx.x) * V; e0 < end; e0 += kTileBatch * tile_unit<S>()) {
         Words4 raw[kTileBatch];
+        float part[V];
+        if (e0 + (kTileBatch - 1) * tile_unit<S>() + V <= end) {
+            float v[kTileBatch * V];
 #pragma unroll
-        for (int u = 0; u < kTileBatch; ++u) {
-            const int64_t e = e0 + u * tile_unit<S>();
-            if (e < end) raw[u] = load_part(xr, e, end);
-        }
+            for (int u = 0; u < kTileBatch; ++u) raw[u] = load_words(xr + e0 + u * tile_unit<S>());
 #pragma unroll
-        for (int u = 0; u < kTileBatch; ++u) {
-            if (e0 + u * tile_unit<S>() >= end) break;
-            float v[V];
-            widen<S>(raw[u], v);
+            for (int u = 0; u < kTileBatch; ++u) {
+                widen<S>(raw[u], part);
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[u * V + i] = part[i];
+            }
             fold(s, v);
+        } else {
+#pragma unroll
+            for (int u = 0; u < kTileBatch; ++u) {
+                const int64_t e = e0 + u * tile_unit<S>();
+                if (e < end) raw[u] = load_part(xr, e, end);
+            }
+#pragma unroll
+            for (int u = 0; u < kTileBatch; ++u) {
+                if (e0 + u * tile_unit<S>() >= end) break;
+                widen<S>(raw[u], part);
+                fold(s, part);
+            }
         }
     }
     s = block_join<kTileThreads>(s, lds);
@@ -316,7 +336,7 @@ __global__ __launch_bounds__(kTileThreads) void loss_tiles(LossCall<S> p) {
 __device__ __forceinline__ MaxSum join_records(const MaxSum* records, int64_t count) {
     MaxSum s = {kNone, 0.0f};
     for (int64_t t = lane_id(); t < count; t += kWave) s = join(s, records[t]);
-    return wave_reduce(s, join);
+    return wave_join(s);
 }
 
 // One wavefront per row joins its records.

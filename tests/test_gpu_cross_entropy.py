@@ -201,7 +201,9 @@ def test_views_ranks_and_in_place(hip_backend, n, dtype):
     column = Tensor.from_numpy(hip_backend, np.ascontiguousarray(x.T)).transpose()
     loss2, g2 = F.cross_entropy_grad(column, T)
     hip_backend.synchronize()
-    assert loss.numpy().shape == (3, 4) and np.array_equal(loss.numpy().reshape(-1), loss2.numpy())
+    # the loss alone and the loss beside a gradient add up in different orders: each within the bound
+    lb = loss_bound(O.load(x), want, 0.0)
+    assert loss.numpy().shape == (3, 4) and O.close(loss.numpy().reshape(-1), want, lb, "f32") and O.close(loss2.numpy(), want, lb, "f32")
     assert O.close(g2.numpy(), grad, gb, dtype)
     one = F.cross_entropy(Tensor.from_numpy(hip_backend, x[0]), Tensor.from_numpy(hip_backend, t[:1]).view(Shape(())))
     hip_backend.synchronize()
