@@ -73,25 +73,27 @@ def build_all(force=False, jobs=None):
     return LIB
 
 
-VENEER_TEST_SRC = os.path.join(HERE, "..", "tests", "cpp", "veneer_test.cpp")
-VENEER_TEST_BIN = os.path.join(HERE, "..", "tests", "cpp", "veneer_test.bin")
+VENEER_TESTS = [os.path.join(HERE, "..", "tests", "cpp", name) for name in ("veneer_test", "sequence_test")]
 
 
 def build_veneer_test(force=False):
-    """Compiles the C++ host veneer's test program (host code + HIP runtime only)."""
-    src, out = os.path.abspath(VENEER_TEST_SRC), os.path.abspath(VENEER_TEST_BIN)
-    if not os.path.exists(src):
-        return None
+    """Compiles the C++ host veneer's test programs (host code + HIP runtime only)."""
     inc = os.path.join(HERE, "include")
-    newest = max([os.path.getmtime(src)] + [os.path.getmtime(os.path.join(inc, f)) for f in os.listdir(inc)])
-    if not force and os.path.exists(out) and os.path.getmtime(out) > newest:
-        return out
-    cmd = [_hipcc(), "-O2", "-std=c++17", "-I", inc, "-I", os.path.join(HERE, "..", "include"), src, "-o", out,
-           "-pthread", "-L", os.path.dirname(LIB), "-ldlfx", "-Wl,-rpath,$ORIGIN/../../dlf_amd/lib"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("veneer test build failed:\n" + r.stderr)
-    return out
+    header_time = max([_newest_header()] + [os.path.getmtime(os.path.join(inc, f)) for f in os.listdir(inc)])
+    outs = []
+    for stem in VENEER_TESTS:
+        src, out = os.path.abspath(stem + ".cpp"), os.path.abspath(stem + ".bin")
+        if not os.path.exists(src):
+            continue
+        outs.append(out)
+        if not force and os.path.exists(out) and os.path.getmtime(out) > max(header_time, os.path.getmtime(src)):
+            continue
+        cmd = [_hipcc(), "-O2", "-std=c++17", "-I", inc, "-I", os.path.join(HERE, "..", "include"), src, "-o", out,
+               "-pthread", "-L", os.path.dirname(LIB), "-ldlfx", "-Wl,-rpath,$ORIGIN/../../dlf_amd/lib"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("veneer test build failed:\n" + r.stderr)
+    return outs
 
 
 if __name__ == "__main__":

@@ -561,4 +561,173 @@ inline DevTensor<T> merge(const DevTensor<T>& A, const DevTensor<T>& B, int axis
     return C;
 }
 
+// ---------------------------------------------------------------- sequence-model operators
+// Not in the reference: a gated linear recurrence along an axis, routing to experts, and softmax cross
+// entropy whole or in pieces of the vocabulary (dlfx.h states their formulas).  States, weights, losses
+// are fp32.
+namespace detail {
+inline gpgpu::dnn::RowState row_state(const DevTensor<float>* S) {
+    gpgpu::dnn::RowState r;
+    if (S) {
+        r.buffer = &S->data();
+        r.offset = S->shape().offset();
+        r.strides = S->shape().strides();
+    }
+    return r;
+}
+inline std::vector<size_t> without_axis(std::vector<size_t> e, int axis) {
+    e.erase(e.begin() + axis);
+    return e;
+}
+inline void want(bool ok, const char* what) {
+    if (!ok) throw shape_error(what);
+}
+// `axis` last, from its other end when reverse
+template <typename T>
+DevTensor<T> along(const DevTensor<T>& X, int axis, bool reverse) {
+    auto v = moveaxis(X, axis, -1);
+    return reverse ? flip(v, -1) : v;
+}
+// Rows of X along its last axis at one stride: {m, n, stride}.
+template <typename T>
+std::vector<size_t> rows_of(const DevTensor<T>& X) {
+    want(X.rank() >= 1 && X.shape().is_contiguous(), "rows along the last axis of a contiguous tensor");
+    const size_t n = X.extent(-1);
+    return {X.size() / n, n, n};
+}
+}  // namespace detail
+
+// h = a h + b along `axis` (kind "gated", "gated_exp", "gated_sigmoid" or "gated_blend").  initial (null:
+// zeros) has X's extents without the axis, as `last` gets; last may be the tensor that initial points
+// to, and Y may be X or G.
+template <typename T>
+void gated_scan(const DevTensor<T>& G, const DevTensor<T>& X, DevTensor<T>& Y, DevTensor<float>& last, int axis = -1,
+                const std::string& kind = "gated", const DevTensor<float>* initial = nullptr, bool reverse = false) {
+    detail::norm_axis(static_cast<int>(X.rank()), axis);
+    const auto kept = detail::without_axis(X.shape().extents(), axis);
+    detail::want(G.shape() == X.shape(), "gated_scan: the gate's extents are not the input's");
+    detail::want(!initial || initial->shape().extents() == kept, "gated_scan: initial's extents");
+    if (&Y != &X && &Y != &G) Y.resize(X.shape());
+    if (&last != initial) last.resize(Shape(kept));
+    const auto g = detail::along(G, axis, reverse), x = detail::along(X, axis, reverse), y = detail::along(Y, axis, reverse);
+    const size_t n = X.extent(axis);
+    gpgpu::dnn::gated_scan(kind, X.size() / n, n, x.shape().extents(), G.data(), g.shape().offset(), g.shape().strides(),
+                           X.data(), x.shape().offset(), x.shape().strides(), detail::row_state(initial),
+                           Y.data(), y.shape().offset(), y.shape().strides(), detail::row_state(&last));
+}
+// Gradients of gated_scan from the Y that it wrote; X is read by "gated_blend" only, dlast null: zeros.
+template <typename T>
+void gated_scan_grad(const DevTensor<T>& G, const DevTensor<T>& X, const DevTensor<T>& Y, const DevTensor<T>& dY,
+                     DevTensor<T>& dG, DevTensor<T>& dX, DevTensor<float>& dinitial, int axis = -1, const std::string& kind = "gated",
+                     const DevTensor<float>* initial = nullptr, const DevTensor<float>* dlast = nullptr, bool reverse = false) {
+    detail::norm_axis(static_cast<int>(Y.rank()), axis);
+    const auto kept = detail::without_axis(Y.shape().extents(), axis);
+    const bool blend = kind == "gated_blend";
+    detail::want(G.shape() == Y.shape() && dY.shape() == Y.shape() && (!blend || X.shape() == Y.shape()), "gated_scan_grad: extents");
+    detail::want((!initial || initial->shape().extents() == kept) && (!dlast || dlast->shape().extents() == kept), "gated_scan_grad: the states' extents");
+    dG.resize(Y.shape());
+    dX.resize(Y.shape());
+    dinitial.resize(Shape(kept));
+    const auto g = detail::along(G, axis, reverse), y = detail::along(Y, axis, reverse), dy = detail::along(dY, axis, reverse);
+    const auto dg = detail::along(dG, axis, reverse), dx = detail::along(dX, axis, reverse);
+    const auto x = blend ? detail::along(X, axis, reverse) : y;
+    const size_t n = Y.extent(axis);
+    gpgpu::dnn::gated_scan_grad(kind, Y.size() / n, n, y.shape().extents(), G.data(), g.shape().offset(), g.shape().strides(),
+                                blend ? &X.data() : nullptr, x.shape().offset(), x.shape().strides(), detail::row_state(initial),
+                                Y.data(), y.shape().offset(), y.shape().strides(), dY.data(), dy.shape().offset(), dy.shape().strides(),
+                                detail::row_state(dlast), dG.data(), dg.shape().offset(), dg.shape().strides(),
+                                dX.data(), dx.shape().offset(), dx.shape().strides(), detail::row_state(&dinitial));
+}
+
+namespace dnn {
+using gpgpu::dnn::Routing;
+
+// The k experts of every row of logits (experts on the last axis): weights and indices, best first.
+template <typename T>
+void route(const DevTensor<T>& X, DevTensor<float>& weights, DevTensor<int32_t>& indices, const Routing& how, const std::string& score = "softmax",
+           const DevTensor<float>* bias = nullptr, DevTensor<int32_t>* loads = nullptr) {
+    const auto r = dlf::detail::rows_of(X);
+    dlf::detail::want((!bias || (bias->size() == r[1] && bias->shape().is_contiguous() && bias->shape().offset() == 0)) &&
+                      (!loads || (loads->size() == r[1] && loads->shape().is_contiguous() && loads->shape().offset() == 0)),
+                      "route: bias and loads have one element per expert");
+    auto dims = X.shape().extents();
+    dims.back() = how.k;
+    weights.resize(Shape(dims));
+    indices.resize(Shape(dims));
+    gpgpu::dnn::route(score, r[0], r[1], X.data(), X.shape().offset(), r[2], bias ? &bias->data() : nullptr, how, weights.data(), indices.data(),
+                      loads ? &loads->data() : nullptr);
+}
+template <typename T>
+void route_grad(const DevTensor<T>& X, const DevTensor<int32_t>& indices, const DevTensor<float>& dweights, DevTensor<T>& dX, const Routing& how,
+                const std::string& score = "softmax") {
+    const auto r = dlf::detail::rows_of(X);
+    auto dims = X.shape().extents();
+    dims.back() = how.k;
+    for (const Shape* s : {&indices.shape(), &dweights.shape()})
+        dlf::detail::want(s->extents() == dims && s->is_contiguous() && s->offset() == 0, "route_grad: indices and gradients of the weights");
+    if (&dX != &X) dX.resize(X.shape());
+    gpgpu::dnn::route_grad(score, r[0], r[1], X.data(), X.shape().offset(), r[2], how, indices.data(), dweights.data(),
+                           dX.data(), dX.shape().offset(), r[2]);
+}
+
+namespace detail {
+template <typename T>
+void per_row(const DevTensor<T>& V, size_t m, const char* what) {
+    dlf::detail::want(V.size() == m && V.shape().is_contiguous() && V.shape().offset() == 0, what);
+}
+template <typename T>
+Shape rows_shape(const DevTensor<T>& X) { return Shape(dlf::detail::without_axis(X.shape().extents(), static_cast<int>(X.rank()) - 1)); }
+}  // namespace detail
+
+// Softmax cross entropy of every row of logits (vocabulary on the last axis); a negative target takes its row out.
+template <typename T, typename I>
+void cross_entropy(const DevTensor<T>& X, const DevTensor<I>& targets, DevTensor<float>& loss, float z_loss = 0.0f) {
+    const auto r = dlf::detail::rows_of(X);
+    detail::per_row(targets, r[0], "cross_entropy: one target per row");
+    loss.resize(detail::rows_shape(X));
+    gpgpu::dnn::cross_entropy(r[0], r[1], X.data(), X.shape().offset(), r[2], targets.data(), z_loss, loss.data());
+}
+// ... and the gradient of the sum of weights * loss (null: ones); dX may be X.
+template <typename T, typename I>
+void cross_entropy_grad(const DevTensor<T>& X, const DevTensor<I>& targets, DevTensor<float>& loss, DevTensor<T>& dX,
+                        const DevTensor<float>* weights = nullptr, float z_loss = 0.0f) {
+    const auto r = dlf::detail::rows_of(X);
+    detail::per_row(targets, r[0], "cross_entropy_grad: one target per row");
+    if (weights) detail::per_row(*weights, r[0], "cross_entropy_grad: one weight per row");
+    loss.resize(detail::rows_shape(X));
+    if (&dX != &X) dX.resize(X.shape());
+    gpgpu::dnn::cross_entropy_grad(r[0], r[1], X.data(), X.shape().offset(), r[2], targets.data(), weights ? &weights->data() : nullptr, z_loss,
+                                   &loss.data(), dX.data(), dX.shape().offset(), r[2]);
+}
+// In pieces: columns first, first + 1, ... of the vocabulary into the rows' state (an empty tensor is
+// started anew); the losses once all have gone by; a piece's gradient from the finished state.
+template <typename T, typename I>
+void cross_entropy_piece(const DevTensor<T>& X, const DevTensor<I>& targets, size_t first, DevTensor<float>& state) {
+    const auto r = dlf::detail::rows_of(X);
+    detail::per_row(targets, r[0], "cross_entropy_piece: one target per row");
+    const bool resume = !state.empty();
+    if (resume) detail::per_row(state, 3 * r[0], "cross_entropy_piece: three values of state per row");
+    else state.resize(Shape({3, r[0]}));
+    gpgpu::dnn::cross_entropy_piece(r[0], r[1], X.data(), X.shape().offset(), r[2], targets.data(), first, resume, state.data());
+}
+template <typename I>
+void cross_entropy_join(const DevTensor<I>& targets, const DevTensor<float>& state, DevTensor<float>& loss, float z_loss = 0.0f) {
+    detail::per_row(targets, targets.size(), "cross_entropy_join: targets in row-major order");
+    detail::per_row(state, 3 * targets.size(), "cross_entropy_join: three values of state per row");
+    loss.resize(targets.shape());
+    gpgpu::dnn::cross_entropy_join(targets.size(), targets.data(), state.data(), z_loss, loss.data());
+}
+template <typename T, typename I>
+void cross_entropy_piece_grad(const DevTensor<T>& X, const DevTensor<I>& targets, size_t first, const DevTensor<float>& state, DevTensor<T>& dX,
+                              const DevTensor<float>* weights = nullptr, float z_loss = 0.0f) {
+    const auto r = dlf::detail::rows_of(X);
+    detail::per_row(targets, r[0], "cross_entropy_piece_grad: one target per row");
+    detail::per_row(state, 3 * r[0], "cross_entropy_piece_grad: three values of state per row");
+    if (weights) detail::per_row(*weights, r[0], "cross_entropy_piece_grad: one weight per row");
+    if (&dX != &X) dX.resize(X.shape());
+    gpgpu::dnn::cross_entropy_piece_grad(r[0], r[1], X.data(), X.shape().offset(), r[2], targets.data(), first, state.data(),
+                                         weights ? &weights->data() : nullptr, z_loss, dX.data(), dX.shape().offset(), r[2]);
+}
+}  // namespace dnn
+
 }  // namespace dlf

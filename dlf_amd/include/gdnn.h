@@ -16,6 +16,7 @@
 #include <complex>
 
 #include "dlfx.h"
+#include "gblas_bfloat16.h"
 #include "gblas_half.h"
 #include "gpgpu.h"
 
@@ -30,6 +31,7 @@ template <> struct dtype_of<int32_t> { static constexpr int value = DLFX_I32; };
 template <> struct dtype_of<int64_t> { static constexpr int value = DLFX_I64; };
 template <> struct dtype_of<int16_t> { static constexpr int value = DLFX_I16; };
 template <> struct dtype_of<blas::half> { static constexpr int value = DLFX_F16; };
+template <> struct dtype_of<blas::bfloat16> { static constexpr int value = DLFX_BF16; };
 template <> struct dtype_of<std::complex<float>>  { static constexpr int value = DLFX_C64; };     // float2
 template <> struct dtype_of<std::complex<double>> { static constexpr int value = DLFX_C128; };    // double2
 
@@ -403,6 +405,156 @@ inline void gather_indices(const size_t m, const size_t n, const bool row_major,
     check_status(dlfx_gather_indices(queue.stream(), m, n, row_major ? 1 : 0, static_cast<int>(d.size()), d.data(),
                                      indices.data(), indices_offset, output.data(), output_offset),
                  "gpgpu::dnn::gather_indices");
+    ev.done();
+}
+
+// ---------------------------------------------------------------- sequence-model operators
+// Not in the reference (dlfx.h: gated_scan, route, cross_entropy).  T: float, blas::half, blas::bfloat16.
+
+// One fp32 value per row of a gated_scan, as a view over the kept extents; a null buffer is no state.
+struct RowState {
+    const Buffer<float>* buffer = nullptr;
+    size_t offset = 0;
+    std::vector<size_t> strides;
+    float* data() const { return buffer ? buffer->data() : nullptr; }
+};
+
+template <typename T>
+void gated_scan(const std::string& name, const size_t m, const size_t n, const std::vector<size_t>& dims,
+                const Buffer<T>& gate_buffer, const size_t gate_offset, const std::vector<size_t>& gate_strides,
+                const Buffer<T>& x_buffer, const size_t x_offset, const std::vector<size_t>& x_strides,
+                const RowState& initial,
+                Buffer<T>& y_buffer, const size_t y_offset, const std::vector<size_t>& y_strides,
+                const RowState& last,
+                const Queue& queue = gpgpu::current::queue(), Event* event = nullptr) {
+    const int dt = detail::dtype_of<T>::value;
+    auto d = detail::signed_vec(dims), gs = detail::signed_vec(gate_strides), xs = detail::signed_vec(x_strides), ys = detail::signed_vec(y_strides);
+    auto is = detail::signed_vec(initial.strides), ls = detail::signed_vec(last.strides);
+    auto tmp = queue.context().getTemporaryBuffer<char>(dlfx_gated_scan_scratch_bytes(dt, m, n));
+    detail::EventScope ev(queue, event);
+    check_status(dlfx_gated_scan(queue.stream(), name.c_str(), dt, m, n, static_cast<int>(d.size()), d.data(),
+                                 gate_buffer.data(), gate_offset, gs.data(), x_buffer.data(), x_offset, xs.data(),
+                                 initial.data(), initial.offset, is.data(), y_buffer.data(), y_offset, ys.data(),
+                                 last.data(), last.offset, ls.data(), tmp.bytes(), tmp.byte_size()), "gpgpu::dnn::gated_scan");
+    ev.done();
+}
+
+// x_buffer is read by "gated_blend" only and may be null otherwise.
+template <typename T>
+void gated_scan_grad(const std::string& name, const size_t m, const size_t n, const std::vector<size_t>& dims,
+                     const Buffer<T>& gate_buffer, const size_t gate_offset, const std::vector<size_t>& gate_strides,
+                     const Buffer<T>* x_buffer, const size_t x_offset, const std::vector<size_t>& x_strides,
+                     const RowState& initial,
+                     const Buffer<T>& y_buffer, const size_t y_offset, const std::vector<size_t>& y_strides,
+                     const Buffer<T>& dy_buffer, const size_t dy_offset, const std::vector<size_t>& dy_strides,
+                     const RowState& dlast,
+                     Buffer<T>& dgate_buffer, const size_t dgate_offset, const std::vector<size_t>& dgate_strides,
+                     Buffer<T>& dx_buffer, const size_t dx_offset, const std::vector<size_t>& dx_strides,
+                     const RowState& dinitial,
+                     const Queue& queue = gpgpu::current::queue(), Event* event = nullptr) {
+    const int dt = detail::dtype_of<T>::value;
+    auto d = detail::signed_vec(dims), gs = detail::signed_vec(gate_strides), xs = detail::signed_vec(x_strides), ys = detail::signed_vec(y_strides);
+    auto dys = detail::signed_vec(dy_strides), dgs = detail::signed_vec(dgate_strides), dxs = detail::signed_vec(dx_strides);
+    auto is = detail::signed_vec(initial.strides), dls = detail::signed_vec(dlast.strides), dis = detail::signed_vec(dinitial.strides);
+    auto tmp = queue.context().getTemporaryBuffer<char>(dlfx_gated_scan_scratch_bytes(dt, m, n));
+    detail::EventScope ev(queue, event);
+    check_status(dlfx_gated_scan_grad(queue.stream(), name.c_str(), dt, m, n, static_cast<int>(d.size()), d.data(),
+                                      gate_buffer.data(), gate_offset, gs.data(),
+                                      x_buffer ? x_buffer->data() : nullptr, x_offset, x_buffer ? xs.data() : nullptr,
+                                      initial.data(), initial.offset, is.data(), y_buffer.data(), y_offset, ys.data(),
+                                      dy_buffer.data(), dy_offset, dys.data(), dlast.data(), dlast.offset, dls.data(),
+                                      dgate_buffer.data(), dgate_offset, dgs.data(), dx_buffer.data(), dx_offset, dxs.data(),
+                                      dinitial.data(), dinitial.offset, dis.data(), tmp.bytes(), tmp.byte_size()), "gpgpu::dnn::gated_scan_grad");
+    ev.done();
+}
+
+// How router logits choose experts; groups == kept_groups: all of them take part.
+struct Routing {
+    size_t k = 1;
+    bool renormalise = false;
+    float scale = 1.0f;
+    size_t groups = 1, kept_groups = 1;
+    int group_best = 1;
+};
+
+// weights and indices: dense [m, k]; bias (n values) and loads (n counters, added to) may be null.
+template <typename T>
+void route(const std::string& score, const size_t m, const size_t n, const Buffer<T>& x_buffer, const size_t x_offset, const size_t row_stride,
+           const Buffer<float>* bias, const Routing& how, Buffer<float>& weights, Buffer<int32_t>& indices, Buffer<int32_t>* loads = nullptr,
+           const Queue& queue = gpgpu::current::queue(), Event* event = nullptr) {
+    detail::EventScope ev(queue, event);
+    check_status(dlfx_route(queue.stream(), score.c_str(), detail::dtype_of<T>::value, m, n, x_buffer.data(), x_offset, row_stride,
+                            bias ? bias->data() : nullptr, how.groups, how.kept_groups, how.group_best, how.k, how.renormalise ? 1 : 0, how.scale,
+                            weights.data(), indices.data(), loads ? loads->data() : nullptr), "gpgpu::dnn::route");
+    ev.done();
+}
+template <typename T>
+void route_grad(const std::string& score, const size_t m, const size_t n, const Buffer<T>& x_buffer, const size_t x_offset, const size_t row_stride,
+                const Routing& how, const Buffer<int32_t>& indices, const Buffer<float>& dweights,
+                Buffer<T>& dx_buffer, const size_t dx_offset, const size_t dx_row_stride,
+                const Queue& queue = gpgpu::current::queue(), Event* event = nullptr) {
+    detail::EventScope ev(queue, event);
+    check_status(dlfx_route_grad(queue.stream(), score.c_str(), detail::dtype_of<T>::value, m, n, x_buffer.data(), x_offset, row_stride, how.k,
+                                 indices.data(), dweights.data(), how.renormalise ? 1 : 0, how.scale, dx_buffer.data(), dx_offset, dx_row_stride),
+                 "gpgpu::dnn::route_grad");
+    ev.done();
+}
+
+// targets: int32_t or int64_t, one per row; weights (one per row) and loss of the gradient may be null.
+template <typename T, typename I>
+void cross_entropy(const size_t m, const size_t n, const Buffer<T>& x_buffer, const size_t x_offset, const size_t row_stride,
+                   const Buffer<I>& targets, const float z_loss, Buffer<float>& loss,
+                   const Queue& queue = gpgpu::current::queue(), Event* event = nullptr) {
+    const int dt = detail::dtype_of<T>::value;
+    auto tmp = queue.context().getTemporaryBuffer<char>(dlfx_cross_entropy_scratch_bytes(dt, m, n));
+    detail::EventScope ev(queue, event);
+    check_status(dlfx_cross_entropy(queue.stream(), dt, detail::dtype_of<I>::value, m, n, x_buffer.data(), x_offset, row_stride, targets.data(),
+                                    z_loss, loss.data(), tmp.bytes(), tmp.byte_size()), "gpgpu::dnn::cross_entropy");
+    ev.done();
+}
+template <typename T, typename I>
+void cross_entropy_grad(const size_t m, const size_t n, const Buffer<T>& x_buffer, const size_t x_offset, const size_t row_stride,
+                        const Buffer<I>& targets, const Buffer<float>* weights, const float z_loss, Buffer<float>* loss,
+                        Buffer<T>& dx_buffer, const size_t dx_offset, const size_t dx_row_stride,
+                        const Queue& queue = gpgpu::current::queue(), Event* event = nullptr) {
+    const int dt = detail::dtype_of<T>::value;
+    auto tmp = queue.context().getTemporaryBuffer<char>(dlfx_cross_entropy_scratch_bytes(dt, m, n));
+    detail::EventScope ev(queue, event);
+    check_status(dlfx_cross_entropy_grad(queue.stream(), dt, detail::dtype_of<I>::value, m, n, x_buffer.data(), x_offset, row_stride, targets.data(),
+                                         weights ? weights->data() : nullptr, z_loss, loss ? loss->data() : nullptr,
+                                         dx_buffer.data(), dx_offset, dx_row_stride, tmp.bytes(), tmp.byte_size()), "gpgpu::dnn::cross_entropy_grad");
+    ev.done();
+}
+// state: 3 m values; resume == false starts it anew.
+template <typename T, typename I>
+void cross_entropy_piece(const size_t m, const size_t n, const Buffer<T>& x_buffer, const size_t x_offset, const size_t row_stride,
+                         const Buffer<I>& targets, const size_t first, const bool resume, Buffer<float>& state,
+                         const Queue& queue = gpgpu::current::queue(), Event* event = nullptr) {
+    const int dt = detail::dtype_of<T>::value;
+    auto tmp = queue.context().getTemporaryBuffer<char>(dlfx_cross_entropy_scratch_bytes(dt, m, n));
+    detail::EventScope ev(queue, event);
+    check_status(dlfx_cross_entropy_piece(queue.stream(), dt, detail::dtype_of<I>::value, m, n, x_buffer.data(), x_offset, row_stride, targets.data(),
+                                          first, resume ? 1 : 0, state.data(), tmp.bytes(), tmp.byte_size()), "gpgpu::dnn::cross_entropy_piece");
+    ev.done();
+}
+template <typename I>
+void cross_entropy_join(const size_t m, const Buffer<I>& targets, const Buffer<float>& state, const float z_loss, Buffer<float>& loss,
+                        const Queue& queue = gpgpu::current::queue(), Event* event = nullptr) {
+    detail::EventScope ev(queue, event);
+    check_status(dlfx_cross_entropy_join(queue.stream(), detail::dtype_of<I>::value, m, targets.data(), state.data(), z_loss, loss.data()),
+                 "gpgpu::dnn::cross_entropy_join");
+    ev.done();
+}
+template <typename T, typename I>
+void cross_entropy_piece_grad(const size_t m, const size_t n, const Buffer<T>& x_buffer, const size_t x_offset, const size_t row_stride,
+                              const Buffer<I>& targets, const size_t first, const Buffer<float>& state, const Buffer<float>* weights, const float z_loss,
+                              Buffer<T>& dx_buffer, const size_t dx_offset, const size_t dx_row_stride,
+                              const Queue& queue = gpgpu::current::queue(), Event* event = nullptr) {
+    detail::EventScope ev(queue, event);
+    check_status(dlfx_cross_entropy_piece_grad(queue.stream(), detail::dtype_of<T>::value, detail::dtype_of<I>::value, m, n,
+                                               x_buffer.data(), x_offset, row_stride, targets.data(), first, state.data(),
+                                               weights ? weights->data() : nullptr, z_loss, dx_buffer.data(), dx_offset, dx_row_stride),
+                 "gpgpu::dnn::cross_entropy_piece_grad");
     ev.done();
 }
 
