@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256) void grad_rows_tiny(const S* x, int64_t m, int
         if (i < n) dx[r * dx_stride + i] = static_cast<S>(g.zero ? 0.0f : g.p * exp_diff(v[i], g.mx) - (i == target ? g.up : 0.0f));
 }
 
-// A row cut into tiles, a workgroup each: blockIdx = row * tiles + tile.
+// A row cut into tiles, a workgroup each: workgroup = row * tiles + tile.
 constexpr int kTileThreads = 256;
 constexpr int kTileBatch = 4;                       // vectors of a thread in flight
 template <typename S> constexpr int64_t tile_unit() { return static_cast<int64_t>(kTileThreads) * vector_width<S>(); }
@@ -254,6 +254,14 @@ template <typename S> constexpr int64_t tile_unit() { return static_cast<int64_t
 struct Tiles {
     int64_t count, length;
 };
+
+// Workgroups of a pass over tiles in rows of 2^20: along one axis of the grid there can be 2^24.
+constexpr uint32_t kGridRow = 1u << 20;
+inline dim3 grid_of(int64_t workgroups) {
+    if (workgroups <= kGridRow) return dim3(static_cast<unsigned>(workgroups));
+    return dim3(kGridRow, static_cast<unsigned>(ceil_div(workgroups, kGridRow)));
+}
+__device__ __forceinline__ uint32_t workgroup() { return blockIdx.y * kGridRow + blockIdx.x; }
 
 // What a call on a matrix of logits works on; state or loss is where a finished row goes.
 template <typename S>
@@ -294,7 +302,9 @@ __global__ __launch_bounds__(kTileThreads) void loss_tiles(LossCall<S> p) {
     constexpr int V = vector_width<S>();
     __shared__ MaxSum lds[kTileThreads / kWave];
     const uint32_t tiles = static_cast<uint32_t>(p.tiles.count);
-    const int64_t r = blockIdx.x / tiles, tile = blockIdx.x % tiles;
+    const uint32_t here = workgroup();
+    const int64_t r = here / tiles, tile = here % tiles;
+    if (r >= p.m) return;
     const S* xr = p.x + r * p.stride;
     const int64_t begin = tile * p.tiles.length;
     const int64_t end = begin + p.tiles.length < p.n ? begin + p.tiles.length : p.n;
@@ -329,7 +339,7 @@ __global__ __launch_bounds__(kTileThreads) void loss_tiles(LossCall<S> p) {
     }
     s = block_join<kTileThreads>(s, lds);
     if (threadIdx.x) return;
-    if (p.tiles.count > 1 || !(p.loss || p.state)) p.records[blockIdx.x] = s;
+    if (p.tiles.count > 1 || !(p.loss || p.state)) p.records[here] = s;
     else finish_row(p, r, s);
 }
 
@@ -359,7 +369,9 @@ template <typename S>
 __global__ __launch_bounds__(kTileThreads) void grad_tiles(LossCall<S> p, int64_t record_count, const float* weights, S* dx, int64_t dx_stride) {
     constexpr int V = vector_width<S>();
     const uint32_t tiles = static_cast<uint32_t>(p.tiles.count);
-    const int64_t r = blockIdx.x / tiles, tile = blockIdx.x % tiles;
+    const uint32_t here = workgroup();
+    const int64_t r = here / tiles, tile = here % tiles;
+    if (r >= p.m) return;
     const S* xr = p.x + r * p.stride;
     S* dr = dx + r * dx_stride;
     const int64_t begin = tile * p.tiles.length;
@@ -370,7 +382,7 @@ __global__ __launch_bounds__(kTileThreads) void grad_tiles(LossCall<S> p, int64_
     if (p.state) s = {p.state[r], p.state[p.m + r]};
     else s = join_records(p.records + r * record_count, record_count);
     const RowGrad g = row_grad(s, target >= 0, weight, p.z);
-    const int64_t here = target < 0 ? -1 : target - p.first;
+    const int64_t column = target < 0 ? -1 : target - p.first;
     for (int64_t e0 = begin + static_cast<int64_t>(threadIdx.x) * V; e0 < end; e0 += kTileBatch * tile_unit<S>()) {
         Words4 raw[kTileBatch];
 #pragma unroll
@@ -381,7 +393,7 @@ __global__ __launch_bounds__(kTileThreads) void grad_tiles(LossCall<S> p, int64_
 #pragma unroll
         for (int u = 0; u < kTileBatch; ++u) {
             const int64_t e = e0 + u * tile_unit<S>();
-            if (e < end) store_part(dr, e, end, grad_vector<S>(e, raw[u], g, here));
+            if (e < end) store_part(dr, e, end, grad_vector<S>(e, raw[u], g, column));
         }
     }
 }
@@ -442,7 +454,7 @@ int launch_loss(LossCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t 
     if (p.tiles.count > 1 && (!scratch || scratch_bytes < scratch_of<S>(p.m, p.n))) p.tiles = {1, p.n};
     if (p.m * p.tiles.count > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
     p.records = static_cast<MaxSum*>(scratch);
-    loss_tiles<S><<<dim3(static_cast<unsigned>(p.m * p.tiles.count)), dim3(kTileThreads), 0, stream>>>(p);
+    loss_tiles<S><<<grid_of(p.m * p.tiles.count), dim3(kTileThreads), 0, stream>>>(p);
     DLFX_CHECK_LAUNCH();
     if (p.tiles.count > 1) {
         loss_join_tiles<S><<<dim3(static_cast<unsigned>(ceil_div(p.m, 4))), dim3(256), 0, stream>>>(p);
@@ -455,7 +467,7 @@ template <typename S>
 int launch_grad_tiles(LossCall<S> p, int64_t record_count, const float* weights, S* dx, int64_t dx_stride, hipStream_t stream) {
     p.tiles = writing_tiles<S>(p.n);
     if (p.m * p.tiles.count > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
-    grad_tiles<S><<<dim3(static_cast<unsigned>(p.m * p.tiles.count)), dim3(kTileThreads), 0, stream>>>(p, record_count, weights, dx, dx_stride);
+    grad_tiles<S><<<grid_of(p.m * p.tiles.count), dim3(kTileThreads), 0, stream>>>(p, record_count, weights, dx, dx_stride);
     DLFX_CHECK_LAUNCH();
     return DLFX_OK;
 }
@@ -504,7 +516,7 @@ int launch_grad(LossCall<S> p, const float* weights, S* dx, int64_t dx_stride, v
     q.records = static_cast<MaxSum*>(scratch);
     float* loss = q.loss;
     q.loss = nullptr;
-    loss_tiles<S><<<dim3(static_cast<unsigned>(p.m * q.tiles.count)), dim3(kTileThreads), 0, stream>>>(q);
+    loss_tiles<S><<<grid_of(p.m * q.tiles.count), dim3(kTileThreads), 0, stream>>>(q);
     DLFX_CHECK_LAUNCH();
     if (loss) {
         q.loss = loss;
@@ -549,7 +561,7 @@ extern "C" int dlfx_cross_entropy_grad(dlfx_stream_t stream, int dtype, int inde
                                        void* dx, int64_t dx_offset, int64_t dx_row_stride,
                                        void* scratch, size_t scratch_bytes) {
     if (int e = check(m, n, x, row_stride, targets)) return e;
-    if (!dx || dx_row_stride < n) return DLFX_ERR_INVALID_ARGUMENT;
+    if (!dx || dx_row_stride < n || (x_offset == dx_offset && overwrites(x, row_stride, dx, dx_row_stride, m))) return DLFX_ERR_INVALID_ARGUMENT;
     if (!index_ok(index_dtype)) return DLFX_ERR_UNSUPPORTED_DTYPE;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     return dispatch_sequence_dtype(dtype, [&](auto tag) {
@@ -590,6 +602,7 @@ extern "C" int dlfx_cross_entropy_piece_grad(dlfx_stream_t stream, int dtype, in
                                              void* dx, int64_t dx_offset, int64_t dx_row_stride) {
     if (int e = check(m, n, x, row_stride, targets)) return e;
     if (!state || first < 0 || !dx || dx_row_stride < n) return DLFX_ERR_INVALID_ARGUMENT;
+    if (x_offset == dx_offset && overwrites(x, row_stride, dx, dx_row_stride, m)) return DLFX_ERR_INVALID_ARGUMENT;
     if (!index_ok(index_dtype)) return DLFX_ERR_UNSUPPORTED_DTYPE;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     return dispatch_sequence_dtype(dtype, [&](auto tag) {

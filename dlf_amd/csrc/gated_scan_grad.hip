@@ -250,7 +250,7 @@ int launch_cols(GradCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t 
     if (segments > 1 && (!scratch || scratch_bytes < records_bytes(p.cut.m, segments))) return DLFX_ERR_SCRATCH_TOO_SMALL;
     p.cut.length = align_up(ceil_div(p.cut.n, segments), W * kGradSteps);
     segments = p.cut.segments = ceil_div(p.cut.n, p.cut.length);
-    if (p.cut.blocks * segments > 0x7ffffff0LL) return DLFX_ERR_TOO_LARGE;
+    if (grid_of(p.cut.blocks * segments) > kMostThreads / (W * kWave)) return DLFX_ERR_TOO_LARGE;
     if (segments > 1) {
         p.records = static_cast<Stretch*>(scratch);
         p.entering = reinterpret_cast<float*>(static_cast<char*>(scratch) + align_up(static_cast<size_t>(p.cut.m * (segments - 1)) * sizeof(Stretch), 256));
@@ -419,7 +419,7 @@ int launch_rows(GradCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t 
     if (segments > 1 && (!scratch || scratch_bytes < records_bytes(p.cut.m, segments))) return DLFX_ERR_SCRATCH_TOO_SMALL;
     p.cut.length = align_up(ceil_div(p.cut.n, segments), PASS);
     segments = p.cut.segments = ceil_div(p.cut.n, p.cut.length);
-    if (p.cut.blocks * segments > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
+    if (p.cut.blocks * segments > kMostThreads / BLOCK) return DLFX_ERR_TOO_LARGE;
     if constexpr (W > 4) {
         if (segments > 1) {
             p.records = static_cast<Stretch*>(scratch);
@@ -447,7 +447,7 @@ template <typename S, int KIND>
 int launch_grad(const GradCall<S>& p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     const int64_t m = p.cut.m, n = p.cut.n;
     if (n <= 2 * kGradSteps) {
-        if (ceil_div(m, 256) > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
+        if (ceil_div(m, 256) > kMostThreads / 256) return DLFX_ERR_TOO_LARGE;
         gated_grad_walk<S, KIND><<<dim3(static_cast<unsigned>(ceil_div(m, 256))), dim3(256), 0, stream>>>(p);
         DLFX_CHECK_LAUNCH();
         return DLFX_OK;

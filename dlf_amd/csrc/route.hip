@@ -609,7 +609,7 @@ int check(const char* name, int64_t m, int64_t n, int64_t k, const void* x, int6
     if (!std::strcmp(name, "softmax")) *kind = kSoftmaxScore;
     else if (!std::strcmp(name, "sigmoid")) *kind = kSigmoidScore;
     else return DLFX_ERR_UNKNOWN_OP;
-    if (n > DLFX_ROUTE_MAX_N || k > DLFX_ROUTE_MAX_K || ceil_div(m, 4) > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
+    if (n > DLFX_ROUTE_MAX_N || k > DLFX_ROUTE_MAX_K || ceil_div(m, 4) > kMostThreads / 256) return DLFX_ERR_TOO_LARGE;
     return DLFX_OK;
 }
 
@@ -665,6 +665,7 @@ extern "C" int dlfx_route_grad(dlfx_stream_t stream, const char* name, int dtype
     int kind;
     if (int e = check(name, m, n, k, x, row_stride, &kind)) return e;
     if (!indices || !dweights || !dx || dx_row_stride < n) return DLFX_ERR_INVALID_ARGUMENT;
+    if (x_offset == dx_offset && overwrites(x, row_stride, dx, dx_row_stride, m)) return DLFX_ERR_INVALID_ARGUMENT;
     RouteGradCall p{m, row_stride, dx_row_stride, static_cast<int>(n), static_cast<int>(k), renormalise, scale, indices, dweights};
     return dispatch_sequence_dtype(dtype, [&](auto tag) {
         using S = decltype(tag);

@@ -277,6 +277,8 @@ class HipBackend:
         """A Tensor over the memory of a torch tensor of this backend's device (no copy; any strides)."""
         if tensor.device != self.device:
             raise ValueError("the tensor is on %s, this backend on %s" % (tensor.device, self.device))
+        if tensor.is_conj() or tensor.is_neg():
+            raise ValueError("a view that torch conjugates or negates when it is read: resolve it first")
         if tensor.requires_grad:
             tensor = tensor.detach()
         extents, strides = tuple(tensor.shape), tensor.stride()

@@ -339,7 +339,9 @@ int dlfx_fill(dlfx_stream_t stream, int dtype, int rank, const int64_t* dims, co
  * a stride of 0 on the gate's side shares a gate between elements.  initial and last hold one fp32
  * value per row: views over the kept dims, rank - 1 strides each, either may be NULL.  A gate that
  * makes the factor 0 (g = 0, or -inf) starts a new sequence at that step; the arithmetic is the
- * formula's, so a state that is already infinite or NaN is not forgotten by it.
+ * formula's, so a state that is already infinite or NaN is not forgotten by it.  The factors of up
+ * to 16 neighbouring steps are multiplied in fp32 before they meet the state: growth by more than
+ * 2^8 a step that lasts can turn a state of 0 into NaN there, decay below 2^-126 in one go is 0.
  * y may be x or gate (the same pointer, offset and strides), last may be initial: with n == 1 that
  * is the step of a decoding loop, the state updated in place.  Outputs with a stride of 0 on an
  * extent above 1 are refused.  The result depends on neither the stream nor the device's load: how
@@ -402,8 +404,8 @@ int dlfx_gated_scan_grad(dlfx_stream_t stream, const char* name, int dtype, int6
  *
  * dlfx_route_grad writes the gradient of the logits [m, n] for the gradient dweights [m, k] of the
  * weights, at the choice `indices` (what dlfx_route wrote; a repeated index counts as often as it
- * stands there, one outside 0 .. n-1 is ignored); dx may be x.
- * n <= DLFX_ROUTE_MAX_N, k <= DLFX_ROUTE_MAX_K, otherwise DLFX_ERR_TOO_LARGE.
+ * stands there, one outside 0 .. n-1 is ignored); dx may be x (same offset and stride).
+ * n <= DLFX_ROUTE_MAX_N, k <= DLFX_ROUTE_MAX_K, m <= 2^26 - 4, otherwise DLFX_ERR_TOO_LARGE.
  */
 #define DLFX_ROUTE_MAX_N 1024
 #define DLFX_ROUTE_MAX_K 64
@@ -428,7 +430,7 @@ int dlfx_route_grad(dlfx_stream_t stream, const char* name, int dtype, int64_t m
  * column is a mistake that shows: loss NaN, a gradient without the target's term.  weights: m fp32
  * values or NULL (1 for every row).  -inf masks a column (gradient 0); a row whose every logit is
  * -inf has loss +inf and gradient 0.  loss: m fp32 values (dlfx_cross_entropy_grad: or NULL).
- * dx may be x (same offset and stride).
+ * dx may be x (same offset and stride; another stride from the same start is refused).
  *
  * A vocabulary too large to keep its logits goes by in pieces of columns, each with its own call
  * as soon as it has been computed; first is the column of the whole that a piece's first column is:
