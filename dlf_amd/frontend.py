@@ -407,8 +407,9 @@ def _along(T: Tensor, axis: int, reverse: bool):
 
 
 def _new(like: Tensor, extents: tuple, dtype) -> Tensor:
-    shape = Shape.dense(extents)
-    return Tensor(like.backend, shape, like.backend.alloc(dtype, shape.size), dtype)
+    if extents and min(extents) <= 0:
+        raise ShapeError("extent must be positive")
+    return like.backend.new(extents, dtype)
 
 
 def gated_scan(G: Tensor, X: Tensor, axis: int = -1, kind: str = "gated", reverse: bool = False,
