@@ -249,7 +249,7 @@ __global__ __launch_bounds__(256) void grad_rows_tiny(const S* x, int64_t m, int
 // A row cut into tiles, a workgroup each: workgroup = row * tiles + tile.
 constexpr int kTileThreads = 256;
 constexpr int kTileBatch = 4;                       // vectors of a thread in flight
-template <typename S> constexpr int64_t tile_unit() { return static_cast<int64_t>(kTileThreads) * vector_width<S>(); }
+template <typename S, int T = kTileThreads> constexpr int64_t tile_unit() { return static_cast<int64_t>(T) * vector_width<S>(); }
 
 struct Tiles {
     int64_t count, length;
@@ -297,10 +297,10 @@ __device__ __forceinline__ void finish_row(const LossCall<S>& p, int64_t r, MaxS
 }
 
 // A tile's record, or with one tile to a row the row's result.
-template <typename S>
-__global__ __launch_bounds__(kTileThreads) void loss_tiles(LossCall<S> p) {
+template <typename S, int T>
+__global__ __launch_bounds__(T) void loss_tiles(LossCall<S> p) {
     constexpr int V = vector_width<S>();
-    __shared__ MaxSum lds[kTileThreads / kWave];
+    __shared__ MaxSum lds[T / kWave];
     const uint32_t tiles = static_cast<uint32_t>(p.tiles.count);
     const uint32_t here = workgroup();
     const int64_t r = here / tiles, tile = here % tiles;
@@ -309,13 +309,13 @@ __global__ __launch_bounds__(kTileThreads) void loss_tiles(LossCall<S> p) {
     const int64_t begin = tile * p.tiles.length;
     const int64_t end = begin + p.tiles.length < p.n ? begin + p.tiles.length : p.n;
     MaxSum s = {kNone, 0.0f};
-    for (int64_t e0 = begin + static_cast<int64_t>(threadIdx.x) * V; e0 < end; e0 += kTileBatch * tile_unit<S>()) {
+    for (int64_t e0 = begin + static_cast<int64_t>(threadIdx.x) * V; e0 < end; e0 += kTileBatch * tile_unit<S, T>()) {
         Words4 raw[kTileBatch];
         float part[V];
-        if (e0 + (kTileBatch - 1) * tile_unit<S>() + V <= end) {
+        if (e0 + (kTileBatch - 1) * tile_unit<S, T>() + V <= end) {
             float v[kTileBatch * V];
 #pragma unroll
-            for (int u = 0; u < kTileBatch; ++u) raw[u] = load_words(xr + e0 + u * tile_unit<S>());
+            for (int u = 0; u < kTileBatch; ++u) raw[u] = load_words(xr + e0 + u * tile_unit<S, T>());
 #pragma unroll
             for (int u = 0; u < kTileBatch; ++u) {
                 widen<S>(raw[u], part);
@@ -326,18 +326,18 @@ __global__ __launch_bounds__(kTileThreads) void loss_tiles(LossCall<S> p) {
         } else {
 #pragma unroll
             for (int u = 0; u < kTileBatch; ++u) {
-                const int64_t e = e0 + u * tile_unit<S>();
+                const int64_t e = e0 + u * tile_unit<S, T>();
                 if (e < end) raw[u] = load_part(xr, e, end);
             }
 #pragma unroll
             for (int u = 0; u < kTileBatch; ++u) {
-                if (e0 + u * tile_unit<S>() >= end) break;
+                if (e0 + u * tile_unit<S, T>() >= end) break;
                 widen<S>(raw[u], part);
                 fold(s, part);
             }
         }
     }
-    s = block_join<kTileThreads>(s, lds);
+    s = block_join<T>(s, lds);
     if (threadIdx.x) return;
     if (p.tiles.count > 1 || !(p.loss || p.state)) p.records[here] = s;
     else finish_row(p, r, s);
@@ -364,7 +364,8 @@ __global__ __launch_bounds__(256) void loss_join(int64_t m, Targets targets, con
     loss[r] = targets[r] < 0 ? 0.0f : loss_of({state[r], state[m + r]}, state[2 * m + r], z);
 }
 
-// Gradient of a tile: the row's maximum and sum come from the state or from the records.
+// Gradient of a tile: the row's maximum and sum come from the state or from the records.  The loss, where
+// it is asked for, is left by the tile that holds the target's logit (dx may be x: nobody else may read it).
 template <typename S>
 __global__ __launch_bounds__(kTileThreads) void grad_tiles(LossCall<S> p, int64_t record_count, const float* weights, S* dx, int64_t dx_stride) {
     constexpr int V = vector_width<S>();
@@ -383,6 +384,15 @@ __global__ __launch_bounds__(kTileThreads) void grad_tiles(LossCall<S> p, int64_
     else s = join_records(p.records + r * record_count, record_count);
     const RowGrad g = row_grad(s, target >= 0, weight, p.z);
     const int64_t column = target < 0 ? -1 : target - p.first;
+    if (p.loss) {
+        const bool inside = column >= 0 && column < p.n;
+        const bool mine = inside ? column >= begin && column < end : tile == 0;
+        if (threadIdx.x == 0 && mine) {
+            const float logit = inside ? static_cast<float>(xr[column]) : std::numeric_limits<float>::quiet_NaN();
+            p.loss[r] = target < 0 ? 0.0f : loss_of(s, logit, p.z);
+        }
+        if (inside && mine) __syncthreads();
+    }
     for (int64_t e0 = begin + static_cast<int64_t>(threadIdx.x) * V; e0 < end; e0 += kTileBatch * tile_unit<S>()) {
         Words4 raw[kTileBatch];
 #pragma unroll
@@ -454,7 +464,18 @@ int launch_loss(LossCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t 
     if (p.tiles.count > 1 && (!scratch || scratch_bytes < scratch_of<S>(p.m, p.n))) p.tiles = {1, p.n};
     if (p.m * p.tiles.count > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
     p.records = static_cast<MaxSum*>(scratch);
-    loss_tiles<S><<<grid_of(p.m * p.tiles.count), dim3(kTileThreads), 0, stream>>>(p);
+    if (p.m <= 512 && p.n * sizeof(S) <= 256 * 1024) {
+        // few rows of middling length: sixteen wavefronts to a row spare the launch that joins tiles.  Calls in a
+        // row, us, tiles and rows: [64, 32768] fp32 14.1 / 11.2, [512, 32768] 18.1 / 16.4, [256, 65536] 18.0 / 14.2;
+        // beyond, [1023, 32768] 25.9 / 29.4 and [64, 131072] 14.1 / 18.5
+        p.tiles = {1, p.n};
+        if (p.n > kTileBatch * tile_unit<S>()) {
+            loss_tiles<S, 1024><<<grid_of(p.m), dim3(1024), 0, stream>>>(p);
+            DLFX_CHECK_LAUNCH();
+            return DLFX_OK;
+        }
+    }
+    loss_tiles<S, kTileThreads><<<grid_of(p.m * p.tiles.count), dim3(kTileThreads), 0, stream>>>(p);
     DLFX_CHECK_LAUNCH();
     if (p.tiles.count > 1) {
         loss_join_tiles<S><<<dim3(static_cast<unsigned>(ceil_div(p.m, 4))), dim3(256), 0, stream>>>(p);
@@ -508,21 +529,16 @@ int launch_grad(LossCall<S> p, const float* weights, S* dx, int64_t dx_stride, v
         return status;
     }
     if (!has_scratch) return DLFX_ERR_SCRATCH_TOO_SMALL;
-    // the records first, then the losses (the target's logit is read before dx, which may be x, is
-    // written), then the gradients tile by tile
+    // the records first, then the gradients and the loss tile by tile
     LossCall<S> q = p;
     q.tiles = joining_tiles<S>(p.m, p.n);
     if (p.m * q.tiles.count > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
     q.records = static_cast<MaxSum*>(scratch);
     float* loss = q.loss;
-    q.loss = nullptr;
-    loss_tiles<S><<<grid_of(p.m * q.tiles.count), dim3(kTileThreads), 0, stream>>>(q);
+    q.loss = nullptr;                       // (records)
+    loss_tiles<S, kTileThreads><<<grid_of(p.m * q.tiles.count), dim3(kTileThreads), 0, stream>>>(q);
     DLFX_CHECK_LAUNCH();
-    if (loss) {
-        q.loss = loss;
-        loss_join_tiles<S><<<dim3(static_cast<unsigned>(ceil_div(p.m, 4))), dim3(256), 0, stream>>>(q);
-        DLFX_CHECK_LAUNCH();
-    }
+    q.loss = loss;
     return launch_grad_tiles(q, q.tiles.count, weights, dx, dx_stride, stream);
 }
 
