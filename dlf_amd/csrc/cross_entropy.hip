@@ -437,9 +437,17 @@ Tiles writing_tiles(int64_t n) {
 // Longest row that a workgroup's registers hold.
 template <typename S> constexpr int64_t held_most() { return 16 * 1024 * vector_width<S>(); }
 
+// Few rows of middling length are a workgroup's of sixteen wavefronts each, which spares the launch that joins
+// tiles.  Calls in a row, us, tiles and rows: the loss of [64, 32768] fp32 14.1 / 11.2, [512, 32768] 18.1 / 16.4,
+// [256, 65536] 18.0 / 14.2, beyond [1023, 32768] 25.9 / 29.4 and [64, 131072] 14.1 / 18.5; the loss with its
+// gradient, [1 to 190, 32768] fp32 19.2 / 16.0, beyond [64, 65536] 18.6 / 21.6 (from about 190 rows on both fill
+// the device: [190, 65536] 32.0 / 31.2).
+constexpr int64_t kFewRows = 512, kLossBytes = 256 * 1024, kGradBytes = 128 * 1024, kHeldRows = 192;
+
 // Records of the tiles; calls that make none ask for nothing.
 template <typename S>
 size_t scratch_of(int64_t m, int64_t n) {
+    if (m <= kFewRows && n * static_cast<int64_t>(sizeof(S)) <= kGradBytes) return 0;
     const int64_t count = joining_tiles<S>(m, n).count;
     return count > 1 || n > held_most<S>() ? static_cast<size_t>(m * count) * sizeof(MaxSum) : 0;
 }
@@ -464,10 +472,7 @@ int launch_loss(LossCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t 
     if (p.tiles.count > 1 && (!scratch || scratch_bytes < scratch_of<S>(p.m, p.n))) p.tiles = {1, p.n};
     if (p.m * p.tiles.count > 0x7fffffffLL) return DLFX_ERR_TOO_LARGE;
     p.records = static_cast<MaxSum*>(scratch);
-    if (p.m <= 512 && p.n * sizeof(S) <= 256 * 1024) {
-        // few rows of middling length: sixteen wavefronts to a row spare the launch that joins tiles.  Calls in a
-        // row, us, tiles and rows: [64, 32768] fp32 14.1 / 11.2, [512, 32768] 18.1 / 16.4, [256, 65536] 18.0 / 14.2;
-        // beyond, [1023, 32768] 25.9 / 29.4 and [64, 131072] 14.1 / 18.5
+    if (p.m <= kFewRows && p.n * static_cast<int64_t>(sizeof(S)) <= kLossBytes) {
         p.tiles = {1, p.n};
         if (p.n > kTileBatch * tile_unit<S>()) {
             loss_tiles<S, 1024><<<grid_of(p.m), dim3(1024), 0, stream>>>(p);
@@ -519,7 +524,7 @@ int launch_grad(LossCall<S> p, const float* weights, S* dx, int64_t dx_stride, v
     if (p.n <= 512 * V) return held(integral_constant<int, 2>(), integral_constant<int, 256>());
     if (p.n <= 768 * V) return held(integral_constant<int, 3>(), integral_constant<int, 256>());
     if (p.n <= 1024 * V) return held(integral_constant<int, 4>(), integral_constant<int, 256>());
-    if (p.n <= held_most<S>() && (p.m >= 192 || !has_scratch)) {
+    if (p.n <= held_most<S>() && (p.n * static_cast<int64_t>(sizeof(S)) <= kGradBytes || p.m >= kHeldRows || !has_scratch)) {
         int status = DLFX_OK;
         const int64_t vectors = ceil_div(p.n, 1024 * V);
         auto one = [&](auto c) {
