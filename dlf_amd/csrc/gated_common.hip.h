@@ -105,6 +105,10 @@ struct Cut {
 constexpr int64_t kBlocksWanted = 512;
 constexpr int kColumnSegments = 64, kRowSegments = 512;      // the most
 
+// Columns in pairs are many and short axes are walked in one pass: only the others are cut.
+template <int V, int W>
+constexpr bool cut_columns() { return V == 1 && W == 16; }
+
 // Workgroups go round the eight XCDs in turn, each with a cache of its own: neighbouring pieces of work
 // (groups of rows that share cache lines where a row of columns is no whole number of them) go to one
 // XCD side by side.  The grid is rounded up to a multiple of 8.
@@ -192,6 +196,28 @@ __device__ __forceinline__ float enter_segment(const Stretch* records, int64_t m
     Stretch before, all;
     join_lanes<kWave>(mine, before, all);
     return through(all, state);
+}
+
+// The same for columns, by a workgroup of W wavefronts: each reads its share of the column's records at
+// once and joins them, the shares meet in LDS.  (One record after the other, by every wavefront:
+// WALKED.)
+template <int W>
+__device__ __forceinline__ float enter_column(const Stretch* records, int64_t m, int64_t r, int64_t count, float state, Stretch (*lds)[kWave]) {
+    constexpr int PER = kColumnSegments / W;
+    const int wave = threadIdx.x / kWave, lane = lane_id();
+    Stretch got[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        got[i] = {1.0, 0.0f};
+        if (wave * PER + i < count) got[i] = records[(wave * PER + i) * m + r];
+    }
+#pragma unroll
+    for (int i = 1; i < PER; ++i) got[0] = join(got[0], got[i]);
+    lds[wave][lane] = got[0];
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) state = through(lds[w][lane], state);
+    return state;
 }
 
 // +1 or -1 when a track's steps lie one element apart in memory, 0 otherwise.

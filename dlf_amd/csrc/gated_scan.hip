@@ -78,8 +78,10 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
                 carry[v] = h;
             }
         } else if (!PARTIAL) {
-            carry[v] = p.entering[r + v];
-            for (int64_t s = 0; s < segment; ++s) carry[v] = through(p.records[s * p.cut.m + r + v], carry[v]);
+            if constexpr (cut_columns<V, W>()) {
+                __shared__ Stretch shares[W][kWave];
+                carry[v] = enter_column<W>(p.records, p.cut.m, r, segment, p.entering[r], shares);
+            }
         }
     }
 
@@ -149,10 +151,7 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
 
     const int64_t passes = (end - begin) / (W * N);
     int64_t t0 = begin + wave * N;
-    if (passes > 0) fetch(t0);
-    for (int64_t pass = 0; pass < passes; ++pass, t0 += W * N) {
-        widen();
-        fetch(pass + 1 < passes ? t0 + W * N : t0);       // (after the last whole pass: values that nobody uses)
+    auto walk = [&] {
         float h[V];
         enter(h);
         if constexpr (!PARTIAL) {
@@ -161,6 +160,17 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
 #pragma unroll
             for (int i = 0; i < N; ++i, yp += p.y.step) store_at<NT, S, V>(yp, yi, state(i, h));
         }
+        t0 += W * N;
+    };
+    if (passes > 0) {
+        fetch(t0);
+        for (int64_t pass = 1; pass < passes; ++pass) {
+            widen();
+            fetch(t0 + W * N);
+            walk();
+        }
+        widen();
+        walk();
     }
     if (begin + passes * (W * N) < end) {
         const S* gp = p.g.base + t0 * p.g.step;
@@ -198,16 +208,18 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
 template <typename S, int KIND, int V, int W, typename OFF, bool NT>
 int launch_cols(ScanCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     p.cut.blocks = ceil_div(p.cut.m, kWave * V);
-    int64_t segments = segments_of(p.cut.blocks, p.cut.n, W * kSteps, 192, kColumnSegments);
+    int64_t segments = cut_columns<V, W>() ? segments_of(p.cut.blocks, p.cut.n, W * kSteps, 192, kColumnSegments) : 1;
     if (segments > 1 && (!scratch || scratch_bytes < records_bytes(p.cut.m, segments))) return DLFX_ERR_SCRATCH_TOO_SMALL;
     p.cut.length = align_up(ceil_div(p.cut.n, segments), W * kSteps);
     segments = p.cut.segments = ceil_div(p.cut.n, p.cut.length);
     if (grid_of(p.cut.blocks * segments) > kMostThreads / (W * kWave)) return DLFX_ERR_TOO_LARGE;
-    if (segments > 1) {
-        p.records = static_cast<Stretch*>(scratch);
-        p.entering = reinterpret_cast<float*>(static_cast<char*>(scratch) + align_up(static_cast<size_t>(p.cut.m * (segments - 1)) * sizeof(Stretch), 256));
-        gated_cols<S, KIND, V, W, OFF, NT, true><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * (segments - 1)))), dim3(W * kWave), 0, stream>>>(p);
-        DLFX_CHECK_LAUNCH();
+    if constexpr (cut_columns<V, W>()) {
+        if (segments > 1) {
+            p.records = static_cast<Stretch*>(scratch);
+            p.entering = reinterpret_cast<float*>(static_cast<char*>(scratch) + align_up(static_cast<size_t>(p.cut.m * (segments - 1)) * sizeof(Stretch), 256));
+            gated_cols<S, KIND, V, W, OFF, NT, true><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * (segments - 1)))), dim3(W * kWave), 0, stream>>>(p);
+            DLFX_CHECK_LAUNCH();
+        }
     }
     gated_cols<S, KIND, V, W, OFF, NT, false><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * segments))), dim3(W * kWave), 0, stream>>>(p);
     DLFX_CHECK_LAUNCH();
@@ -305,16 +317,24 @@ __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_rows(ScanCall<S
         load_run<true, DIR>(gp, i, end, graw);
         load_run<true, DIR>(xp, i, end, xraw);
     };
-    if (passes > 0) fetch(i0);
-    for (int64_t pass = 0; pass < passes; ++pass, i0 += PASS) {
-        widen();
-        fetch(pass + 1 < passes ? i0 + PASS : i0);        // (after the last whole pass: values that nobody uses)
+    auto walk = [&] {
         const float h = enter();
         if constexpr (!PARTIAL) {
             S out[N];
             states(h, out);
             store_run<true, DIR>(yp, i0, end, out);
         }
+        i0 += PASS;
+    };
+    if (passes > 0) {
+        fetch(i0);
+        for (int64_t pass = 1; pass < passes; ++pass) {
+            widen();
+            fetch(i0 + PASS);
+            walk();
+        }
+        widen();
+        walk();
     }
     if (begin + passes * PASS < end) {
 #pragma unroll

@@ -94,8 +94,10 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
                 carry[v] = d;
             }
         } else if (!PARTIAL) {
-            carry[v] = p.entering[r + v];
-            for (int64_t s = 0; s < segment; ++s) carry[v] = through(p.records[s * p.cut.m + r + v], carry[v]);
+            if constexpr (cut_columns<V, W>()) {
+                __shared__ Stretch shares[W][kWave];
+                carry[v] = enter_column<W>(p.records, p.cut.m, r, segment, p.entering[r], shares);
+            }
         }
     }
 
@@ -185,10 +187,7 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
     const int64_t reach = end < top ? end : top;
     const int64_t passes = reach > begin ? (reach - begin) / (W * N) : 0;
     int64_t i0 = begin + wave * N;
-    if (passes > 0) fetch(i0);
-    for (int64_t pass = 0; pass < passes; ++pass, i0 += W * N) {
-        widen(i0, false);
-        fetch(pass + 1 < passes ? i0 + W * N : i0);       // (after the last whole pass: values that nobody uses)
+    auto walk = [&] {
         float mu[V];
         enter(mu);
         if constexpr (!PARTIAL) {
@@ -203,6 +202,17 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
                 store_at<NT, S, V>(dxp, dxi, dx);
             }
         }
+        i0 += W * N;
+    };
+    if (passes > 0) {
+        fetch(i0);
+        for (int64_t pass = 1; pass < passes; ++pass) {
+            widen(i0, false);
+            fetch(i0 + W * N);
+            walk();
+        }
+        widen(i0, false);
+        walk();
     }
     if (begin + passes * (W * N) < end) {
 #pragma unroll
@@ -246,16 +256,18 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
 template <typename S, int KIND, int V, int W, typename OFF, bool NT>
 int launch_cols(GradCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     p.cut.blocks = ceil_div(p.cut.m, kWave * V);
-    int64_t segments = segments_of(p.cut.blocks, p.cut.n, W * kGradSteps, 192, kColumnSegments);
+    int64_t segments = cut_columns<V, W>() ? segments_of(p.cut.blocks, p.cut.n, W * kGradSteps, 192, kColumnSegments) : 1;
     if (segments > 1 && (!scratch || scratch_bytes < records_bytes(p.cut.m, segments))) return DLFX_ERR_SCRATCH_TOO_SMALL;
     p.cut.length = align_up(ceil_div(p.cut.n, segments), W * kGradSteps);
     segments = p.cut.segments = ceil_div(p.cut.n, p.cut.length);
     if (grid_of(p.cut.blocks * segments) > kMostThreads / (W * kWave)) return DLFX_ERR_TOO_LARGE;
-    if (segments > 1) {
-        p.records = static_cast<Stretch*>(scratch);
-        p.entering = reinterpret_cast<float*>(static_cast<char*>(scratch) + align_up(static_cast<size_t>(p.cut.m * (segments - 1)) * sizeof(Stretch), 256));
-        gated_grad_cols<S, KIND, V, W, OFF, NT, true><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * (segments - 1)))), dim3(W * kWave), 0, stream>>>(p);
-        DLFX_CHECK_LAUNCH();
+    if constexpr (cut_columns<V, W>()) {
+        if (segments > 1) {
+            p.records = static_cast<Stretch*>(scratch);
+            p.entering = reinterpret_cast<float*>(static_cast<char*>(scratch) + align_up(static_cast<size_t>(p.cut.m * (segments - 1)) * sizeof(Stretch), 256));
+            gated_grad_cols<S, KIND, V, W, OFF, NT, true><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * (segments - 1)))), dim3(W * kWave), 0, stream>>>(p);
+            DLFX_CHECK_LAUNCH();
+        }
     }
     gated_grad_cols<S, KIND, V, W, OFF, NT, false><<<dim3(static_cast<unsigned>(grid_of(p.cut.blocks * segments))), dim3(W * kWave), 0, stream>>>(p);
     DLFX_CHECK_LAUNCH();
@@ -372,10 +384,7 @@ __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_grad_rows(GradC
     const int64_t reach = end < top ? end : top;
     const int64_t passes = reach > begin ? (reach - begin) / PASS : 0;
     int64_t i0 = begin + place * N;
-    if (passes > 0) fetch(i0);
-    for (int64_t pass = 0; pass < passes; ++pass, i0 += PASS) {
-        widen(i0, false);
-        fetch(pass + 1 < passes ? i0 + PASS : i0);        // (after the last whole pass: values that nobody uses)
+    auto walk = [&] {
         const float mu = enter();
         if constexpr (!PARTIAL) {
             S dg[N], dx[N];
@@ -383,6 +392,17 @@ __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_grad_rows(GradC
             store_run<true, DIR>(dgp, i0, end, dg);
             store_run<true, DIR>(dxp, i0, end, dx);
         }
+        i0 += PASS;
+    };
+    if (passes > 0) {
+        fetch(i0);
+        for (int64_t pass = 1; pass < passes; ++pass) {
+            widen(i0, false);
+            fetch(i0 + PASS);
+            walk();
+        }
+        widen(i0, false);
+        walk();
     }
     if (begin + passes * PASS < end) {
 #pragma unroll
