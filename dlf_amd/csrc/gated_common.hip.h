@@ -105,7 +105,23 @@ struct Cut {
 constexpr int64_t kBlocksWanted = 512;
 constexpr int kColumnSegments = 64, kRowSegments = 512;      // the most
 
-// Columns in pairs are many and short axes are walked in one pass: only the others are cut.
+// How rows side by side are walked.  All times: us, forward / backward.
+// A lane per row and nothing else up to four steps (decoding: one).
+constexpr int64_t kWalked = 4;
+// Pairs of two-byte rows to a lane and a workgroup of one wavefront once there are four wavefronts for
+// every CU, against 16 wavefronts over one group of 64 rows: bf16 [1024, 131072] 152 / 251 against 157 / 262,
+// [1000, 262144] 303 / 518 against 353 / 564; with fewer, [1024, 65536] 116 against 80.
+constexpr int64_t kManyPairs = 131072;
+// Wavefronts of a workgroup: more of them put more steps in flight, but a pass (16 or 8 steps each) that is
+// longer than the axis leaves some idle.  2, 4, 8 and 16 of them, bf16 rows 262144: n = 48 20 23 42 80 / 33 34 45 77,
+// n = 128 41 40 43 86 / 77 74 78 91, n = 200 67 70 76 95 / 118 116 128 146, n = 300 106 104 113 159 / 175 173 171 213;
+// 16384 rows: n = 200 13.9 11.0 9.5 8.5, n = 300 17.7 12.7 12.5 12.0 / 27.7 20.3 19.1 19.1, n = 1000 48 31 26 24 / 75 49 41 40.
+inline int waves_of(int64_t m, int64_t n) {
+    if (n <= 64) return 2;
+    if (n <= 128 || m >= 131072) return 4;
+    return n <= 256 ? 8 : 16;
+}
+// Only 16 wavefronts over single rows are cut into segments: shorter axes are a pass or two, pairs are many.
 template <int V, int W>
 constexpr bool cut_columns() { return V == 1 && W == 16; }
 
@@ -200,7 +216,7 @@ __device__ __forceinline__ float enter_segment(const Stretch* records, int64_t m
 
 // The same for columns, by a workgroup of W wavefronts: each reads its share of the column's records at
 // once and joins them, the shares meet in LDS.  (One record after the other, by every wavefront:
-// WALKED.)
+// 158.7 us against 149.1 for the second launch of fp32 [1, 65536, 1000].)
 template <int W>
 __device__ __forceinline__ float enter_column(const Stretch* records, int64_t m, int64_t r, int64_t count, float state, Stretch (*lds)[kWave]) {
     constexpr int PER = kColumnSegments / W;

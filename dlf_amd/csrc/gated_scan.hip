@@ -173,15 +173,20 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
         walk();
     }
     if (begin + passes * (W * N) < end) {
-        const S* gp = p.g.base + t0 * p.g.step;
-        const S* xp = p.x.base + t0 * p.x.step;
+        // the last, shorter pass: steps past the end read the last one and become neutral, without a branch
+        const OFF gi = as_it_is(go), xi = as_it_is(xo);
 #pragma unroll
-        for (int i = 0; i < N; ++i, gp += p.g.step, xp += p.x.step) {
+        for (int i = 0; i < N; ++i) {
+            const int64_t t = t0 + i < end ? t0 + i : end - 1;
+            graw[i] = load_at<NT, S, V>(p.g.base + t * p.g.step, gi);
+            xraw[i] = load_at<NT, S, V>(p.x.base + t * p.x.step, xi);
+        }
 #pragma unroll
-            for (int v = 0; v < V; ++v) graw[i].v[v] = neutral_gate<S, KIND>(), xraw[i].v[v] = static_cast<S>(0.0f);
-            if (t0 + i < end) {
-                graw[i] = load_at<NT, S, V>(gp, go);
-                xraw[i] = load_at<NT, S, V>(xp, xo);
+        for (int i = 0; i < N; ++i) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                graw[i].v[v] = t0 + i < end ? graw[i].v[v] : neutral_gate<S, KIND>();
+                xraw[i].v[v] = t0 + i < end ? xraw[i].v[v] : static_cast<S>(0.0f);
             }
         }
         widen();
@@ -390,7 +395,7 @@ int launch_direction(const ScanCall<S>& p, void* scratch, size_t scratch_bytes, 
 template <typename S, int KIND>
 int launch_scan(const ScanCall<S>& p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     const int64_t m = p.cut.m, n = p.cut.n;
-    if (n <= kSteps) {
+    if (n <= kWalked) {
         if (ceil_div(m, 256) > kMostThreads / 256) return DLFX_ERR_TOO_LARGE;
         gated_walk<S, KIND><<<dim3(static_cast<unsigned>(ceil_div(m, 256))), dim3(256), 0, stream>>>(p);
         DLFX_CHECK_LAUNCH();
@@ -401,13 +406,16 @@ int launch_scan(const ScanCall<S>& p, void* scratch, size_t scratch_bytes, hipSt
         return d > 0 ? launch_direction<S, KIND, 1>(p, scratch, scratch_bytes, stream) : launch_direction<S, KIND, -1>(p, scratch, scratch_bytes, stream);
     if (!(short_offsets(p.g) && short_offsets(p.x) && short_offsets(p.y)))
         return launch_cols<S, KIND, 1, 16, int64_t, false>(p, scratch, scratch_bytes, stream);
-    if (n <= 64) return launch_cols<S, KIND, 1, 4, uint32_t, false>(p, scratch, scratch_bytes, stream);
     const bool lines = whole_lines(p.g) && whole_lines(p.x) && whole_lines(p.y);
     if constexpr (sizeof(S) == 2) {
-        if (ceil_div(m, 2 * kWave) >= 512 && pairs_of_rows(p.g) && pairs_of_rows(p.x) && pairs_of_rows(p.y))
-            return lines ? launch_cols<S, KIND, 2, 8, uint32_t, true>(p, scratch, scratch_bytes, stream)
-                         : launch_cols<S, KIND, 2, 8, uint32_t, false>(p, scratch, scratch_bytes, stream);
+        if (m >= kManyPairs && pairs_of_rows(p.g) && pairs_of_rows(p.x) && pairs_of_rows(p.y))
+            return lines ? launch_cols<S, KIND, 2, 1, uint32_t, true>(p, scratch, scratch_bytes, stream)
+                         : launch_cols<S, KIND, 2, 1, uint32_t, false>(p, scratch, scratch_bytes, stream);
     }
+    const int waves = waves_of(m, n);
+    if (waves == 2) return launch_cols<S, KIND, 1, 2, uint32_t, false>(p, scratch, scratch_bytes, stream);
+    if (waves == 4) return launch_cols<S, KIND, 1, 4, uint32_t, false>(p, scratch, scratch_bytes, stream);
+    if (waves == 8) return launch_cols<S, KIND, 1, 8, uint32_t, false>(p, scratch, scratch_bytes, stream);
     return lines ? launch_cols<S, KIND, 1, 16, uint32_t, true>(p, scratch, scratch_bytes, stream)
                  : launch_cols<S, KIND, 1, 16, uint32_t, false>(p, scratch, scratch_bytes, stream);
 }
@@ -420,7 +428,7 @@ using namespace dlfx;
 // (an upper bound over every layout of m rows of n steps, forward and backward: the query does not see the strides)
 extern "C" size_t dlfx_gated_scan_scratch_bytes(int dtype, int64_t m, int64_t n) {
     if (m <= 0 || n <= 0 || (dtype != DLFX_F32 && dtype != DLFX_F16 && dtype != DLFX_BF16)) return 0;
-    return records_bytes(m, std::max(segments_of(ceil_div(m, kWave), n, 32, 192, kColumnSegments), segments_of(m, n, 8192, 192, kRowSegments)));
+    return records_bytes(m, std::max(segments_of(ceil_div(m, kWave), n, 128, 192, kColumnSegments), segments_of(m, n, 8192, 192, kRowSegments)));
 }
 
 extern "C" int dlfx_gated_scan(dlfx_stream_t stream, const char* name, int dtype, int64_t m, int64_t n,

@@ -215,17 +215,21 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
         walk();
     }
     if (begin + passes * (W * N) < end) {
+        // the last, shorter pass: positions past the end read the last one and become neutral, without a branch
+        const OFF gi = as_it_is(go), dyi = as_it_is(dyo), yi = as_it_is(yo), xi = as_it_is(xo);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int64_t t = top - (i0 + i < end ? i0 + i : end - 1);
+            fetch_one(i, p.g.base + t * p.g.step, p.dy.base + t * p.dy.step, p.y.base + (t > 0 ? t - 1 : 0) * p.y.step,
+                      KIND == kGatedBlend ? p.x.base + t * p.x.step : nullptr, gi, dyi, yi, xi);
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                graw[i].v[v] = neutral_gate<S, KIND>();
-                dyraw[i].v[v] = yraw[i].v[v] = xraw[i].v[v] = static_cast<S>(0.0f);
+                graw[i].v[v] = i0 + i < end ? graw[i].v[v] : neutral_gate<S, KIND>();
+                dyraw[i].v[v] = i0 + i < end ? dyraw[i].v[v] : static_cast<S>(0.0f);
             }
-            const int64_t t = top - i0 - i;
-            if (i0 + i < end)
-                fetch_one(i, p.g.base + t * p.g.step, p.dy.base + t * p.dy.step, p.y.base + (t > 0 ? t - 1 : 0) * p.y.step,
-                          KIND == kGatedBlend ? p.x.base + t * p.x.step : nullptr, go, dyo, yo, xo);
         }
         widen(i0, true);
         float mu[V];
@@ -466,7 +470,7 @@ int launch_direction(const GradCall<S>& p, void* scratch, size_t scratch_bytes, 
 template <typename S, int KIND>
 int launch_grad(const GradCall<S>& p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     const int64_t m = p.cut.m, n = p.cut.n;
-    if (n <= 2 * kGradSteps) {
+    if (n <= kWalked) {
         if (ceil_div(m, 256) > kMostThreads / 256) return DLFX_ERR_TOO_LARGE;
         gated_grad_walk<S, KIND><<<dim3(static_cast<unsigned>(ceil_div(m, 256))), dim3(256), 0, stream>>>(p);
         DLFX_CHECK_LAUNCH();
@@ -477,14 +481,17 @@ int launch_grad(const GradCall<S>& p, void* scratch, size_t scratch_bytes, hipSt
         return d > 0 ? launch_direction<S, KIND, -1>(p, scratch, scratch_bytes, stream) : launch_direction<S, KIND, 1>(p, scratch, scratch_bytes, stream);
     if (!(short_offsets(p.g) && short_offsets(p.x) && short_offsets(p.y) && short_offsets(p.dy) && short_offsets(p.dg) && short_offsets(p.dx)))
         return launch_cols<S, KIND, 1, 16, int64_t, false>(p, scratch, scratch_bytes, stream);
-    if (n <= 64) return launch_cols<S, KIND, 1, 4, uint32_t, false>(p, scratch, scratch_bytes, stream);
     const bool lines = whole_lines(p.g) && whole_lines(p.x) && whole_lines(p.y) && whole_lines(p.dy) && whole_lines(p.dg) && whole_lines(p.dx);
     if constexpr (sizeof(S) == 2) {
-        if (ceil_div(m, 2 * kWave) >= 512 && pairs_of_rows(p.g) && pairs_of_rows(p.x) && pairs_of_rows(p.y) && pairs_of_rows(p.dy) &&
+        if (m >= kManyPairs && pairs_of_rows(p.g) && pairs_of_rows(p.x) && pairs_of_rows(p.y) && pairs_of_rows(p.dy) &&
             pairs_of_rows(p.dg) && pairs_of_rows(p.dx))
-            return lines ? launch_cols<S, KIND, 2, 8, uint32_t, true>(p, scratch, scratch_bytes, stream)
-                         : launch_cols<S, KIND, 2, 8, uint32_t, false>(p, scratch, scratch_bytes, stream);
+            return lines ? launch_cols<S, KIND, 2, 1, uint32_t, true>(p, scratch, scratch_bytes, stream)
+                         : launch_cols<S, KIND, 2, 1, uint32_t, false>(p, scratch, scratch_bytes, stream);
     }
+    const int waves = waves_of(m, n);
+    if (waves == 2) return launch_cols<S, KIND, 1, 2, uint32_t, false>(p, scratch, scratch_bytes, stream);
+    if (waves == 4) return launch_cols<S, KIND, 1, 4, uint32_t, false>(p, scratch, scratch_bytes, stream);
+    if (waves == 8) return launch_cols<S, KIND, 1, 8, uint32_t, false>(p, scratch, scratch_bytes, stream);
     return lines ? launch_cols<S, KIND, 1, 16, uint32_t, true>(p, scratch, scratch_bytes, stream)
                  : launch_cols<S, KIND, 1, 16, uint32_t, false>(p, scratch, scratch_bytes, stream);
 }

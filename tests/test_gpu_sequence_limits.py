@@ -123,3 +123,20 @@ def test_views_that_torch_changes_when_read_are_refused(hip_backend):
     with pytest.raises(ValueError):
         hip_backend.from_torch(z.conj().imag)
     assert hip_backend.from_torch(z.conj().resolve_conj()).size == 4
+
+
+# (extents, scanned axis): rows in pairs, on whole cache lines and off them, odd; two, four, eight wavefronts to them
+MANY = [((19, 131072), 0), ((37, 131074), 0), ((5, 131073), 0), ((70, 131073), 0), ((3, 17, 65536), 1), ((2, 33, 65601), 1), ((130, 131075), 0),
+        ((5, 70), 0), ((33, 70), 0), ((90, 70), 0), ((129, 130), 0), ((200, 70), 0), ((256, 66), 0), ((257, 66), 0)]
+
+
+@pytest.mark.parametrize("extents,axis", MANY)
+@pytest.mark.parametrize("kind,dtype", [("gated_blend", "bf16"), ("gated_exp", "f16"), ("gated_sigmoid", "f32")])
+def test_many_columns_and_every_width(hip_backend, extents, axis, kind, dtype):
+    a = [scan_tests.stored(kind, 60 + i, extents, dtype, gate=i == 0) for i in range(3)]
+    G, X, dY = (scan_tests.pair(hip_backend, v) for v in a)
+    kept = extents[:axis] + extents[axis + 1:]
+    initial = normal(63, int(np.prod(kept))).astype(np.float32).reshape(kept)
+    for reverse in (False, True):
+        Y, _ = scan_tests.check_forward(hip_backend, kind, dtype, G, X, axis, reverse, initial)
+        scan_tests.check_grad(hip_backend, kind, dtype, G, X if kind == "gated_blend" else None, (Y, Y.numpy()), dY, axis, reverse, initial, initial)
