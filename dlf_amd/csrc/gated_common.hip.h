@@ -102,7 +102,6 @@ struct Cut {
     int64_t segments, length;    // of the axis; length steps each, the last one shorter
 };
 
-constexpr int64_t kBlocksWanted = 512;
 constexpr int kColumnSegments = 64, kRowSegments = 512;      // the most
 
 // How rows side by side are walked.  All times: us, forward / backward.
@@ -240,15 +239,23 @@ __device__ __forceinline__ float enter_column(const Stretch* records, int64_t m,
 template <typename S>
 int direction(const Track<S>& t) { return t.step == 1 ? 1 : t.step == -1 ? -1 : 0; }
 
-// How many segments: one while the groups of rows alone give the device its workgroups, otherwise
-// about kBlocksWanted workgroups in all, none shorter than `shortest` steps.
-inline int64_t segments_of(int64_t groups, int64_t n, int64_t shortest, int64_t enough, int64_t limit) {
+// How many segments: one while the groups of rows alone are enough, otherwise about `wanted` workgroups in
+// all, none shorter than `shortest` steps.  A cut axis is read nearly twice.
+inline int64_t segments_of(int64_t groups, int64_t n, int64_t shortest, int64_t enough, int64_t wanted, int64_t limit) {
     if (groups >= enough) return 1;
-    int64_t s = ceil_div(kBlocksWanted, groups);
+    int64_t s = ceil_div(wanted, groups);
     if (s > limit) s = limit;
     const int64_t most = n / shortest;
     return s < most ? s : (most < 1 ? 1 : most);
 }
+// us, whole and cut: columns bf16 [8192, 4096] 119 / 76, [8192, 8192] 128 / 139, fp32 [8192, 8192] 182 / 238.  256, 512
+// and 1024 workgroups wanted: bf16 [8192, 4096] 71 76 85, [65536, 1024] 133 142 149, fp32 [65536, 1000] 278 268 274.
+template <typename S>
+int64_t column_segments(int64_t groups, int64_t n, int64_t shortest) {
+    return segments_of(groups, n, shortest, 128, sizeof(S) == 2 ? 256 : 512, kColumnSegments);
+}
+// Rows of 131072 bf16, whole and cut: 64 of them 30 / 28, 128 of them 32 / 46.
+inline int64_t row_segments(int64_t groups, int64_t n, int64_t shortest) { return segments_of(groups, n, shortest, 64, 512, kRowSegments); }
 
 // Scratch of a cut call: what every segment but the last does to the state, and a copy of the
 // states that enter the axis (the tensor they come from may be the one that `last` is written to).

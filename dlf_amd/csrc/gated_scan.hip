@@ -213,7 +213,7 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
 template <typename S, int KIND, int V, int W, typename OFF, bool NT>
 int launch_cols(ScanCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     p.cut.blocks = ceil_div(p.cut.m, kWave * V);
-    int64_t segments = cut_columns<V, W>() ? segments_of(p.cut.blocks, p.cut.n, W * kSteps, 192, kColumnSegments) : 1;
+    int64_t segments = cut_columns<V, W>() ? column_segments<S>(p.cut.blocks, p.cut.n, W * kSteps) : 1;
     if (segments > 1 && (!scratch || scratch_bytes < records_bytes(p.cut.m, segments))) return DLFX_ERR_SCRATCH_TOO_SMALL;
     p.cut.length = align_up(ceil_div(p.cut.n, segments), W * kSteps);
     segments = p.cut.segments = ceil_div(p.cut.n, p.cut.length);
@@ -364,7 +364,7 @@ template <typename S, int KIND, int G, int W, int DIR>
 int launch_rows(ScanCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     constexpr int BLOCK = W > 4 ? W * kWave : 256, PASS = W * G * run_length<S>();
     p.cut.blocks = ceil_div(p.cut.m, BLOCK / (W * G));
-    int64_t segments = W > 4 ? segments_of(p.cut.blocks, p.cut.n, PASS, 192, kRowSegments) : 1;
+    int64_t segments = W > 4 ? row_segments(p.cut.blocks, p.cut.n, PASS) : 1;
     if (segments > 1 && (!scratch || scratch_bytes < records_bytes(p.cut.m, segments))) return DLFX_ERR_SCRATCH_TOO_SMALL;
     p.cut.length = align_up(ceil_div(p.cut.n, segments), PASS);
     segments = p.cut.segments = ceil_div(p.cut.n, p.cut.length);
@@ -382,13 +382,18 @@ int launch_rows(ScanCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t 
     return DLFX_OK;
 }
 
+// How rows along memory are walked: no pass is longer than the row (a run is 32 bytes), which would leave lanes
+// idle.  us, 4, 16, 32, 64 lanes: bf16 [262144, 64] 22 71 - -, [65536, 256] 22 23 42 -, [32768, 512] - 23 23 42,
+// [16384, 1024] - - 22 23.  One, four, sixteen wavefronts: [512, 32768] 45 21 26, [2048, 32768] 86 80 89,
+// [256, 131072] - 44 39, [512, 131072] - 82 85; [64, 4096] 10.6 9.8 10.2.
 template <typename S, int KIND, int DIR>
 int launch_direction(const ScanCall<S>& p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
-    if (p.cut.n <= 4 * run_length<S>()) return launch_rows<S, KIND, 4, 1, DIR>(p, scratch, scratch_bytes, stream);
-    if (p.cut.n <= 16 * run_length<S>()) return launch_rows<S, KIND, 16, 1, DIR>(p, scratch, scratch_bytes, stream);
-    if (p.cut.n <= 32 * run_length<S>()) return launch_rows<S, KIND, 32, 1, DIR>(p, scratch, scratch_bytes, stream);
-    if (p.cut.m >= 2048) return launch_rows<S, KIND, kWave, 1, DIR>(p, scratch, scratch_bytes, stream);
-    if (p.cut.m >= 512 || p.cut.n <= 4 * kWave * run_length<S>()) return launch_rows<S, KIND, kWave, 4, DIR>(p, scratch, scratch_bytes, stream);
+    const int64_t runs = p.cut.n / run_length<S>();
+    if (runs < 16) return launch_rows<S, KIND, 4, 1, DIR>(p, scratch, scratch_bytes, stream);
+    if (runs < 32) return launch_rows<S, KIND, 16, 1, DIR>(p, scratch, scratch_bytes, stream);
+    if (runs < kWave) return launch_rows<S, KIND, 32, 1, DIR>(p, scratch, scratch_bytes, stream);
+    if (p.cut.m >= 2048 && runs < 32 * kWave) return launch_rows<S, KIND, kWave, 1, DIR>(p, scratch, scratch_bytes, stream);
+    if (p.cut.m >= 512 || runs <= 4 * kWave) return launch_rows<S, KIND, kWave, 4, DIR>(p, scratch, scratch_bytes, stream);
     return launch_rows<S, KIND, kWave, 16, DIR>(p, scratch, scratch_bytes, stream);
 }
 
@@ -428,7 +433,7 @@ using namespace dlfx;
 // (an upper bound over every layout of m rows of n steps, forward and backward: the query does not see the strides)
 extern "C" size_t dlfx_gated_scan_scratch_bytes(int dtype, int64_t m, int64_t n) {
     if (m <= 0 || n <= 0 || (dtype != DLFX_F32 && dtype != DLFX_F16 && dtype != DLFX_BF16)) return 0;
-    return records_bytes(m, std::max(segments_of(ceil_div(m, kWave), n, 128, 192, kColumnSegments), segments_of(m, n, 8192, 192, kRowSegments)));
+    return records_bytes(m, std::max(column_segments<float>(ceil_div(m, kWave), n, 128), row_segments(m, n, 8192)));
 }
 
 extern "C" int dlfx_gated_scan(dlfx_stream_t stream, const char* name, int dtype, int64_t m, int64_t n,

@@ -260,7 +260,7 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
 template <typename S, int KIND, int V, int W, typename OFF, bool NT>
 int launch_cols(GradCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     p.cut.blocks = ceil_div(p.cut.m, kWave * V);
-    int64_t segments = cut_columns<V, W>() ? segments_of(p.cut.blocks, p.cut.n, W * kGradSteps, 192, kColumnSegments) : 1;
+    int64_t segments = cut_columns<V, W>() ? column_segments<S>(p.cut.blocks, p.cut.n, W * kGradSteps) : 1;
     if (segments > 1 && (!scratch || scratch_bytes < records_bytes(p.cut.m, segments))) return DLFX_ERR_SCRATCH_TOO_SMALL;
     p.cut.length = align_up(ceil_div(p.cut.n, segments), W * kGradSteps);
     segments = p.cut.segments = ceil_div(p.cut.n, p.cut.length);
@@ -439,7 +439,7 @@ template <typename S, int KIND, int G, int W, int DIR>
 int launch_rows(GradCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
     constexpr int BLOCK = W > 4 ? W * kWave : 256, PASS = W * G * run_length<S>();
     p.cut.blocks = ceil_div(p.cut.m, BLOCK / (W * G));
-    int64_t segments = W > 4 ? segments_of(p.cut.blocks, p.cut.n, PASS, 192, kRowSegments) : 1;
+    int64_t segments = W > 4 ? row_segments(p.cut.blocks, p.cut.n, PASS) : 1;
     if (segments > 1 && (!scratch || scratch_bytes < records_bytes(p.cut.m, segments))) return DLFX_ERR_SCRATCH_TOO_SMALL;
     p.cut.length = align_up(ceil_div(p.cut.n, segments), PASS);
     segments = p.cut.segments = ceil_div(p.cut.n, p.cut.length);
@@ -459,11 +459,12 @@ int launch_rows(GradCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t 
 
 template <typename S, int KIND, int DIR>
 int launch_direction(const GradCall<S>& p, void* scratch, size_t scratch_bytes, hipStream_t stream) {
-    if (p.cut.n <= 4 * run_length<S>()) return launch_rows<S, KIND, 4, 1, DIR>(p, scratch, scratch_bytes, stream);
-    if (p.cut.n <= 16 * run_length<S>()) return launch_rows<S, KIND, 16, 1, DIR>(p, scratch, scratch_bytes, stream);
-    if (p.cut.n <= 32 * run_length<S>()) return launch_rows<S, KIND, 32, 1, DIR>(p, scratch, scratch_bytes, stream);
-    if (p.cut.m >= 2048) return launch_rows<S, KIND, kWave, 1, DIR>(p, scratch, scratch_bytes, stream);
-    if (p.cut.m >= 512 || p.cut.n <= 4 * kWave * run_length<S>()) return launch_rows<S, KIND, kWave, 4, DIR>(p, scratch, scratch_bytes, stream);
+    const int64_t runs = p.cut.n / run_length<S>();
+    if (runs < 16) return launch_rows<S, KIND, 4, 1, DIR>(p, scratch, scratch_bytes, stream);
+    if (runs < 32) return launch_rows<S, KIND, 16, 1, DIR>(p, scratch, scratch_bytes, stream);
+    if (runs < kWave) return launch_rows<S, KIND, 32, 1, DIR>(p, scratch, scratch_bytes, stream);
+    if (p.cut.m >= 2048 && runs < 32 * kWave) return launch_rows<S, KIND, kWave, 1, DIR>(p, scratch, scratch_bytes, stream);
+    if (p.cut.m >= 512 || runs <= 4 * kWave) return launch_rows<S, KIND, kWave, 4, DIR>(p, scratch, scratch_bytes, stream);
     return launch_rows<S, KIND, kWave, 16, DIR>(p, scratch, scratch_bytes, stream);
 }
 
