@@ -28,7 +28,7 @@ def test_more_threads_than_a_launch_counts():
             assert call(1 << 33, 20, (20, 1), dtype) == LARGE                 # lanes along the row
             assert call(1 << 33, 2000, (2000, 1), dtype) == LARGE
             assert call(1 << 31, 40, (1, 1 << 31), dtype) == LARGE            # rows side by side
-            assert call(1 << 30, 400, (1, 1 << 30), dtype) == LARGE
+            assert call(1 << 34, 400, (1, 1 << 34), dtype) == LARGE
             assert call(1 << 30, 400, (2, 1 << 32), dtype) == LARGE           # ... far apart
     m = (1 << 26) - 3
     assert lib.dlfx_route(None, b"softmax", 0, m, 8, FAKE, 0, 8, None, 1, 1, 1, 2, 0, 1.0, OTHER, OTHER, None) == LARGE
