@@ -522,15 +522,16 @@ struct RouteGradCall {
 //                            only the k chosen logits are read.
 // The places' gradients meet the row in LDS; a lane writes ITEMS neighbouring experts.  (The same by
 // handing every place to every lane and comparing: 14.6 us for bf16 [65537, 128], k = 8, against this one's
-// 9.6.)  An index that stands in the row twice is added up in the order of the places.
+// 8.2, at 4.6 TB/s.)  An index that stands in the row twice is added up in the order of the places.
 template <typename S, int KIND, int L, int ITEMS>
 __global__ __launch_bounds__(256) void route_grad_rows(const S* x, S* dx, RouteGradCall p) {
     constexpr int TEAMS = 256 / L;
     const int lane = threadIdx.x % L, team = threadIdx.x / L;
     const int64_t r = static_cast<int64_t>(blockIdx.x) * TEAMS + team;
-    __shared__ float lds[TEAMS][L * ITEMS + 16];           // (16: the teams of a wavefront start on different banks)
+    __shared__ float lds[TEAMS][L * (ITEMS + 1)];          // (one left over per lane: 64 lanes, 64 banks, also over four teams)
     __shared__ uint8_t owners[TEAMS][L * ITEMS];
-    float* const slots = lds[team];
+    auto slot = [&](int e) -> float& { return lds[team][e + e / ITEMS]; };
+    float* const own = &lds[team][lane * (ITEMS + 1)];
     const bool live = r < p.m;
     const int64_t rr = live ? r : p.m - 1;
     const S* xr = x + rr * p.stride;
@@ -544,7 +545,7 @@ __global__ __launch_bounds__(256) void route_grad_rows(const S* x, S* dx, RouteG
         row.normalise();
     }
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) slots[lane * ITEMS + i] = 0.0f;
+    for (int i = 0; i < ITEMS; ++i) own[i] = 0.0f;
     // the places of the row, L at a time: place t in lane t % L
     float top = kMinusInfinity, total = 0.0f, dot = 0.0f;
     auto fetch = [&](int t, int& e, float& v, float& d) {
@@ -601,11 +602,11 @@ __global__ __launch_bounds__(256) void route_grad_rows(const S* x, S* dx, RouteG
         wave_sync();
         if (__any(e >= 0 && owners[team][e] != lane)) {
             for (int t = 0; t < L && t0 + t < p.k; ++t) {
-                if (lane == t && e >= 0) slots[e] += g;
+                if (lane == t && e >= 0) slot(e) += g;
                 wave_sync();
             }
         } else if (e >= 0) {
-            slots[e] += g;
+            slot(e) += g;
         }
         wave_sync();
     }
@@ -613,7 +614,7 @@ __global__ __launch_bounds__(256) void route_grad_rows(const S* x, S* dx, RouteG
     float grad[ITEMS];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        grad[i] = slots[lane * ITEMS + i];
+        grad[i] = own[i];
         if (KIND == kSoftmaxScore && !p.renormalise) grad[i] -= dot * row.score(row.x[i]);
     }
     S* out = dx + r * p.dx_stride + lane * ITEMS;
