@@ -15,6 +15,7 @@
 // other calls are one launch.
 // fp32 [32768, 256] sigmoid, bias, the best 4 of 8 groups, k = 8: 29.2 us (VALU 86 % busy) + 10.3 (the latency of a
 // few rows in 64 bits); bf16 [65537, 128] softmax, k = 8: 21.8 us (VALU 91 %); [24, 64]: 3.5 us.
+#include <cmath>
 #include <cstring>
 
 #include "sequence.hip.h"
@@ -107,15 +108,17 @@ struct Best {
     }
 };
 
-// Values of the groups in sums[] from their experts' in items[] (NaN: absent), by a team of L lanes.
+// Values of the groups in sums[] from their experts' in items[] (NaN: absent), by a team of L lanes.  Returns the
+// largest magnitude among the lane's experts.
 template <int L, typename C>
-__device__ __forceinline__ void group_values(const RouteCall& p, const C* items, C* sums, int lane) {
+__device__ __forceinline__ C group_values(const RouteCall& p, const C* items, C* sums, int lane) {
     const C none = -std::numeric_limits<C>::infinity();
     // lanes_per lanes (a power of two) to a group; a lane walks its part of the group's experts from a
     // place of its own, so that the lanes read different LDS banks
     int lanes_per = L;
     while (lanes_per > 1 && lanes_per * p.groups > L) lanes_per >>= 1;
     const int part = lane & (lanes_per - 1), side_by_side = L / lanes_per;
+    C largest = 0;
     for (int g0 = 0; g0 < p.groups; g0 += side_by_side) {
         const int g = g0 + lane / lanes_per;
         Best<C> best = {none, none, 0};
@@ -124,19 +127,23 @@ __device__ __forceinline__ void group_values(const RouteCall& p, const C* items,
             for (int i = part; i < p.size; i += lanes_per) {
                 int e = i + from;
                 e -= e >= p.size ? p.size : 0;
-                best.add(items[g * p.size + e]);
+                const C v = items[g * p.size + e];
+                best.add(v);
+                largest = std::fmax(largest, std::fabs(v));          // (of a NaN and a number: the number)
             }
         }
         for (int j = 1; j < lanes_per; j <<= 1) best.add({lane_xor(best.first, j), lane_xor(best.second, j), lane_xor(best.count, j)});
         if (g < p.groups && part == 0) sums[g] = best.value(p.group_best);
     }
     wave_sync();
+    return largest;
 }
 
 // Which groups are kept, a byte each.  `unsure` when the values are not exact and a kept group's lies too
-// close to one that was left.
+// close to one that was left; `largest`: of the |choices| that the lane has seen.
 template <int L, typename C>
-__device__ __forceinline__ void keep_groups(const RouteCall& p, const C* sums, uint8_t* kept, bool exact, float scores, int lane, bool& unsure) {
+__device__ __forceinline__ void keep_groups(const RouteCall& p, const C* sums, uint8_t* kept, bool exact, float scores, float largest, int lane,
+                                            bool& unsure) {
     const C none = -std::numeric_limits<C>::infinity();
     C worst_kept = -none, best_left = none;
     for (int g = lane; g < p.groups; g += L) {
@@ -159,9 +166,12 @@ __device__ __forceinline__ void keep_groups(const RouteCall& p, const C* sums, u
     if (!exact) {
         worst_kept = team_reduce<L>(worst_kept, [](C a, C b) { return b < a ? b : a; });
         best_left = team_reduce<L>(best_left, [](C a, C b) { return b > a ? b : a; });
-        // (a sum of two choices carries two errors)
+        // Two sums of two choices carry four scores' errors, a rounding of each sum (2 u of the larger one in all, at
+        // most 4 u of the largest choice) and of each choice with its bias: 4 u of the largest choice, however
+        // small the sums are where biases cancel.
+        largest = team_reduce<L>(largest, [](float a, float b) { return fmaxf(a, b); });
         const float a = static_cast<float>(worst_kept), b = static_cast<float>(best_left);
-        if (best_left != none && !(a - b > 2.0f * border(scores, a, b))) unsure = true;
+        if (best_left != none && !(a - b > 2.0f * scores + 0x1p-20f * largest)) unsure = true;
     }
 }
 
@@ -257,7 +267,7 @@ __device__ __forceinline__ int choose_exactly(const RouteCall& p, const S* x, do
         double* sums = items;                                // (groups of one expert are their experts)
         bool settled = false;
         if (p.size > 1) group_values<kWave>(p, items, sums = items + p.n, lane);
-        keep_groups<kWave>(p, sums, flags, true, 0.0f, lane, settled);
+        keep_groups<kWave>(p, sums, flags, true, 0.0f, 0.0f, lane, settled);
     }
     uint64_t* images = reinterpret_cast<uint64_t*>(items);
 #pragma unroll 1
@@ -307,8 +317,8 @@ __device__ __forceinline__ int choose(const RouteCall& p, const RouteRow<S, KIND
                 if (i * L + lane < p.n) lds[i * L + lane] = row.x[i] == kMinusInfinity ? std::numeric_limits<float>::quiet_NaN() : v;
             }
             wave_sync();
-            group_values<L>(p, lds, lds + L * ITEMS, lane);
-            keep_groups<L>(p, lds + L * ITEMS, flags, exact, row.error(), lane, unsure);
+            const float largest = group_values<L>(p, lds, lds + L * ITEMS, lane);
+            keep_groups<L>(p, lds + L * ITEMS, flags, exact, row.error(), largest, lane, unsure);
         }
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
@@ -460,8 +470,10 @@ __device__ __forceinline__ void flush_loads(const RouteCall& p, int32_t* histogr
         if (histogram[e]) atomicAdd(&p.loads[e], histogram[e]);
 }
 
+// (four wavefronts to a SIMD, which the LDS of 256 experts has room for: left alone, the compiler takes 130 registers,
+// two too many, and fp32 [32768, 256] with groups takes 44.1 us a call instead of 38.6)
 template <typename S, int KIND, int L, int ITEMS>
-__global__ __launch_bounds__(256) void route_rows(const S* x, RouteCall p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void route_rows(const S* x, RouteCall p) {
     constexpr int TEAMS = 256 / L;
     __shared__ double lds[TEAMS][team_doubles<L, ITEMS>()];
     __shared__ int32_t histogram[L * ITEMS];
