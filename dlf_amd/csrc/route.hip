@@ -528,7 +528,7 @@ struct RouteGradCall {
 };
 
 // With c the chosen experts, d the weights' gradients times scale:
-//   sigmoid:                 ds[c] = d;  renormalised: (d - sum d s / S) / S, S the chosen scores' sum;  dx = ds s (1 - s)
+//   sigmoid:                 dx[c] = d s (1 - s);  renormalised: q (d - sum d q) (1 - s), q = s / S, S the chosen scores' sum
 //   softmax:                 dx = s (ds - sum ds s), over every expert
 //   softmax, renormalised:   the weights are the chosen logits' own softmax q: dx[c] = q (d - sum d q), 0 elsewhere -
 //                            only the k chosen logits are read.
@@ -605,8 +605,9 @@ __global__ __launch_bounds__(256) void route_grad_rows(const S* x, S* dx, RouteG
         place(t0, e, v, d);
         float g = 0.0f;
         if (e >= 0) {
-            const float s = score(v);
-            if (p.renormalise) d = (d - dot * by) * by;
+            float s = score(v);
+            // (the score's share first, at most 1: by alone can be large enough to overflow beside d)
+            if (p.renormalise) s *= by, d -= dot * by;
             if constexpr (KIND == kSoftmaxScore) g = s * d;
             else g = s * d * row.score(-v);
         }

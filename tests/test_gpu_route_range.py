@@ -1,4 +1,4 @@
-"""route at the ends of its range: sums of choices that cancel."""
+"""route at the ends of its range: sums of choices that cancel, chosen scores near 2^-126."""
 import numpy as np
 import pytest
 
@@ -37,3 +37,33 @@ def test_groups_whose_biases_cancel(hip_backend, n, spread, score):
     clear = ranked[:, kept] - ranked[:, kept - 1] > 64 * 2.0 ** -53 * spread
     assert clear.mean() > 0.99
     assert np.array_equal(I.numpy()[clear], want[clear])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,k", [(16, 4), (300, 6), (64, 20)])
+@pytest.mark.parametrize("low", [-82.0])
+def test_renormalised_scores_near_the_end_of_fp32(hip_backend, dtype, n, k, low):
+    # logistic scores of about exp(low): only their ratios count
+    m = 33
+    x = O.store(low - 3.0 * uniform01(7, m * n).reshape(m, n), dtype)
+    X, values = Tensor.from_numpy(hip_backend, x), O.load(x)
+    # ratios from exp(x - top) / (1 + exp(x)): the second factor is 1 in 64 bits
+    I0 = np.argsort(-values, axis=1, kind="stable")[:, :k]
+    v = np.take_along_axis(values, I0, 1)
+    q = np.exp(v - v[:, :1])
+    q /= q.sum(1, keepdims=True)
+    W, I = F.route(X, k, "sigmoid", renormalise=True, scale=2.5)
+    hip_backend.synchronize()
+    assert np.array_equal(I.numpy(), I0)
+    assert O.close(W.numpy(), 2.5 * q, T.BOUND * 2.5 * q, "f32")
+    # the gradient under a loss scaled by 2^16: d(w)/dx = q (d - sum d q) with 1 - s = 1
+    dw = (65536 * normal(8, m * k)).astype(np.float32).reshape(m, k)
+    G = F.route_grad(X, Tensor.from_numpy(hip_backend, I0.astype(np.int32)), Tensor.from_numpy(hip_backend, dw), "sigmoid", renormalise=True, scale=2.5)
+    hip_backend.synchronize()
+    d = 2.5 * dw.astype(np.float64)
+    mean = (d * q).sum(1, keepdims=True)
+    want, size = np.zeros((m, n)), np.zeros((m, n))
+    np.put_along_axis(want, I0, q * (d - mean), 1)
+    np.put_along_axis(size, I0, q * (np.abs(d) + (np.abs(d) * q).sum(1, keepdims=True)), 1)
+    assert np.isfinite(want).all()
+    assert O.close(G.numpy(), want, 2 * T.BOUND * size, dtype)
