@@ -431,6 +431,14 @@ __device__ __forceinline__ int choose(const RouteCall& p, const RouteRow<S, KIND
     return static_cast<int>(0xffffffffu - static_cast<uint32_t>(mine));
 }
 
+// A chosen logit's score over exp(top) (logistic: over exp(min(top, 0))), top the largest chosen one: where only ratios
+// count, as after a renormalisation, scores below fp32's range keep theirs.
+template <int KIND>
+__device__ __forceinline__ float score_to(float v, float top) {
+    if constexpr (KIND == kSoftmaxScore) return __builtin_amdgcn_exp2f((v - top) * kLog2E);
+    else return __builtin_amdgcn_exp2f((fminf(v, 0.0f) - fminf(top, 0.0f)) * kLog2E) / (1.0f + __builtin_amdgcn_exp2f(-fabsf(v) * kLog2E));
+}
+
 // What place `lane` < k of row r gets once its expert e is settled.
 constexpr int32_t kUnsettled = -1;
 template <typename S, int KIND, int L, int ITEMS>
@@ -440,10 +448,9 @@ __device__ __forceinline__ void settle(const RouteCall& p, const RouteRow<S, KIN
     const bool place = lane < p.k;
     const float v = place ? static_cast<float>(xr[e]) : kMinusInfinity;
     const bool there = place && !(v <= lowest_of<S>());
-    if (KIND == kSoftmaxScore && p.renormalise) {
-        // the chosen logits' own softmax: what all scores have in common cancels
+    if (p.renormalise) {
         const float top = team_reduce<L>(there ? v : kMinusInfinity, [](float a, float b) { return fmaxf(a, b); });
-        if (there) s = __builtin_amdgcn_exp2f((v - top) * kLog2E);
+        if (there) s = score_to<KIND>(v, top);
     } else if (there) {
         s = row.score(v);
     }
@@ -574,7 +581,7 @@ __global__ __launch_bounds__(256) void route_grad_rows(const S* x, S* dx, RouteG
         if (t0) fetch(t0 + lane, e, v, d);
         else e = first_e, v = first_v, d = first_d;
     };
-    if (KIND == kSoftmaxScore && p.renormalise) {
+    if (p.renormalise) {
         for (int t0 = 0; t0 < p.k; t0 += L) {
             int e;
             float v, d;
@@ -583,10 +590,7 @@ __global__ __launch_bounds__(256) void route_grad_rows(const S* x, S* dx, RouteG
         }
         top = team_reduce<L>(top, [](float a, float b) { return fmaxf(a, b); });
     }
-    auto score = [&](float v) {
-        if (KIND == kSoftmaxScore && p.renormalise) return __builtin_amdgcn_exp2f((v - top) * kLog2E);
-        return row.score(v);
-    };
+    auto score = [&](float v) { return p.renormalise ? score_to<KIND>(v, top) : row.score(v); };
     for (int t0 = 0; t0 < p.k; t0 += L) {
         int e;
         float v, d;
@@ -606,7 +610,6 @@ __global__ __launch_bounds__(256) void route_grad_rows(const S* x, S* dx, RouteG
         float g = 0.0f;
         if (e >= 0) {
             float s = score(v);
-            // (the score's share first, at most 1: by alone can be large enough to overflow beside d)
             if (p.renormalise) s *= by, d -= dot * by;
             if constexpr (KIND == kSoftmaxScore) g = s * d;
             else g = s * d * row.score(-v);

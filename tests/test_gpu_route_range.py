@@ -1,4 +1,4 @@
-"""route at the ends of its range: sums of choices that cancel, chosen scores near 2^-126."""
+"""route at the ends of its range: sums of choices that cancel, chosen scores near and below 2^-126."""
 import numpy as np
 import pytest
 
@@ -41,11 +41,11 @@ def test_groups_whose_biases_cancel(hip_backend, n, spread, score):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("n,k", [(16, 4), (300, 6), (64, 20)])
-@pytest.mark.parametrize("low", [-82.0])
-def test_renormalised_scores_near_the_end_of_fp32(hip_backend, dtype, n, k, low):
+@pytest.mark.parametrize("low", [-82.0, -88.0, -100.0, -5000.0])
+def test_renormalised_scores_near_and_below_the_end_of_fp32(hip_backend, dtype, n, k, low):
     # logistic scores of about exp(low): only their ratios count
     m = 33
-    x = O.store(low - 3.0 * uniform01(7, m * n).reshape(m, n), dtype)
+    x = O.store(low - 3.0 * uniform01(7, m * n).reshape(m, n) if low > -1000 else np.round(low - 3.0 * uniform01(7, m * n).reshape(m, n)), dtype)
     X, values = Tensor.from_numpy(hip_backend, x), O.load(x)
     # ratios from exp(x - top) / (1 + exp(x)): the second factor is 1 in 64 bits
     I0 = np.argsort(-values, axis=1, kind="stable")[:, :k]
@@ -67,3 +67,29 @@ def test_renormalised_scores_near_the_end_of_fp32(hip_backend, dtype, n, k, low)
     np.put_along_axis(size, I0, q * (np.abs(d) + (np.abs(d) * q).sum(1, keepdims=True)), 1)
     assert np.isfinite(want).all()
     assert O.close(G.numpy(), want, 2 * T.BOUND * size, dtype)
+
+
+def test_renormalised_scores_of_both_signs(hip_backend):
+    # chosen logits from -120 to 120 in one row: weights and gradients from ratios to the largest score
+    m, n, k = 64, 24, 10
+    x = O.store(240.0 * uniform01(17, m * n).reshape(m, n) - 120.0, "f32")
+    x[0], x[1] = O.store(-np.arange(n, dtype=np.float64) - 86.0, "f32"), O.store(np.arange(n, dtype=np.float64) + 90.0, "f32")
+    X, values = Tensor.from_numpy(hip_backend, x), O.load(x)
+    idx = np.stack([np.argsort(uniform01(100 + r, n))[:k] for r in range(m)])
+    W, I = F.route(X, k, "sigmoid", renormalise=True)
+    hip_backend.synchronize()
+    s = O.sigmoid(np.take_along_axis(values, I.numpy().astype(np.int64), 1))
+    want = s / s.sum(1, keepdims=True)
+    # terms (1.5 |x| + 2) u of the exponential of a logit up to 120 below 0
+    assert O.close(W.numpy(), want, (180 * O.U + T.BOUND) * want, "f32")
+    dw = normal(18, m * k).astype(np.float32).reshape(m, k)
+    G = F.route_grad(X, Tensor.from_numpy(hip_backend, idx.astype(np.int32)), Tensor.from_numpy(hip_backend, dw), "sigmoid", renormalise=True)
+    hip_backend.synchronize()
+    v = np.take_along_axis(values, idx, 1)
+    s = O.sigmoid(v)
+    q = s / s.sum(1, keepdims=True)
+    d = dw.astype(np.float64)
+    g, size = np.zeros((m, n)), np.zeros((m, n))
+    np.put_along_axis(g, idx, q * (d - (d * q).sum(1, keepdims=True)) * O.sigmoid(-v), 1)
+    np.put_along_axis(size, idx, q * (np.abs(d) + (np.abs(d) * q).sum(1, keepdims=True)) * O.sigmoid(-v), 1)
+    assert O.close(G.numpy(), g, (4 * 180 * O.U + 2 * T.BOUND) * size, "f32")
