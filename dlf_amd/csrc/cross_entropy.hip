@@ -10,7 +10,8 @@
 // bf16 [8192, 128000], loss and gradient: 803 us (5.3 TB/s); fp16 [4096, 8192] pieces: 18.9 us a state (3.6 TB/s), 25.6 a
 // gradient (5.2 TB/s); loss of fp32 [64, 32000]: 6.1 us.
 // Sums and maxima are fp32; exponentials are the hardware's 2^x of (x - maximum) log2(e), where the
-// difference comes first: it is exact for neighbours, whatever the logits' common offset.
+// difference comes first: it is exact for neighbours, whatever the logits' common offset.  An fp32 gradient's own
+// exponentials are exact to the function's error (scaled_exp); a sum is not nearer to 64 bits for it.
 #include <atomic>
 #include <utility>
 
@@ -36,6 +37,21 @@ constexpr float kNone = -std::numeric_limits<float>::infinity();
 constexpr float kLargest = std::numeric_limits<float>::max();
 
 __device__ __forceinline__ float exp_diff(float x, float mx) { return __builtin_amdgcn_exp2f((x - mx) * kLog2E); }
+
+// factor * exp(x - mx), an element of a gradient.  For fp32 elements what the product with log2(e) loses, d u of the
+// result at a distance d below the maximum, is made up for to first order; ln 2 itself, rounded, leaves d u / 22.
+// Two-byte elements round far above it.
+template <typename S>
+__device__ __forceinline__ float scaled_exp(float factor, float x, float mx) {
+    if constexpr (sizeof(S) == 4) {
+        const float d = fmaxf(x - mx, -200.0f);            // (exp(d) is 0 long before; of -inf nothing would be left to make up)
+        const float t = d * kLog2E;
+        const float v = factor * __builtin_amdgcn_exp2f(t);
+        return fmaf(v, fmaf(-t, 0.693147180559945309417f, d), v);
+    } else {
+        return factor * exp_diff(x, mx);
+    }
+}
 
 __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b) {
     const float mx = fmaxf(a.mx, b.mx);
@@ -147,7 +163,7 @@ __device__ __forceinline__ Vec<S, vector_width<S>()> grad_vector(int64_t e0, con
     float v[V];
     widen<S>(x, v);
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = g.p * exp_diff(v[i], g.mx);
+    for (int i = 0; i < V; ++i) v[i] = scaled_exp<S>(g.p, v[i], g.mx);
     const uint64_t at = static_cast<uint64_t>(target - e0);
     if (at < V) {
 #pragma unroll
@@ -245,7 +261,7 @@ __global__ __launch_bounds__(256) void grad_rows_tiny(const S* x, int64_t m, int
     const RowGrad g = row_grad(s, target >= 0, weights ? weights[r] : 1.0f, z);
 #pragma unroll
     for (int i = 0; i < V; ++i)
-        if (i < n) dx[r * dx_stride + i] = static_cast<S>(g.zero ? 0.0f : g.p * exp_diff(v[i], g.mx) - (i == target ? g.up : 0.0f));
+        if (i < n) dx[r * dx_stride + i] = static_cast<S>(g.zero ? 0.0f : scaled_exp<S>(g.p, v[i], g.mx) - (i == target ? g.up : 0.0f));
 }
 
 // A row cut into tiles, a workgroup each: workgroup = row * tiles + tile.
