@@ -47,7 +47,7 @@ __device__ __forceinline__ S neutral_gate() {
 
 // What a stretch of steps does to the state that enters it: h -> a h + b.  The product of many
 // gates can leave the range of fp32 where the states do not (growth from a tiny state, decay of a
-// large one), so it is held in 64 bits; an exact zero stays one under any growth.
+// large one), so it is held in 64 bits.
 struct Stretch {
     double a;
     float b;
@@ -55,7 +55,17 @@ struct Stretch {
 __device__ __forceinline__ float through(const Stretch& s, float h) {
     return h == 0.0f ? s.b : static_cast<float>(s.a * static_cast<double>(h) + static_cast<double>(s.b));
 }
-__device__ __forceinline__ Stretch join(const Stretch& first, const Stretch& then) { return {first.a * then.a, through(then, first.b)}; }
+
+// Products that pass fp64 as well, from there on the largest number: growth that no state but 0 survives.  A gate of 0
+// behind them or before still makes 0, which an infinity would not.
+constexpr double kFar = 0x1p1000;
+__device__ __forceinline__ bool in_range(double a) { return fabs(a) < kFar; }
+__device__ __forceinline__ double times(double a, double b) {
+    const double p = a * b;
+    if (a == 0.0 || b == 0.0 || !(fabs(a) <= std::numeric_limits<double>::max()) || !(fabs(b) <= std::numeric_limits<double>::max())) return p;
+    return in_range(a) && in_range(b) && in_range(p) ? p : copysign(std::numeric_limits<double>::max(), p);
+}
+__device__ __forceinline__ Stretch join(const Stretch& first, const Stretch& then) { return {times(first.a, then.a), through(then, first.b)}; }
 
 // V neighbouring elements at base + off bytes.  The base is the same for the whole wavefront and the
 // offset a lane's own: with 32 bits of it an access takes both as they are, without address arithmetic.
@@ -177,8 +187,9 @@ __device__ __forceinline__ void store_run(S* row, int64_t i0, int64_t end, const
 // The stretches of a group of G lanes (4, 16, 32 or 64, in order) joined from the group's first lane up
 // to each; `before` is what lies before the lane, `all` the whole group's.
 template <int G>
-__device__ __forceinline__ void join_lanes(Stretch s, Stretch& before, Stretch& all) {
+__device__ __forceinline__ void join_lanes(const Stretch& own, Stretch& before, Stretch& all) {
     const int lane = lane_id();
+    Stretch s = own;
     auto step = [&](double pa, float pb, bool mine) {
         if (!mine) pa = 1.0, pb = 0.0f;
         s.b = through(s, pb);
@@ -193,6 +204,17 @@ __device__ __forceinline__ void join_lanes(Stretch s, Stretch& before, Stretch& 
     }
     if constexpr (G >= 32) step(dpp_fetch<kRowBcast15, 0xa>(s.a, 1.0), dpp_fetch<kRowBcast15, 0xa>(s.b, 0.0f), true);
     if constexpr (G >= 64) step(dpp_fetch<kRowBcast31, 0xc>(s.a, 1.0), dpp_fetch<kRowBcast31, 0xc>(s.b, 0.0f), true);
+    // a product that passed the range left its mark on all lanes behind it: an infinity, or the NaN that it and a 0
+    // make.  Groups of lanes with such a mark once more, by products that stay in range.
+    if (const uint64_t far = __ballot(!in_range(s.a))) {
+        Stretch f = own;
+#pragma unroll 1
+        for (int d = 1; d < G; d <<= 1) {
+            const Stretch first = {lane_get(f.a, (lane - d) & (kWave - 1)), lane_get(f.b, (lane - d) & (kWave - 1))};
+            if (lane % G >= d) f = join(first, f);
+        }
+        if (G == kWave || (far >> (lane & ~(G - 1)) & ((1ull << (G & (kWave - 1))) - 1))) s = f;
+    }
     before.a = lane_get(s.a, (lane + kWave - 1) % kWave);
     before.b = lane_get(s.b, (lane + kWave - 1) % kWave);
     if (lane % G == 0) before = {1.0, 0.0f};

@@ -130,12 +130,21 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float c = carry[v], mine = carry[v];
+            double far = product[v];
 #pragma unroll
             for (int w = 0; w < W; ++w) {
                 if (w == wave) mine = c;
                 const float wa = lds[parity][w][lane][2 * v];
                 c = fmaf(wa, c, lds[parity][w][lane][2 * v + 1]);
-                if constexpr (PARTIAL) product[v] *= static_cast<double>(wa);
+                if constexpr (PARTIAL) far *= static_cast<double>(wa);
+            }
+            if constexpr (PARTIAL) {
+                if (!in_range(far)) {
+                    far = product[v];
+#pragma unroll 1
+                    for (int w = 0; w < W; ++w) far = times(far, static_cast<double>(lds[parity][w][lane][2 * v]));
+                }
+                product[v] = far;
             }
             carry[v] = c;
             h[v] = mine;
@@ -298,18 +307,26 @@ __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_rows(ScanCall<S
             if (lane_id() == 0) lds[parity][team][wave] = all;
             __syncthreads();
             float c = carry;
+            double far = product;
 #pragma unroll
             for (int w = 0; w < W; ++w) {
                 if (w == wave) h = c;
                 const Stretch s = lds[parity][team][w];
                 c = through(s, c);
-                if constexpr (PARTIAL) product *= s.a;
+                if constexpr (PARTIAL) far *= s.a;
+            }
+            if constexpr (PARTIAL) {
+                if (!in_range(far)) {
+                    far = product;
+#pragma unroll 1
+                    for (int w = 0; w < W; ++w) far = times(far, lds[parity][team][w].a);
+                }
+                product = far;
             }
             carry = c;
             parity ^= 1;
         } else {
             carry = through(all, carry);
-            if constexpr (PARTIAL) product *= all.a;
         }
         return through(before, h);
     };
