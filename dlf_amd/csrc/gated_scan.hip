@@ -114,6 +114,7 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
     };
     // The pass's states from the stretches of all wavefronts; h: the state that enters this one's steps.
     int parity = 0;
+    float entering[V], first[V];
     auto enter = [&](float (&h)[V]) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -129,7 +130,7 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
         __syncthreads();
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            float c = carry[v], mine = carry[v];
+            float c = entering[v] = carry[v], mine = carry[v];
             double far = product[v];
 #pragma unroll
             for (int w = 0; w < W; ++w) {
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
                 product[v] = far;
             }
             carry[v] = c;
-            h[v] = mine;
+            h[v] = first[v] = mine;
         }
         parity ^= 1;
     };
@@ -163,6 +164,17 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
 
     const int64_t passes = (end - begin) / (W * N);
     int64_t t0 = begin + wave * N;
+    // (after enter has turned to the other half of lds)
+    auto repair = [&](int64_t past) {
+        repair_pass<V, W>(lds[parity], wave, lane, entering, carry, first, [&](float (&h)[V]) {
+            S* yp = p.y.base + t0 * p.y.step;
+#pragma unroll
+            for (int i = 0; i < N; ++i, yp += p.y.step) {
+                const Vec<S, V> out = state(i, h);
+                if (t0 + i < past) store_at<false, S, V>(yp, yo, out);
+            }
+        });
+    };
     auto walk = [&] {
         float h[V];
         enter(h);
@@ -171,6 +183,7 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
             const OFF yi = as_it_is(yo);
 #pragma unroll
             for (int i = 0; i < N; ++i, yp += p.y.step) store_at<NT, S, V>(yp, yi, state(i, h));
+            repair(t0 + N);
         }
         t0 += W * N;
     };
@@ -211,6 +224,23 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
                 const Vec<S, V> out = state(i, h);
                 if (t0 + i < end) store_at<NT, S, V>(yp, yo, out);
             }
+            repair(end);
+        }
+    }
+    if constexpr (PARTIAL) {
+        // a segment whose state got lost (as in repair_pass) once more, step after step
+        if (wave == 0 && !finite(carry[0])) {
+            float h = 0.0f;
+            double far = 1.0;
+            for (int64_t t = begin; t < end; ++t) {
+                float factor, keep = 1.0f, x = static_cast<float>(load_at<false, S, 1>(p.x.base + t * p.x.step, xo).v[0]);
+                gate_of<S, KIND>(static_cast<float>(load_at<false, S, 1>(p.g.base + t * p.g.step, go).v[0]), factor, keep);
+                if constexpr (KIND == kGatedBlend) x *= keep;
+                h = fmaf(factor, h, x);
+                far = times(far, static_cast<double>(factor));
+            }
+            carry[0] = h;
+            product[0] = far;
         }
     }
     if (wave == 0) {
@@ -300,8 +330,12 @@ __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_rows(ScanCall<S
             pa *= a[i];
             pb = fmaf(a[i], pb, b[i]);
         }
-        Stretch before, all;
-        join_lanes<G>({pa, pb}, before, all);
+        Stretch own = {pa, pb}, before, all;
+        if (__any(!finite(pa))) {
+            const double p = product_of(a);
+            if (!finite(pa)) own.a = p;
+        }
+        join_lanes<G>(own, before, all);
         float h = carry;
         if constexpr (W > 1) {
             if (lane_id() == 0) lds[parity][team][wave] = all;

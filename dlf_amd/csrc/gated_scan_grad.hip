@@ -147,6 +147,7 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
         }
     };
     int parity = 0;
+    float entering[V], first[V];
     auto enter = [&](float (&mu)[V]) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -162,7 +163,7 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
         __syncthreads();
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            float c = carry[v], mine = carry[v];
+            float c = entering[v] = carry[v], mine = carry[v];
             double far = product[v];
 #pragma unroll
             for (int w = 0; w < W; ++w) {
@@ -180,7 +181,7 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
                 product[v] = far;
             }
             carry[v] = c;
-            mu[v] = mine;
+            mu[v] = first[v] = mine;
         }
         parity ^= 1;
     };
@@ -198,6 +199,22 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
     const int64_t reach = end < top ? end : top;
     const int64_t passes = reach > begin ? (reach - begin) / (W * N) : 0;
     int64_t i0 = begin + wave * N;
+    // (after enter has turned to the other half of lds)
+    auto repair = [&](int64_t past) {
+        repair_pass<V, W>(lds[parity], wave, lane, entering, carry, first, [&](float (&mu)[V]) {
+            S* dgp = p.dg.base + (top - i0) * p.dg.step;
+            S* dxp = p.dx.base + (top - i0) * p.dx.step;
+#pragma unroll
+            for (int i = 0; i < N; ++i, dgp -= p.dg.step, dxp -= p.dx.step) {
+                Vec<S, V> dg, dx;
+                gradient(i, mu, dg, dx);
+                if (i0 + i < past) {
+                    store_at<false, S, V>(dgp, dgo, dg);
+                    store_at<false, S, V>(dxp, dxo, dx);
+                }
+            }
+        });
+    };
     auto walk = [&] {
         float mu[V];
         enter(mu);
@@ -212,6 +229,7 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
                 store_at<NT, S, V>(dgp, dgi, dg);
                 store_at<NT, S, V>(dxp, dxi, dx);
             }
+            repair(i0 + N);
         }
         i0 += W * N;
     };
@@ -257,6 +275,22 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
                     store_at<NT, S, V>(dxp, dxo, dx);
                 }
             }
+            repair(end);
+        }
+    }
+    if constexpr (PARTIAL) {
+        // a segment whose state got lost (as in repair_pass) once more, step after step
+        if (wave == 0 && !finite(carry[0])) {
+            float state = 0.0f;
+            double far = 1.0;
+            for (int64_t t = top - begin; t > top - end; --t) {
+                float factor, rest = 1.0f;
+                gate_of<S, KIND>(static_cast<float>(load_at<false, S, 1>(p.g.base + t * p.g.step, go).v[0]), factor, rest);
+                state = factor * (static_cast<float>(load_at<false, S, 1>(p.dy.base + t * p.dy.step, dyo).v[0]) + state);
+                far = times(far, static_cast<double>(factor));
+            }
+            carry[0] = state;
+            product[0] = far;
         }
     }
     if (wave == 0) {
@@ -363,8 +397,12 @@ __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_grad_rows(GradC
             pa *= a[i];
             pb = a[i] * (d[i] + pb);
         }
-        Stretch before, all;
-        join_lanes<G>({pa, pb}, before, all);
+        Stretch own = {pa, pb}, before, all;
+        if (__any(!finite(pa))) {
+            const double p = product_of(a);
+            if (!finite(pa)) own.a = p;
+        }
+        join_lanes<G>(own, before, all);
         float mu = carry;
         if constexpr (W > 1) {
             if (lane_id() == 0) lds[parity][team][wave] = all;

@@ -340,8 +340,8 @@ int dlfx_fill(dlfx_stream_t stream, int dtype, int rank, const int64_t* dims, co
  * value per row: views over the kept dims, rank - 1 strides each, either may be NULL.  A gate that
  * makes the factor 0 (g = 0, or -inf) starts a new sequence at that step; the arithmetic is the
  * formula's, so a state that is already infinite or NaN is not forgotten by it.  The factors of up
- * to 16 neighbouring steps are multiplied in fp32 before they meet the state: growth by more than
- * 2^8 a step that lasts can turn a state of 0 into NaN there, decay below 2^-126 in one go is 0.
+ * to 16 neighbouring steps are multiplied in fp32 before they meet the state: decay below 2^-126 in
+ * one go is 0.  (Growth past fp32 there is noticed and the steps are taken one by one.)
  * y may be x or gate (the same pointer, offset and strides), last may be initial: with n == 1 that
  * is the step of a decoding loop, the state updated in place.  Outputs with a stride of 0 on an
  * extent above 1 are refused.  The result depends on neither the stream nor the device's load: how

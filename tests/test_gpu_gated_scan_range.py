@@ -68,3 +68,22 @@ def test_growth_behind_a_reset(hip_backend, extents, axis, reverse, dtype):
     got, want = run_grad(hip_backend, "gated", dtype, along(g[::-1], extents, axis, reverse), along(x[::-1], extents, axis, reverse), 1.0, axis, reverse)
     for a, b in zip(got, want):
         assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("extents,axis", LAYOUTS + [((19, 131072), 0)])
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_growth_past_fp32_in_a_few_steps(hip_backend, extents, axis, reverse, dtype):
+    # factors of 2^20: ten of them take a state from 2^-100 to 2^100, seven overflow a product in fp32; before that a
+    # state of 0 under the same factors.  Every fortieth step starts over.
+    n = extents[axis]
+    t = (np.arange(n) + 7) % 40
+    g = np.where(t == 0, 0.0, np.where(t <= 10, 2.0 ** 20, 1.0))
+    x = np.where((t == 0) & (np.arange(n) >= 60), 2.0 ** -100, 0.0)
+    y, last, want, want_last = run(hip_backend, "gated", dtype, along(g, extents, axis, reverse), along(x, extents, axis, reverse), 0.0, axis, reverse)
+    assert np.array_equal(y, want) and np.array_equal(last, want_last)
+    # (backwards the state is multiplied after it is added to: lam = 2^-100 at the step before a growth)
+    got, want = run_grad(hip_backend, "gated", dtype, along(g[::-1], extents, axis, reverse), along(np.roll(x, 1)[::-1], extents, axis, reverse), 0.0,
+                         axis, reverse)
+    for a, b in zip(got, want):
+        assert np.isfinite(b).all() and np.array_equal(a, b)
