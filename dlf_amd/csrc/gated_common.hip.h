@@ -47,13 +47,13 @@ __device__ __forceinline__ S neutral_gate() {
 
 // What a stretch of steps does to the state that enters it: h -> a h + b.  The product of many
 // gates can leave the range of fp32 where the states do not (growth from a tiny state, decay of a
-// large one), so it is held in 64 bits.
+// large one), so it is held in 64 bits; it is finite unless a gate is not (times()).
 struct Stretch {
     double a;
     float b;
 };
 __device__ __forceinline__ float through(const Stretch& s, float h) {
-    return h == 0.0f ? s.b : static_cast<float>(s.a * static_cast<double>(h) + static_cast<double>(s.b));
+    return static_cast<float>(s.a * static_cast<double>(h) + static_cast<double>(s.b));
 }
 
 // Products that pass fp64 as well, from there on the largest number: growth that no state but 0 survives.  A gate of 0

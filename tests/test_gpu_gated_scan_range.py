@@ -87,3 +87,21 @@ def test_growth_past_fp32_in_a_few_steps(hip_backend, extents, axis, reverse, dt
                          axis, reverse)
     for a, b in zip(got, want):
         assert np.isfinite(b).all() and np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("extents,axis", LAYOUTS + [((19, 131072), 0), ((3, 60), 0)])
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("kind", ["gated", "gated_sigmoid"])
+def test_a_gate_of_nan_shows(hip_backend, extents, axis, reverse, kind):
+    # also where the state that it meets is 0: NaN from there on
+    n = extents[axis]
+    for at in sorted({0, 1, n // 2, n // 2 // 16 * 16, n // 2 // 2048 * 2048, n - 2}):
+        g = np.full(n, 0.5)
+        g[at] = np.nan
+        full, zeros = along(g, extents, axis, reverse), np.zeros(extents)
+        y, last, want, want_last = run(hip_backend, kind, "f32", full, zeros, 0.0, axis, reverse)
+        assert np.isnan(want).sum() == want.size // n * (n - at)
+        assert np.array_equal(y, want, equal_nan=True) and np.array_equal(last, want_last, equal_nan=True), at
+        got, want = run_grad(hip_backend, kind, "f32", full, zeros, 0.0, axis, reverse)
+        for a, b in zip(got, want):
+            assert np.array_equal(np.isnan(a), np.isnan(b)), at
