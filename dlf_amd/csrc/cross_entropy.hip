@@ -600,12 +600,13 @@ extern "C" int dlfx_cross_entropy_grad(dlfx_stream_t stream, int dtype, int inde
                                        void* dx, int64_t dx_offset, int64_t dx_row_stride,
                                        void* scratch, size_t scratch_bytes) {
     if (int e = check(m, n, x, row_stride, targets)) return e;
-    if (!dx || dx_row_stride < n || (x_offset == dx_offset && overwrites(x, row_stride, dx, dx_row_stride, m))) return DLFX_ERR_INVALID_ARGUMENT;
+    if (!dx || dx_row_stride < n) return DLFX_ERR_INVALID_ARGUMENT;
     if (!index_ok(index_dtype)) return DLFX_ERR_UNSUPPORTED_DTYPE;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     return dispatch_sequence_dtype(dtype, [&](auto tag) {
         using S = decltype(tag);
         LossCall<S> p{static_cast<const S*>(x) + x_offset, m, n, row_stride, Targets{targets, index_dtype == DLFX_I64}, 0, 0, nullptr, z_loss, loss, {}, nullptr};
+        if (overwrites(p.x, row_stride, static_cast<const S*>(dx) + dx_offset, dx_row_stride, m)) return static_cast<int>(DLFX_ERR_INVALID_ARGUMENT);
         return launch_grad(p, weights, static_cast<S*>(dx) + dx_offset, dx_row_stride, scratch, scratch_bytes, s);
     });
 }
@@ -641,13 +642,13 @@ extern "C" int dlfx_cross_entropy_piece_grad(dlfx_stream_t stream, int dtype, in
                                              void* dx, int64_t dx_offset, int64_t dx_row_stride) {
     if (int e = check(m, n, x, row_stride, targets)) return e;
     if (!state || first < 0 || !dx || dx_row_stride < n) return DLFX_ERR_INVALID_ARGUMENT;
-    if (x_offset == dx_offset && overwrites(x, row_stride, dx, dx_row_stride, m)) return DLFX_ERR_INVALID_ARGUMENT;
     if (!index_ok(index_dtype)) return DLFX_ERR_UNSUPPORTED_DTYPE;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     return dispatch_sequence_dtype(dtype, [&](auto tag) {
         using S = decltype(tag);
         LossCall<S> p{static_cast<const S*>(x) + x_offset, m, n, row_stride, Targets{targets, index_dtype == DLFX_I64}, first, 0, const_cast<float*>(state), z_loss,
                          nullptr, {}, nullptr};
+        if (overwrites(p.x, row_stride, static_cast<const S*>(dx) + dx_offset, dx_row_stride, m)) return static_cast<int>(DLFX_ERR_INVALID_ARGUMENT);
         return launch_grad_tiles(p, 0, weights, static_cast<S*>(dx) + dx_offset, dx_row_stride, s);
     });
 }

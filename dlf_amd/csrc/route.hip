@@ -721,10 +721,11 @@ extern "C" int dlfx_route_grad(dlfx_stream_t stream, const char* name, int dtype
     int kind;
     if (int e = check(name, m, n, k, x, row_stride, &kind)) return e;
     if (!indices || !dweights || !dx || dx_row_stride < n) return DLFX_ERR_INVALID_ARGUMENT;
-    if (x_offset == dx_offset && overwrites(x, row_stride, dx, dx_row_stride, m)) return DLFX_ERR_INVALID_ARGUMENT;
     RouteGradCall p{m, row_stride, dx_row_stride, static_cast<int>(n), static_cast<int>(k), renormalise, scale, indices, dweights};
     return dispatch_sequence_dtype(dtype, [&](auto tag) {
         using S = decltype(tag);
+        if (overwrites(static_cast<const S*>(x) + x_offset, row_stride, static_cast<const S*>(dx) + dx_offset, dx_row_stride, m))
+            return static_cast<int>(DLFX_ERR_INVALID_ARGUMENT);
         return dispatch_team(n, 1, [&](auto lanes, auto items) {
             constexpr int L = decltype(lanes)::value, ITEMS = decltype(items)::value;
             auto run = [&](auto kernel) {

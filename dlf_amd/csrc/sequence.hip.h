@@ -44,8 +44,10 @@ struct AnyVec {
 // A launch counts its threads along an axis of the grid in 32 bits.
 constexpr int64_t kMostThreads = 0xffffffffLL;
 
-// The same matrix written over itself at another stride would be read where it has been written.
-inline bool overwrites(const void* x, int64_t stride, const void* dx, int64_t dx_stride, int64_t m) { return x == dx && stride != dx_stride && m > 1; }
+// The same matrix written over itself at another stride would be read where it has been written.  (By the address
+// that an offset leads to: one start can be given as different pointers and offsets.)
+template <typename S>
+bool overwrites(const S* x, int64_t stride, const S* dx, int64_t dx_stride, int64_t m) { return x == dx && stride != dx_stride && m > 1; }
 
 inline bool strides_distinct(int rank, const int64_t* dims, const int64_t* strides) {
     for (int i = 0; i < rank; ++i)
