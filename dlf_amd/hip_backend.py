@@ -282,12 +282,18 @@ class HipBackend:
         return tensor
 
     def from_torch(self, tensor) -> Tensor:
-        """A Tensor over the memory of a torch tensor of this backend's device (no copy; any strides)."""
+        """A Tensor over the memory of a torch tensor of this backend's device (no copy; any strides).
+
+        What is computed from it has no history: torch's autograd neither sees these calls nor their gradients, which
+        are calls of their own.  A tensor that requires a gradient is therefore refused while torch records (detach it,
+        or call inside torch.no_grad() or an autograd function)."""
         if tensor.device != self.device:
             raise ValueError("the tensor is on %s, this backend on %s" % (tensor.device, self.device))
         if tensor.is_conj() or tensor.is_neg():
             raise ValueError("a view that torch conjugates or negates when it is read: resolve it first")
         if tensor.requires_grad:
+            if self.torch.is_grad_enabled():
+                raise ValueError("the tensor requires a gradient, which torch would not get through these calls: detach() it first")
             tensor = tensor.detach()
         extents = tuple(tensor.shape)
         if 0 in extents:
