@@ -443,7 +443,9 @@ def gated_scan_grad(G: Tensor, X: Optional[Tensor], Y: Tensor, dY: Tensor, axis:
                     initial: Optional[Tensor] = None, dlast: Optional[Tensor] = None):
     """Gradients (dG, dX, dinitial) of gated_scan for dY and dlast (None: zeros), from the Y that it
     returned.  Only "gated_blend" reads X (None otherwise will do).  dG has every element of X's
-    extents: where G shares a gate, sum it over the shared axes (reduce_sum)."""
+    extents: where G shares a gate, sum it over the shared axes (reduce_sum; for bfloat16, which that does
+    not take, the last state of gated_scan(one, dG, axis) with gates of 1, a single one under strides of
+    0 will do, is the sum in fp32)."""
     where = "gated_scan_grad(%s)" % kind
     if kind not in GATE_KINDS:
         raise ValueError("%s: kind is one of %s" % (where, ", ".join(GATE_KINDS)))

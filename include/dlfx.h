@@ -355,8 +355,9 @@ int dlfx_fill(dlfx_stream_t stream, int dtype, int rank, const int64_t* dims, co
  *   dgate[t] = lam[t] y[t-1] a'[t]  ("gated_blend": lam[t] (y[t-1] - x[t]) a'[t]),  y[-1] = initial,
  * a[t] the factor and a'[t] its derivative by g.  dgate has an element of its own for every
  * element of dims, also where the gate's stride is 0: its sum over the shared extents is then the
- * gate's gradient (dlfx_reduce).  dx may be dy, dgate may be gate, dinitial may be dlast; the other
- * tensors must not overlap the outputs.  dinitial may be NULL.
+ * gate's gradient (dlfx_reduce; DLFX_BF16, which that refuses: `last` of a "gated" call along the
+ * shared extent with gates of 1 is the sum in fp32).  dx may be dy, dgate may be gate, dinitial may
+ * be dlast; the other tensors must not overlap the outputs.  dinitial may be NULL.
  */
 size_t dlfx_gated_scan_scratch_bytes(int dtype, int64_t m, int64_t n);
 int dlfx_gated_scan(dlfx_stream_t stream, const char* name, int dtype, int64_t m, int64_t n,
