@@ -73,7 +73,7 @@ def build_all(force=False, jobs=None):
     return LIB
 
 
-VENEER_TESTS = [os.path.join(HERE, "..", "tests", "cpp", name) for name in ("veneer_test", "sequence_test")]
+VENEER_TESTS = [os.path.join(HERE, "..", "tests", "cpp", name) for name in ("veneer_test", "sequence_test", "sequence_views_test")]
 
 
 def build_veneer_test(force=False):

@@ -588,12 +588,22 @@ DevTensor<T> along(const DevTensor<T>& X, int axis, bool reverse) {
     auto v = moveaxis(X, axis, -1);
     return reverse ? flip(v, -1) : v;
 }
-// Rows of X along its last axis at one stride: {m, n, stride}.
+// Rows of X along its last axis, contiguous each and at one stride (a slice of a wider matrix): {m, n, stride}.
 template <typename T>
 std::vector<size_t> rows_of(const DevTensor<T>& X) {
-    want(X.rank() >= 1 && X.shape().is_contiguous(), "rows along the last axis of a contiguous tensor");
+    const char* what = "rows along the last axis, contiguous and at one stride";
+    want(X.rank() >= 1, what);
     const size_t n = X.extent(-1);
-    return {X.size() / n, n, n};
+    want(n == 1 || X.shape().stride(-1) == 1, what);
+    size_t stride = n, size = 1;
+    for (int i = static_cast<int>(X.rank()) - 2; i >= 0; --i) {
+        if (X.extent(i) == 1) continue;
+        if (size == 1) stride = X.shape().stride(i);
+        want(X.shape().stride(i) == stride * size, what);
+        size *= X.extent(i);
+    }
+    want(stride >= n && stride <= static_cast<size_t>(std::numeric_limits<int64_t>::max()), what);      // (a negative one wraps)
+    return {X.size() / n, n, stride};
 }
 }  // namespace detail
 
@@ -667,7 +677,7 @@ void route_grad(const DevTensor<T>& X, const DevTensor<int32_t>& indices, const 
         dlf::detail::want(s->extents() == dims && s->is_contiguous() && s->offset() == 0, "route_grad: indices and gradients of the weights");
     if (&dX != &X) dX.resize(X.shape());
     gpgpu::dnn::route_grad(score, r[0], r[1], X.data(), X.shape().offset(), r[2], how, indices.data(), dweights.data(),
-                           dX.data(), dX.shape().offset(), r[2]);
+                           dX.data(), dX.shape().offset(), &dX != &X ? r[1] : r[2]);
 }
 
 namespace detail {
@@ -697,7 +707,7 @@ void cross_entropy_grad(const DevTensor<T>& X, const DevTensor<I>& targets, DevT
     loss.resize(detail::rows_shape(X));
     if (&dX != &X) dX.resize(X.shape());
     gpgpu::dnn::cross_entropy_grad(r[0], r[1], X.data(), X.shape().offset(), r[2], targets.data(), weights ? &weights->data() : nullptr, z_loss,
-                                   &loss.data(), dX.data(), dX.shape().offset(), r[2]);
+                                   &loss.data(), dX.data(), dX.shape().offset(), &dX != &X ? r[1] : r[2]);
 }
 // In pieces: columns first, first + 1, ... of the vocabulary into the rows' state (an empty tensor is
 // started anew); the losses once all have gone by; a piece's gradient from the finished state.
@@ -726,7 +736,7 @@ void cross_entropy_piece_grad(const DevTensor<T>& X, const DevTensor<I>& targets
     if (weights) detail::per_row(*weights, r[0], "cross_entropy_piece_grad: one weight per row");
     if (&dX != &X) dX.resize(X.shape());
     gpgpu::dnn::cross_entropy_piece_grad(r[0], r[1], X.data(), X.shape().offset(), r[2], targets.data(), first, state.data(),
-                                         weights ? &weights->data() : nullptr, z_loss, dX.data(), dX.shape().offset(), r[2]);
+                                         weights ? &weights->data() : nullptr, z_loss, dX.data(), dX.shape().offset(), &dX != &X ? r[1] : r[2]);
 }
 }  // namespace dnn
 
