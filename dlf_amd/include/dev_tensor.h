@@ -626,6 +626,7 @@ void gated_scan(const DevTensor<T>& G, const DevTensor<T>& X, DevTensor<T>& Y, D
                            Y.data(), y.shape().offset(), y.shape().strides(), detail::row_state(&last));
 }
 // Gradients of gated_scan from the Y that it wrote; X is read by "gated_blend" only, dlast null: zeros.
+// dG may be G, dX may be dY, dinitial may be the tensor that dlast points to.
 template <typename T>
 void gated_scan_grad(const DevTensor<T>& G, const DevTensor<T>& X, const DevTensor<T>& Y, const DevTensor<T>& dY,
                      DevTensor<T>& dG, DevTensor<T>& dX, DevTensor<float>& dinitial, int axis = -1, const std::string& kind = "gated",
@@ -635,9 +636,10 @@ void gated_scan_grad(const DevTensor<T>& G, const DevTensor<T>& X, const DevTens
     const bool blend = kind == "gated_blend";
     detail::want(G.shape() == Y.shape() && dY.shape() == Y.shape() && (!blend || X.shape() == Y.shape()), "gated_scan_grad: extents");
     detail::want((!initial || initial->shape().extents() == kept) && (!dlast || dlast->shape().extents() == kept), "gated_scan_grad: the states' extents");
-    dG.resize(Y.shape());
-    dX.resize(Y.shape());
-    dinitial.resize(Shape(kept));
+    // (over an input: where and how that lies)
+    if (&dG != &G) dG.resize(Y.shape());
+    if (&dX != &dY) dX.resize(Y.shape());
+    if (&dinitial != dlast) dinitial.resize(Shape(kept));
     const auto g = detail::along(G, axis, reverse), y = detail::along(Y, axis, reverse), dy = detail::along(dY, axis, reverse);
     const auto dg = detail::along(dG, axis, reverse), dx = detail::along(dX, axis, reverse);
     const auto x = blend ? detail::along(X, axis, reverse) : y;

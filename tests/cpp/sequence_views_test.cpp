@@ -92,9 +92,28 @@ static void test_rows_at_a_stride() {
     CHECK(refuses([&] { dnn::cross_entropy(W.view(Shape::as_strided({6, 8}, {0, 1}, 0)), t, l1); }));
 }
 
+// A gradient over an input that is a view: the input is read where it lies.
+static void test_gradients_over_views() {
+    const std::vector<float> gate = {0.5f, 0.25f, 1.f, 2.f, 0.5f, 1.f, 0.f, 0.5f}, dy = {1.f, 2.f, -1.f, 0.5f, 4.f, 1.f, 2.f, 8.f};
+    auto dense_g = dev(Tensor<float>({2, 3}, {gate[1], gate[3], gate[5], gate[2], gate[4], gate[6]}));
+    auto dense_dy = dev(Tensor<float>({2, 3}, {dy[1], dy[3], dy[5], dy[2], dy[4], dy[6]}));
+    auto Y = dev(Tensor<float>({2, 3}, {1.f, 2.f, 3.f, 4.f, 5.f, 6.f}));
+    auto dlast = dev(Tensor<float>({2}, {0.5f, -1.f}));
+    DevTensor<float> dG, dX, dS;
+    gated_scan_grad(dense_g, Y, Y, dense_dy, dG, dX, dS, 1, "gated", nullptr, &dlast);
+    auto g = dev(Tensor<float>({8}, gate)).view(Shape::as_strided({2, 3}, {1, 2}, 1));
+    auto d = dev(Tensor<float>({8}, dy)).view(Shape::as_strided({2, 3}, {1, 2}, 1));
+    auto s = dev(Tensor<float>({4}, {9.f, 0.5f, 9.f, -1.f})).view(Shape::as_strided({2}, {2}, 1));
+    gated_scan_grad(g, Y, Y, d, g, d, s, 1, "gated", nullptr, &s);
+    CHECK(g.read() == dG.read());
+    CHECK(d.read() == dX.read());
+    CHECK(s.read() == dS.read());
+}
+
 int main() {
     try {
         test_rows_at_a_stride();
+        test_gradients_over_views();
     } catch (const std::exception& e) {
         std::fprintf(stderr, "exception: %s\n", e.what());
         return 1;
