@@ -268,19 +268,38 @@ __device__ __forceinline__ float enter_column(const Stretch* records, int64_t m,
     return state;
 }
 
+// Every wavefront of the workgroup goes on from the same bits, those of the first one, even if a caller's error lets
+// something write to them meanwhile: whether repair_pass waits at barriers must never differ between wavefronts.
+template <int V, int W>
+__device__ __forceinline__ void share_carry(float (&carry)[V], int wave, int lane) {
+    if constexpr (W > 1) {
+        __shared__ float start[kWave][V];
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (wave == 0) start[lane][v] = carry[v];
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < V; ++v) carry[v] = start[lane][v];
+    }
+}
+
 // After a pass of rows side by side that turned a finite state into an infinite one or NaN: in truth, or because a
 // wavefront's gates multiplied past fp32 before they met the state.  Such rows go through the pass again, wavefront
-// after wavefront and step after step.  All wavefronts hold the same `entering` and `state` (the pass's), so all of them
-// come here or none.  first: the state that entered the wavefront's steps; again(h) walks them from h and stores what
-// they give.  `lds` is the half that the next pass is going to use.  (Here, behind the pass's stores: between them and
-// the join it cost the gradient 4 % of its time.)
+// after wavefront and step after step.  All wavefronts hold the same `entering` and `state` (share_carry, then the
+// records in LDS), so all of them come here or none.  first: the state that entered the wavefront's steps; again(h)
+// walks them from h and stores what they give.  `lds` is the half that the next pass is going to use.  (Here, behind
+// the pass's stores: between them and the join it cost the gradient 4 % of its time.)
 template <int V, int W, typename Again>
 __device__ __forceinline__ void repair_pass(float (*lds)[kWave][2 * V], int wave, int lane, const float (&entering)[V], float (&state)[V],
                                             const float (&first)[V], Again&& again) {
     bool lost = false;
 #pragma unroll
-    for (int v = 0; v < V; ++v) lost = lost || (finite(entering[v]) && !finite(state[v]));
+    for (int v = 0; v < V; ++v) lost = lost || !finite(state[v]);
     if (__builtin_expect(!__any(lost), 1)) return;
+    lost = false;
+#pragma unroll
+    for (int v = 0; v < V; ++v) lost = lost || (finite(entering[v]) && !finite(state[v]));
+    if (!__any(lost)) return;
     float h[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) h[v] = entering[v];

@@ -88,6 +88,8 @@ __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
         }
     }
 
+    if constexpr (!PARTIAL) share_carry<V, W>(carry, wave, lane);
+
     Vec<S, V> graw[N], xraw[N];
     float a[N][V], b[N][V];
     auto fetch = [&](int64_t t0) {

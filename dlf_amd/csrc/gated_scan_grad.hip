@@ -103,6 +103,8 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
         }
     }
 
+    if constexpr (!PARTIAL) share_carry<V, W>(carry, wave, lane);
+
     Vec<S, V> graw[N], dyraw[N], yraw[N], xraw[N];
     float a[N][V], d[N][V], keep[N][V], side[N][V];
     // Position i0 + i: the state before it is the next position's, for the axis's last one `initial`.
