@@ -166,21 +166,12 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float c = entering[v] = carry[v], mine = carry[v];
-            double far = product[v];
 #pragma unroll
             for (int w = 0; w < W; ++w) {
                 if (w == wave) mine = c;
                 const float wa = lds[parity][w][lane][2 * v];
                 c = fmaf(wa, c, lds[parity][w][lane][2 * v + 1]);
-                if constexpr (PARTIAL) far *= static_cast<double>(wa);
-            }
-            if constexpr (PARTIAL) {
-                if (!in_range(far)) {
-                    far = product[v];
-#pragma unroll 1
-                    for (int w = 0; w < W; ++w) far = times(far, static_cast<double>(lds[parity][w][lane][2 * v]));
-                }
-                product[v] = far;
+                if constexpr (PARTIAL) product[v] *= static_cast<double>(wa);
             }
             carry[v] = c;
             mu[v] = first[v] = mine;
@@ -281,8 +272,8 @@ __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
         }
     }
     if constexpr (PARTIAL) {
-        // a segment whose state got lost (as in repair_pass) once more, step after step
-        if (wave == 0 && !finite(carry[0])) {
+        // a segment whose state got lost (as in repair_pass) or whose product passed the range once more, step after step
+        if (wave == 0 && !(finite(carry[0]) && in_range(product[0]))) {
             float state = 0.0f;
             double far = 1.0;
             for (int64_t t = top - begin; t > top - end; --t) {
