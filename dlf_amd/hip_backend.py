@@ -223,6 +223,8 @@ class HipBackend:
             raise RuntimeError("no HIP device visible to PyTorch")
         self.torch = torch
         self.device = torch.device(device)
+        if self.device.index is None:            # "cuda": the current one, from here on
+            self.device = torch.device(self.device.type, torch.cuda.current_device())
         self.lib = load_library()
         self._scratch = None
         self._retired = []
