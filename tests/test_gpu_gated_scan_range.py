@@ -8,7 +8,7 @@ import pytest
 import sequence_oracle as O
 from dlf_amd import frontend as F
 from dlf_amd.frontend import Tensor
-from test_gpu_gated_scan import back, columns, state
+from test_gpu_gated_scan import back, columns, state, stored
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +105,38 @@ def test_a_gate_of_nan_shows(hip_backend, extents, axis, reverse, kind):
         got, want = run_grad(hip_backend, kind, "f32", full, zeros, 0.0, axis, reverse)
         for a, b in zip(got, want):
             assert np.array_equal(np.isnan(a), np.isnan(b)), at
+
+
+@pytest.mark.parametrize("extents,axis", LAYOUTS + [((37, 131072), 0), ((16, 4100), 0)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_neighbours_of_such_a_row_keep_their_bits(hip_backend, extents, axis, dtype):
+    # every seventh row leaves fp32's range within a pass (or fp64's in a product), the others are ordinary: they give what
+    # they give beside ordinary rows, and the same when the states are written over the inputs
+    n = extents[axis]
+    ordinary = stored("gated", 31, extents, dtype, gate=True), stored("gated", 32, extents, dtype)
+    rows = int(np.prod(extents)) // n
+    kept = extents[:axis] + extents[axis + 1:]
+    far = (np.arange(rows) % 7 == 3).reshape(kept)
+    t = (np.arange(n) + 5) % 40
+    g = along(np.where(t == 0, 0.0, np.where(t <= 10, 2.0 ** 20, 64.0)), extents, axis, False)
+    x = along(np.where((t == 0) & (np.arange(n) % 80 < 40), 2.0 ** -300, 0.0), extents, axis, False)      # (0 in both types)
+    mask = np.expand_dims(far, axis)
+    wild = np.where(mask, O.store(g, dtype), ordinary[0]), np.where(mask, O.store(x, dtype), ordinary[1])
+    dY = Tensor.from_numpy(hip_backend, stored("gated", 33, extents, dtype))
+    results = []
+    for G, X in (ordinary, wild):
+        G, X = Tensor.from_numpy(hip_backend, G), Tensor.from_numpy(hip_backend, X)
+        Y, L = F.gated_scan(G, X, axis, "gated")
+        grads = F.gated_scan_grad(G, None, Y, dY, axis, "gated")
+        hip_backend.synchronize()
+        results.append([v.numpy() for v in (Y, L) + tuple(grads)])
+        over, last = F.gated_scan(G, X, axis, "gated", out=X)
+        hip_backend.synchronize()
+        assert over.numpy().tobytes() == results[-1][0].tobytes() and last.numpy().tobytes() == results[-1][1].tobytes()
+    near = ~far
+    for a, b in zip(*results):
+        a, b = (np.moveaxis(v, axis, 0) if v.shape == tuple(extents) else v[None] for v in (a.view(np.uint16) if a.dtype == O.TYPES["bf16"] else a,
+                                                                                           b.view(np.uint16) if b.dtype == O.TYPES["bf16"] else b))
+        assert np.array_equal(a[:, near], b[:, near])
+    y = np.moveaxis(O.load(results[1][0]), axis, 0)
+    assert (y[:, far] == 0).all()
