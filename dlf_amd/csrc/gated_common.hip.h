@@ -69,13 +69,13 @@ __device__ __forceinline__ Stretch join(const Stretch& first, const Stretch& the
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= std::numeric_limits<float>::max(); }
 
-// A product of a lane's gates that fp32 does not hold, once more in 64 bits.
+// The product of a lane's gates, in 64 bits where fp32 did not hold it.
 template <int N>
-__device__ __forceinline__ double product_of(const float (&a)[N]) {
+__device__ __forceinline__ double product_of(float in_fp32, const float (&a)[N]) {
     double p = a[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) p = times(p, static_cast<double>(a[i]));
-    return p;
+    return finite(in_fp32) ? static_cast<double>(in_fp32) : p;
 }
 
 // V neighbouring elements at base + off bytes.  The base is the same for the whole wavefront and the
@@ -196,9 +196,10 @@ __device__ __forceinline__ void store_run(S* row, int64_t i0, int64_t end, const
 }
 
 // The stretches of a group of G lanes (4, 16, 32 or 64, in order) joined from the group's first lane up
-// to each; `before` is what lies before the lane, `all` the whole group's.
-template <int G>
-__device__ __forceinline__ void join_lanes(const Stretch& own, Stretch& before, Stretch& all) {
+// to each; `before` is what lies before the lane, `all` the whole group's.  again(): the lane's product in 64 bits,
+// where fp32 did not hold it.
+template <int G, typename Again>
+__device__ __forceinline__ void join_lanes(const Stretch& own, Stretch& before, Stretch& all, Again&& again) {
     const int lane = lane_id();
     Stretch s = own;
     auto step = [&](double pa, float pb, bool mine) {
@@ -216,9 +217,10 @@ __device__ __forceinline__ void join_lanes(const Stretch& own, Stretch& before, 
     if constexpr (G >= 32) step(dpp_fetch<kRowBcast15, 0xa>(s.a, 1.0), dpp_fetch<kRowBcast15, 0xa>(s.b, 0.0f), true);
     if constexpr (G >= 64) step(dpp_fetch<kRowBcast31, 0xc>(s.a, 1.0), dpp_fetch<kRowBcast31, 0xc>(s.b, 0.0f), true);
     // a product that passed the range left its mark on all lanes behind it: an infinity, or the NaN that it and a 0
-    // make.  Groups of lanes with such a mark once more, by products that stay in range.
+    // make; one that passed fp32 in a lane's own steps is marked so already.  Groups of lanes with such a mark once
+    // more, by products that stay in range.
     if (const uint64_t far = __ballot(!in_range(s.a))) {
-        Stretch f = own;
+        Stretch f = {again(), own.b};
 #pragma unroll 1
         for (int d = 1; d < G; d <<= 1) {
             const Stretch first = {lane_get(f.a, (lane - d) & (kWave - 1)), lane_get(f.b, (lane - d) & (kWave - 1))};
@@ -242,7 +244,7 @@ __device__ __forceinline__ float enter_segment(const Stretch* records, int64_t m
         if (s < count) mine = join(mine, records[s * m + r]);
     }
     Stretch before, all;
-    join_lanes<kWave>(mine, before, all);
+    join_lanes<kWave>(mine, before, all, [&] { return mine.a; });
     return through(all, state);
 }
 

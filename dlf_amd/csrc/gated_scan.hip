@@ -323,12 +323,8 @@ __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_rows(ScanCall<S
             pa *= a[i];
             pb = fmaf(a[i], pb, b[i]);
         }
-        Stretch own = {pa, pb}, before, all;
-        if (__any(!finite(pa))) {
-            const double p = product_of(a);
-            if (!finite(pa)) own.a = p;
-        }
-        join_lanes<G>(own, before, all);
+        Stretch before, all;
+        join_lanes<G>({pa, pb}, before, all, [&] { return product_of(pa, a); });
         float h = carry;
         if constexpr (W > 1) {
             if (lane_id() == 0) lds[parity][team][wave] = all;

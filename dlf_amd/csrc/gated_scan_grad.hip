@@ -390,12 +390,8 @@ __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_grad_rows(GradC
             pa *= a[i];
             pb = a[i] * (d[i] + pb);
         }
-        Stretch own = {pa, pb}, before, all;
-        if (__any(!finite(pa))) {
-            const double p = product_of(a);
-            if (!finite(pa)) own.a = p;
-        }
-        join_lanes<G>(own, before, all);
+        Stretch before, all;
+        join_lanes<G>({pa, pb}, before, all, [&] { return product_of(pa, a); });
         float mu = carry;
         if constexpr (W > 1) {
             if (lane_id() == 0) lds[parity][team][wave] = all;
