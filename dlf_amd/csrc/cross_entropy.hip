@@ -6,9 +6,10 @@
 //     maximum and sum go over the workgroup, the gradient leaves from the registers; a register that
 //     has been stored takes the next row's elements at once, so loads and stores overlap.
 //   * Everything else is cut into tiles of a row: a tile leaves its maximum and sum (a record, or the
-//     row's result where it has one tile), and the gradient of a tile folds the row's few records.
-// bf16 [8192, 128000], loss and gradient: 803 us (5.3 TB/s); fp16 [4096, 8192] pieces: 18.9 us a state (3.6 TB/s), 25.6 a
-// gradient (5.2 TB/s); loss of fp32 [64, 32000]: 6.1 us.
+//     row's result where it has one tile), and the gradient of a tile folds the row's records.
+// bf16 [8192, 128000], loss and gradient: 799 us (5.3 TB/s), loss alone 308 (6.8); [8192, 151936], rows too long for a
+// workgroup's registers, which are read twice: 1191 us (6.3 TB/s of three crossings), loss alone 363 (6.9).  fp16
+// [4096, 8192] pieces: 17.7 us a state (3.8 TB/s), 24.1 a gradient (5.6 TB/s).  Loss of fp32 [64, 32000]: 6.4 us.
 // Sums and maxima are fp32; exponentials are the hardware's 2^x of (x - maximum) log2(e), where the
 // difference comes first: it is exact for neighbours, whatever the logits' common offset.  An fp32 gradient's own
 // exponentials are exact to the function's error (scaled_exp); a sum is not nearer to 64 bits for it.

@@ -17,7 +17,7 @@ struct ScanCall {
     float* entering;        // m states (cut calls)
 };
 
-// A short axis: one lane per row, step after step.  A decoding step, bf16 [48, 1, 2560]: 4.9 us, a launch's latency.
+// A short axis: one lane per row, step after step.  A decoding step, bf16 [48, 1, 2560]: 5.1 us, a launch's latency.
 template <typename S, int KIND>
 __global__ __launch_bounds__(256) void gated_walk(ScanCall<S> p) {
     const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -46,7 +46,7 @@ constexpr int kSteps = 16;       // of a wavefront in a pass
 // work over, value for value.
 // PARTIAL: only what the segment does to the state, for the segments behind it.
 // Bound by HBM, short of it by passes that join at a barrier while the VALU is half busy: bf16 [8, 4096, 2048] blend
-// 92 us (4.4 TB/s; a workgroup per CU), [64, 4096, 512] 158 us (5.1 TB/s), fp32 [8, 4096, 2048] 155 us (5.2 TB/s);
+// 91 us (4.4 TB/s; a workgroup per CU), [64, 4096, 512] 156 us (5.2 TB/s), fp32 [8, 4096, 2048] 154 us (5.2 TB/s);
 // cut, fp32 [1, 65536, 1000] 121 + 148 us (4.4 and 5.4 TB/s of what the two launches move).
 template <typename S, int KIND, int V, int W, typename OFF, bool NT, bool PARTIAL>
 __global__ __launch_bounds__(W * kWave) void gated_cols(ScanCall<S> p) {
@@ -268,8 +268,9 @@ int launch_cols(ScanCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t 
 
 // Rows along memory: G lanes (4, 16, 32 or 64) or W wavefronts per row, a run of consecutive steps to a
 // lane; the lanes' stretches are joined by DPP, the wavefronts' through LDS, pass after pass.  Bound by HBM:
-// bf16 [16384, 4096] 78 us (5.1 TB/s), [1000000, 64] 71 us (5.4 TB/s), fp16 [6144, 5001] 42 us (4.4 TB/s: rows start
-// on odd elements, so 16-byte accesses span lines).
+// bf16 [16384, 4096] 77 us (5.2 TB/s), [1000000, 64] 72 us (5.3 TB/s), fp16 [6144, 5001] 43 us (4.3 TB/s: the loads of
+// the last, shorter pass wait behind the stores of the one before; calls of [6144, 5120] 42.4 us, five whole passes, of
+// [6144, 5000] 45.6, on even elements or odd).
 template <typename S, int KIND, int G, int W, int DIR, bool PARTIAL>
 __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_rows(ScanCall<S> p) {
     static_assert(W == 1 || G == kWave, "whole wavefronts share a row");

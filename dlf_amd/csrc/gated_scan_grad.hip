@@ -56,8 +56,8 @@ constexpr int kGradSteps = 8;       // of a wavefront in a pass
 
 // Rows side by side, as in the forward kernel, from the last step to the first: position i of the
 // walk is step n - 1 - i.  Eight steps a pass: four inputs of them and two outputs fill the registers.
-// Bound by HBM as the forward kernel: bf16 [8, 4096, 2048] sigmoid 144 us (4.7 TB/s), blend 171 us (4.7), [64, 4096, 512]
-// 316 us (5.1); fp32 [3, 1777, 515], cut, 11.4 + 22.5 us (latency: a pass or two by 176 workgroups).
+// Bound by HBM as the forward kernel: bf16 [8, 4096, 2048] sigmoid 147 us (4.6 TB/s), blend 173 us (4.7), [64, 4096, 512]
+// 316 us (5.1); fp32 [3, 1777, 515], cut, 11.3 + 21.8 us (latency: a pass or two by 176 workgroups).
 template <typename S, int KIND, int V, int W, typename OFF, bool NT, bool PARTIAL>
 __global__ __launch_bounds__(W * kWave) void gated_grad_cols(GradCall<S> p) {
     constexpr int N = kGradSteps;
@@ -317,7 +317,7 @@ int launch_cols(GradCall<S> p, void* scratch, size_t scratch_bytes, hipStream_t 
 }
 
 // Rows along memory, as in the forward kernel, from the last step to the first; DIR is the direction
-// of the walk in memory.  bf16 [16384, 4096] 140 us (4.8 TB/s), fp32 [1000000, 64] 238 us (5.4 TB/s).
+// of the walk in memory.  bf16 [16384, 4096] 139 us (4.8 TB/s), fp32 [1000000, 64] 236 us (5.4 TB/s).
 template <typename S, int KIND, int G, int W, int DIR, bool PARTIAL>
 __global__ __launch_bounds__(W > 4 ? W * kWave : 256) void gated_grad_rows(GradCall<S> p) {
     static_assert(W == 1 || G == kWave, "whole wavefronts share a row");
