@@ -45,10 +45,11 @@ __device__ __forceinline__ float exp_diff(float x, float mx) { return __builtin_
 template <typename S>
 __device__ __forceinline__ float scaled_exp(float factor, float x, float mx) {
     if constexpr (sizeof(S) == 4) {
-        const float d = fmaxf(x - mx, -200.0f);            // (exp(d) is 0 long before; of -inf nothing would be left to make up)
-        const float t = d * kLog2E;
+        const float d = x - mx, t = d * kLog2E;
         const float v = factor * __builtin_amdgcn_exp2f(t);
-        return fmaf(v, fmaf(-t, 0.693147180559945309417f, d), v);
+        // (under 2^-16 wherever exp(d) is not 0; far below and of -inf any number will do, and a NaN is in v as well)
+        const float left = __builtin_amdgcn_fmed3f(fmaf(-t, 0.693147180559945309417f, d), -0x1p-16f, 0x1p-16f);
+        return fmaf(v, left, v);
     } else {
         return factor * exp_diff(x, mx);
     }
