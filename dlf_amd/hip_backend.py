@@ -262,7 +262,8 @@ class HipBackend:
         for e in reversed(shape.extents):
             dense.insert(0, size)
             size *= e
-        self.copy(_dtype_code_of(storage.dtype, self.torch), shape.extents, storage, shape.offset, shape.strides, out, 0, dense)
+        self._call(self.lib.dlfx_copy, "dlfx_copy", _dtype_code_of(storage.dtype, self.torch), len(shape.extents), _arr(shape.extents),
+                   storage.data_ptr(), shape.offset, _arr(shape.strides), out.data_ptr(), 0, _arr(dense))
         return out
 
     def copy(self, dtype, extents, x, x_offset, x_strides, y, y_offset, y_strides, defer=False):
